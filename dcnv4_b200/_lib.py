@@ -42,6 +42,9 @@ _SIGNATURES = {
     "dcnv4b200_linear_pair_fwd": (_i, [_p, _p, _p, _p, _i, _p, _i, _i, C.c_longlong, _i, _p]),
     "dcnv4b200_fwd_fused_offset": (_i, [_p] * 5 + [_i] * 8 + [_f, _p]),
     "dcnv4b200_linear_ln_fwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _p, _i, C.c_longlong, _i, _i, _p]),
+    "dcnv4b200_layernorm_train_fwd": (_i, [_p] * 10 + [_i] * 4 + [C.c_longlong, _i, C.c_longlong, _f, _i, _p]),
+    "dcnv4b200_layernorm_train_bwd_workspace_bytes": (_z, [_i, C.c_longlong, _i]),
+    "dcnv4b200_layernorm_train_bwd": (_i, [_p] * 15 + [_z] + [_i] * 4 + [C.c_longlong, _i, C.c_longlong, _i, _p]),
     "dcnv4b200_device_status": (_i, [C.POINTER(_i)]),
     "dcnv4b200_bwd_static_scratch_max_elements": (_z, []),
     "dcnv4b200_bwd_static_scratch": (_i, [_p] * 5 + [_i] + _DCN_SCALARS + [_p]),

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "layernorm_train.cuh"
 
 using namespace dcnb200;
 
@@ -268,8 +269,8 @@ const char* dcnv4b200_strerror(int code) {
     case DCNV4B200_ERR_ALIGN: return "pointer not 16-byte aligned";
     case DCNV4B200_ERR_WORKSPACE: return "workspace missing or smaller than *_bwd_workspace_bytes()";
     case DCNV4B200_ERR_UNSUPPORTED:
-      return "outside the supported parameter space (more than 8 levels, or one query's packed row "
-             "exceeds the shared-memory staging budget)";
+      return "outside the supported parameter space (more than 8 levels, one query's packed row "
+             "exceeds the shared-memory staging budget, or a size or option this entry point does not cover)";
     case DCNV4B200_ERR_PADDED_DIM: return "padded_offset_dim must be a multiple of 8 and >= 3*K*group";
     case DCNV4B200_ERR_CHANNELS: return "group_channels must be a multiple of 4 (fp32) or 8 (fp16/bf16)";
     case DCNV4B200_ERR_TOO_LARGE: return "tensor too large for 31-bit indexing";
@@ -432,6 +433,95 @@ int dcnv4b200_layernorm_act_fwd(const void* x, const void* gamma, const void* be
   if (int rc = status_ptr(&status, &sms)) return rc;
   return (int)launch_layernorm_fwd(dtype, param_dtype, x, gamma, beta, y, rows, C, eps, activation, sms,
                                    static_cast<cudaStream_t>(stream));
+}
+
+// Checks the two LayerNorm training passes share; fills the arguments they have in common.
+static int fill_ln_train(LnTrainArgs& a, const void* weight, const void* bias, const void* layer_scale,
+                         const float* sample_scale, int mode, int dtype, int out_dtype, int param_dtype,
+                         long long rows, int C, long long rows_per_sample, int activation) {
+  if (mode < DCNV4B200_LN_PLAIN || mode > DCNV4B200_LN_PRE) return DCNV4B200_ERR_UNSUPPORTED;
+  if (activation != DCNV4B200_ACT_NONE && (activation != DCNV4B200_ACT_GELU || mode != DCNV4B200_LN_PLAIN))
+    return DCNV4B200_ERR_UNSUPPORTED;
+  if (!dtype_ok(dtype) || (out_dtype != dtype && out_dtype != DCNV4B200_F32) ||
+      (param_dtype != dtype && param_dtype != DCNV4B200_F32))
+    return DCNV4B200_ERR_DTYPE;
+  if (rows < 0 || C <= 0) return DCNV4B200_ERR_SHAPE;
+  if (C > ln_train_max_channels()) return DCNV4B200_ERR_UNSUPPORTED;
+  if (rows >= (1LL << 31)) return DCNV4B200_ERR_TOO_LARGE;
+  if (sample_scale && (rows_per_sample <= 0 || rows % rows_per_sample != 0)) return DCNV4B200_ERR_SHAPE;
+  const uintptr_t pa = (param_dtype == DCNV4B200_F32 ? 4 : 2) - 1;
+  if (((uintptr_t)weight | (uintptr_t)bias | (uintptr_t)layer_scale) & pa || (uintptr_t)sample_scale & 3)
+    return DCNV4B200_ERR_ALIGN;
+  a = LnTrainArgs{};
+  a.w = weight; a.b = bias; a.gamma = mode == DCNV4B200_LN_POST ? layer_scale : nullptr;
+  a.s = mode == DCNV4B200_LN_PLAIN ? nullptr : sample_scale;
+  a.rows = (int)rows; a.C = C; a.param_f32 = param_dtype == DCNV4B200_F32;
+  a.rows_per_sample = (unsigned)(sample_scale ? rows_per_sample : 1);
+  return 0;
+}
+static inline bool element_aligned(const void* p, int dtype) { return ((uintptr_t)p & (elem_size(dtype) - 1)) == 0; }
+
+int dcnv4b200_layernorm_train_fwd(const void* x, const void* residual, const void* weight, const void* bias,
+                                  const void* layer_scale, const float* sample_scale, void* y, void* h, float* mean,
+                                  float* rstd, int mode, int dtype, int out_dtype, int param_dtype, long long rows,
+                                  int C, long long rows_per_sample, float eps, int activation, void* stream) {
+  LnTrainArgs a;
+  if (int rc = fill_ln_train(a, weight, bias, layer_scale, sample_scale, mode, dtype, out_dtype, param_dtype, rows, C,
+                             rows_per_sample, activation))
+    return rc;
+  if (rows == 0) return 0;
+  if (!x || !weight || !bias || !y || !mean || !rstd || (mode != DCNV4B200_LN_PLAIN && !residual) ||
+      (mode == DCNV4B200_LN_PRE && !h))
+    return DCNV4B200_ERR_NULL;
+  if (!element_aligned(x, dtype) || !element_aligned(residual, out_dtype) || !element_aligned(y, out_dtype) ||
+      !element_aligned(h, out_dtype) || !element_aligned(mean, DCNV4B200_F32) || !element_aligned(rstd, DCNV4B200_F32))
+    return DCNV4B200_ERR_ALIGN;
+  a.x = x; a.res = residual; a.y = y; a.h = h; a.mean = mean; a.rstd = rstd; a.eps = eps;
+  return (int)launch_ln_train_fwd(mode, activation, dtype, out_dtype, a, static_cast<cudaStream_t>(stream));
+}
+
+size_t dcnv4b200_layernorm_train_bwd_workspace_bytes(int dtype, long long rows, int C) {
+  if (!dtype_ok(dtype) || rows <= 0 || rows >= (1LL << 31) || C <= 0 || C > ln_train_max_channels()) return 0;
+  return ln_train_workspace_bytes(dtype, (int)rows, C);
+}
+
+int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const void* x, const float* mean,
+                                  const float* rstd, const void* weight, const void* bias, const void* layer_scale,
+                                  const float* sample_scale, void* grad_x, void* grad_branch, void* grad_weight,
+                                  void* grad_bias, void* grad_layer_scale, void* workspace, size_t workspace_bytes,
+                                  int mode, int dtype, int out_dtype, int param_dtype, long long rows, int C,
+                                  long long rows_per_sample, int activation, void* stream) {
+  LnTrainArgs a;
+  if (int rc = fill_ln_train(a, weight, bias, layer_scale, sample_scale, mode, dtype, out_dtype, param_dtype, rows, C,
+                             rows_per_sample, activation))
+    return rc;
+  if (!grad_weight || !grad_bias || (a.gamma && !grad_layer_scale)) return DCNV4B200_ERR_NULL;
+  if (!element_aligned(grad_weight, param_dtype) || !element_aligned(grad_bias, param_dtype) ||
+      !element_aligned(grad_layer_scale, param_dtype))
+    return DCNV4B200_ERR_ALIGN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    const size_t n = (size_t)C * elem_size(param_dtype);
+    cudaError_t e = cudaMemsetAsync(grad_weight, 0, n, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(grad_bias, 0, n, s);
+    if (e == cudaSuccess && a.gamma) e = cudaMemsetAsync(grad_layer_scale, 0, n, s);
+    return (int)e;
+  }
+  if (!grad_y || !x || !mean || !rstd || !weight || !bias || !grad_x) return DCNV4B200_ERR_NULL;
+  const bool pre = mode == DCNV4B200_LN_PRE;
+  if (pre && !grad_branch && (sample_scale || dtype != out_dtype)) return DCNV4B200_ERR_NULL;
+  if (!element_aligned(grad_y, out_dtype) || !element_aligned(grad_h, out_dtype) ||
+      !element_aligned(x, pre ? out_dtype : dtype) || !element_aligned(grad_x, pre ? out_dtype : dtype) ||
+      !element_aligned(grad_branch, dtype) || !aligned16(workspace) || !element_aligned(mean, DCNV4B200_F32) ||
+      !element_aligned(rstd, DCNV4B200_F32))
+    return DCNV4B200_ERR_ALIGN;
+  if (!workspace || workspace_bytes < ln_train_workspace_bytes(dtype, (int)rows, C)) return DCNV4B200_ERR_WORKSPACE;
+  if (pre) a.h = const_cast<void*>(x);
+  else a.x = x;
+  a.gy = grad_y; a.gh = pre ? grad_h : nullptr; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+  a.dx = grad_x; a.dx2 = pre ? grad_branch : nullptr; a.partial = static_cast<float*>(workspace);
+  a.dw = grad_weight; a.db = grad_bias; a.dgamma = grad_layer_scale;
+  return (int)launch_ln_train_bwd(mode, activation, dtype, out_dtype, a, s);
 }
 
 int dcnv4b200_center_scale_blend_fwd(const void* x, const void* x_proj, const void* weight, const void* bias,

@@ -504,6 +504,12 @@ inline cudaError_t persistent_ctas_per_sm(size_t smem, int* per_sm) {
 cudaError_t launch_layernorm_fwd(int dtype, int param_dtype, const void* x, const void* gamma, const void* beta,
                                  void* y, long long rows, int C, float eps, int act, int sm_count, cudaStream_t s);
 int layernorm_max_channels(int dtype);
+// LayerNorm training passes (layernorm_train.cu); xd / yd: types of the branch input and of residual / result.
+struct LnTrainArgs;
+cudaError_t launch_ln_train_fwd(int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s);
+cudaError_t launch_ln_train_bwd(int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s);
+size_t ln_train_workspace_bytes(int xd, int rows, int C);
+int ln_train_max_channels();
 
 // out = x*(1 - s) + x_proj*s with s = sigmoid(x . weight^T + bias) per row and group (center_scale.cu).
 cudaError_t launch_center_scale_blend(int dtype, int param_dtype, const void* x, const void* xp, const void* w,

@@ -1,0 +1,10 @@
+// LayerNorm training kernels for one pair of tensor types (see layernorm_train.cuh).
+#include "layernorm_train.cuh"
+
+namespace dcnb200 {
+
+cudaError_t ln_train_run_f16_f16(bool backward, int mode, int act, bool vec_ok, const LnTrainArgs& a, cudaStream_t s) {
+  return ln::run<__half, __half>(backward, mode, act, vec_ok, a, s);
+}
+
+}  // namespace dcnb200

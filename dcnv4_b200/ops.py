@@ -234,6 +234,173 @@ def layer_norm_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
         and x.data_ptr() % 16 == 0
 
 
+# LayerNorm training passes ---------------------------------------------------------------------------------
+
+LAYER_NORM_MAX_CHANNELS = 8192
+_LN_PLAIN, _LN_POST, _LN_PRE = 0, 1, 2
+
+
+def layer_norm_train_supported(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> bool:
+    """True when the LayerNorm training passes cover this input (dtypes, size, layout)."""
+    return (x.is_cuda and x.is_contiguous() and x.dtype in _DTYPES and x.dim() > 0
+            and 0 < x.shape[-1] <= LAYER_NORM_MAX_CHANNELS and x.numel() // x.shape[-1] < 2 ** 31
+            and weight is not None and weight.is_cuda and weight.is_contiguous()
+            and weight.dtype in (torch.float32, x.dtype) and out_dtype in (None, torch.float32, x.dtype))
+
+
+def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
+    """Argument checks of the training passes; returns (rows, C, rows_per_sample).  `x_dtype` is the dtype of the
+    branch input (x itself, except in the backward pass over a stored sum)."""
+    C = x.shape[-1] if x.dim() else 0
+    for t, n in ((x, "input"), (weight, "weight"), (bias, "bias"), (layer_scale, "layer_scale"),
+                 (sample_scale, "sample_scale")):
+        if t is not None:
+            _check_tensor(t, n)
+            if t.device != x.device:
+                raise RuntimeError(f"{n} must be on the device of the input")
+    _code(x)
+    if x_dtype not in _DTYPES:
+        raise RuntimeError(f"dcnv4_b200 supports float32/float16/bfloat16 tensors, got {x_dtype}")
+    if out_dtype not in (torch.float32, x_dtype):
+        raise RuntimeError("the result must have the dtype of the input or be float32")
+    if C == 0:
+        raise RuntimeError("the last dimension must not be empty")
+    for t, n in ((weight, "weight"), (bias, "bias"), (layer_scale, "layer_scale")):
+        if t is not None and (t.numel() != C or t.dtype != weight.dtype):
+            raise RuntimeError(f"{n} must have the size of the last dimension and the dtype of weight")
+    if weight.dtype not in (torch.float32, x_dtype):
+        raise RuntimeError("parameters must have the dtype of the input or be float32")
+    for t, n in others:
+        if t is not None:
+            _check_tensor(t, n)
+            if t.shape != x.shape or t.dtype != out_dtype or t.device != x.device:
+                raise RuntimeError(f"{n} must have the shape of the input, dtype {out_dtype}, and its device")
+    rows = x.numel() // C
+    per = rows
+    if sample_scale is not None:
+        n = sample_scale.numel()
+        if sample_scale.dtype != torch.float32 or x.dim() < 2 or (x.shape[0] % n if n else x.shape[0]) != 0:
+            raise RuntimeError("sample_scale must be float32 with one factor per sample (its size divides the first "
+                               "dimension of the input)")
+        per = max(rows // n, 1) if n else 1
+    return rows, C, per
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _ln_forward(mode, x, residual, weight, bias, eps, layer_scale, sample_scale, activation, out_dtype, what):
+    rows, C, per = _check_ln(x, x.dtype, weight, bias, ((residual, "residual"),), layer_scale, sample_scale, out_dtype)
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    h = torch.empty_like(y) if mode == _LN_PRE else None
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    with torch.cuda.device(x.device):
+        rc = _lib.lib().dcnv4b200_layernorm_train_fwd(
+            x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale),
+            y.data_ptr(), _ptr(h), mean.data_ptr(), rstd.data_ptr(), mode, _code(x), _DTYPES[out_dtype], _code(weight),
+            rows, C, per, float(eps), 1 if activation == "gelu" else 0, _stream(x))
+    _lib.check(rc, what)
+    return y, h, mean, rstd
+
+
+def _ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale, sample_scale, activation, x_dtype,
+                 what):
+    out_dtype = grad_y.dtype
+    pre = mode == _LN_PRE
+    grads = ((grad_y, "grad_y"), (grad_h, "grad_h")) + (((x, "h"),) if pre else ())
+    rows, C, per = _check_ln(x, x_dtype, weight, bias, grads, layer_scale, sample_scale, out_dtype)
+    for t, n in ((mean, "mean"), (rstd, "rstd")):
+        _check_tensor(t, n)
+        if t.dtype != torch.float32 or t.numel() != rows or t.device != x.device:
+            raise RuntimeError(f"{n} must be the float32 row statistics the forward pass returned")
+    lib = _lib.lib()
+    code = _DTYPES[x_dtype]
+    grad_x = torch.empty_like(x)
+    branch = torch.empty(x.shape, dtype=x_dtype, device=x.device) \
+        if pre and (sample_scale is not None or x_dtype != out_dtype) else None
+    params = torch.empty((2 if layer_scale is None else 3, C), dtype=weight.dtype, device=x.device)
+    ws_bytes = lib.dcnv4b200_layernorm_train_bwd_workspace_bytes(code, rows, C)
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
+    es = params.element_size() * C
+    p0 = params.data_ptr()
+    with torch.cuda.device(x.device):
+        rc = lib.dcnv4b200_layernorm_train_bwd(
+            grad_y.data_ptr(), _ptr(grad_h), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), weight.data_ptr(),
+            bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale), grad_x.data_ptr(), _ptr(branch), p0, p0 + es,
+            None if layer_scale is None else p0 + 2 * es, ws.data_ptr(), ws_bytes, mode, code, _DTYPES[out_dtype],
+            _code(weight), rows, C, per, 1 if activation == "gelu" else 0, _stream(x))
+    _lib.check(rc, what)
+    return (grad_x, branch if branch is not None else grad_x) + params.unbind(0)
+
+
+def layer_norm_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float,
+                             activation: str = "none", out_dtype: Optional[torch.dtype] = None):
+    """LayerNorm over the last dimension of a contiguous CUDA tensor for training: (y, mean, rstd), with y optionally
+    through the exact GELU in the same pass and the fp32 row statistics that `layer_norm_backward` reads.  `out_dtype`
+    is the dtype of x (default) or float32; weight and bias are float32 or have the dtype of x.  Any number of rows,
+    1 to 8192 channels."""
+    if activation not in ("none", "gelu"):
+        raise ValueError("activation must be 'none' or 'gelu'")
+    y, _, mean, rstd = _ln_forward(_LN_PLAIN, x, None, weight, bias, eps, None, None, activation,
+                                   x.dtype if out_dtype is None else out_dtype, "layer_norm_train_forward")
+    return y, mean, rstd
+
+
+def layer_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                        weight: torch.Tensor, bias: torch.Tensor, activation: str = "none"):
+    """(grad_x, grad_weight, grad_bias) of `layer_norm_train_forward`, each in the dtype of what it is the gradient
+    of.  Deterministic."""
+    if activation not in ("none", "gelu"):
+        raise ValueError("activation must be 'none' or 'gelu'")
+    gx, _, gw, gb = _ln_backward(_LN_PLAIN, grad_y, None, x, mean, rstd, weight, bias, None, None, activation,
+                                 x.dtype, "layer_norm_backward")
+    return gx, gw, gb
+
+
+def layer_norm_residual_forward(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
+                                eps: float, layer_scale: Optional[torch.Tensor] = None,
+                                sample_scale: Optional[torch.Tensor] = None):
+    """The tail of a post-norm block in one pass: out = residual + sample_scale * layer_scale * LN(x), returned with
+    the row statistics as (out, mean, rstd).  `layer_scale` (C) like weight; `sample_scale` (N) float32, one factor
+    per sample of the first dimension (stochastic depth: 0 or 1 / keep probability).  out and residual have the dtype
+    of x or are float32."""
+    out, _, mean, rstd = _ln_forward(_LN_POST, x, residual, weight, bias, eps, layer_scale, sample_scale, "none",
+                                     residual.dtype, "layer_norm_residual_forward")
+    return out, mean, rstd
+
+
+def layer_norm_residual_backward(grad_out: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                                 weight: torch.Tensor, bias: torch.Tensor, layer_scale: Optional[torch.Tensor] = None,
+                                 sample_scale: Optional[torch.Tensor] = None):
+    """(grad_x, grad_weight, grad_bias, grad_layer_scale or None) of `layer_norm_residual_forward`; the gradient of
+    the residual is `grad_out` itself.  Deterministic."""
+    g = _ln_backward(_LN_POST, grad_out, None, x, mean, rstd, weight, bias, layer_scale, sample_scale, "none", x.dtype,
+                     "layer_norm_residual_backward")
+    return g[0], g[2], g[3], (g[4] if layer_scale is not None else None)
+
+
+def add_layer_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
+                           eps: float, sample_scale: Optional[torch.Tensor] = None):
+    """The seam of two pre-norm branches in one pass: h = residual + sample_scale * x and y = LN(h), returned as
+    (h, y, mean, rstd).  Statistics and y are taken of the fp32 sum, before h is rounded.  Types and `sample_scale`
+    as `layer_norm_residual_forward`."""
+    y, h, mean, rstd = _ln_forward(_LN_PRE, x, residual, weight, bias, eps, None, sample_scale, "none",
+                                   residual.dtype, "add_layer_norm_forward")
+    return h, y, mean, rstd
+
+
+def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor], h: torch.Tensor, mean: torch.Tensor,
+                            rstd: torch.Tensor, weight: torch.Tensor, sample_scale: Optional[torch.Tensor] = None,
+                            x_dtype: Optional[torch.dtype] = None):
+    """(grad_residual, grad_x, grad_weight, grad_bias) of `add_layer_norm_forward`; `grad_h` may be None, `x_dtype` is
+    the dtype of the forward's x (default: that of h).  Without `sample_scale` and with equal dtypes the first two are
+    one tensor.  Deterministic."""
+    return _ln_backward(_LN_PRE, grad_y, grad_h, h, mean, rstd, weight, weight, None, sample_scale, "none",
+                        h.dtype if x_dtype is None else x_dtype, "add_layer_norm_backward")
+
+
 def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                    residual: Optional[torch.Tensor] = None, activation: str = "none") -> torch.Tensor:
     """y = act(x @ weight.T + bias) [+ residual] in one tensor-core kernel (forward only; no

@@ -50,6 +50,11 @@ enum {
 #define DCNV4B200_ACT_NONE 0
 #define DCNV4B200_ACT_GELU 1
 
+/* Where a LayerNorm of the training entry points stands in its block. */
+#define DCNV4B200_LN_PLAIN 0 /* y = act(LN(x))                                       */
+#define DCNV4B200_LN_POST 1  /* y = residual + sample_scale * layer_scale * LN(x)    */
+#define DCNV4B200_LN_PRE 2   /* h = residual + sample_scale * x, y = LN(h)           */
+
 /* Version of this ABI (DCNV4B200_ABI_VERSION of the build). */
 int dcnv4b200_abi_version(void);
 
@@ -173,6 +178,50 @@ int dcnv4b200_layernorm_fwd(const void* x, const void* gamma, const void* beta, 
  */
 int dcnv4b200_layernorm_act_fwd(const void* x, const void* gamma, const void* beta, void* y, int dtype,
                                 int param_dtype, long long rows, int C, float eps, int activation, void* stream);
+
+/*
+ * LayerNorm training passes over the last dimension of a channels-last tensor.  The reference runs these norms,
+ * the layer-scale product, stochastic depth and the residual addition as separate PyTorch kernels
+ * (classification/models/flash_intern_image.py:34-56, :414-432) and has no kernel of its own.
+ *
+ * Forward; `mode` is one of DCNV4B200_LN_*; LN(v) = (v - mean) * rstd * weight + bias:
+ *   x            (rows, C) in `dtype`: the normalised tensor (PLAIN, POST) or the branch that is added (PRE)
+ *   residual     (rows, C) in `out_dtype` (POST, PRE; NULL for PLAIN)
+ *   weight, bias, layer_scale (C) in `param_dtype`; layer_scale may be NULL and is read by POST alone
+ *   sample_scale (rows / rows_per_sample) fp32 or NULL: one factor per sample (stochastic depth; POST, PRE)
+ *   y            (rows, C) in `out_dtype`; h (rows, C) in `out_dtype` (PRE: the sum; statistics and y are taken of the
+ *                sum before it is rounded), NULL otherwise
+ *   mean, rstd   (rows) fp32: the row statistics, kept for the backward pass
+ * `out_dtype` is `dtype` or fp32 (16-bit branches beside an fp32 residual stream, as autocast has them),
+ * `param_dtype` is fp32 or `dtype`.  `activation` may be DCNV4B200_ACT_GELU (erf form) with PLAIN only.
+ * 1 <= C <= 8192, any alignment of rows: tensors and C that fill 16-byte vectors take the wide loads.
+ */
+int dcnv4b200_layernorm_train_fwd(const void* x, const void* residual, const void* weight, const void* bias,
+                                  const void* layer_scale, const float* sample_scale, void* y, void* h, float* mean,
+                                  float* rstd, int mode, int dtype, int out_dtype, int param_dtype, long long rows,
+                                  int C, long long rows_per_sample, float eps, int activation, void* stream);
+
+/* Scratch bytes dcnv4b200_layernorm_train_bwd needs (partial sums of the parameter gradients); 0 for no rows. */
+size_t dcnv4b200_layernorm_train_bwd_workspace_bytes(int dtype, long long rows, int C);
+
+/*
+ * Backward of dcnv4b200_layernorm_train_fwd, same modes, types and limits:
+ *   grad_y       (rows, C) in `out_dtype`; grad_h (rows, C) in `out_dtype` or NULL (PRE: gradient of h)
+ *   x            the forward's x (PLAIN, POST) in `dtype`, or its h in `out_dtype` (PRE)
+ *   grad_x       PLAIN, POST: gradient of x, in `dtype`; PRE: gradient of the residual, in `out_dtype`
+ *   grad_branch  PRE: gradient of the forward's x, in `dtype`, or NULL where it equals grad_x (sample_scale NULL and
+ *                dtype == out_dtype); NULL otherwise
+ *   grad_weight, grad_bias, grad_layer_scale (C) in `param_dtype`; the last one with layer_scale only
+ *   workspace    16-byte aligned, at least dcnv4b200_layernorm_train_bwd_workspace_bytes() bytes
+ * The gradient of POST's residual is grad_y itself.  Everything is fully overwritten; no atomics, results repeat
+ * bit for bit.  With rows == 0 the parameter gradients are zero.
+ */
+int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const void* x, const float* mean,
+                                  const float* rstd, const void* weight, const void* bias, const void* layer_scale,
+                                  const float* sample_scale, void* grad_x, void* grad_branch, void* grad_weight,
+                                  void* grad_bias, void* grad_layer_scale, void* workspace, size_t workspace_bytes,
+                                  int mode, int dtype, int out_dtype, int param_dtype, long long rows, int C,
+                                  long long rows_per_sample, int activation, void* stream);
 
 /*
  * Centre-feature-scale blend of the DCNv4 module, forward, in one pass:
