@@ -45,6 +45,8 @@ _SIGNATURES = {
     "dcnv4b200_layernorm_train_fwd": (_i, [_p] * 10 + [_i] * 4 + [C.c_longlong, _i, C.c_longlong, _f, _i, _p]),
     "dcnv4b200_layernorm_train_bwd_workspace_bytes": (_z, [_i, C.c_longlong, _i]),
     "dcnv4b200_layernorm_train_bwd": (_i, [_p] * 15 + [_z] + [_i] * 4 + [C.c_longlong, _i, C.c_longlong, _i, _p]),
+    "dcnv4b200_newton_schulz_workspace_bytes": (_z, [C.c_longlong, _i, _i]),
+    "dcnv4b200_newton_schulz": (_i, [_p, _p, _p, _z, _i, C.c_longlong, _i, _i, _i, _f, _f, _f, _f, _p]),
     "dcnv4b200_device_status": (_i, [C.POINTER(_i)]),
     "dcnv4b200_bwd_static_scratch_max_elements": (_z, []),
     "dcnv4b200_bwd_static_scratch": (_i, [_p] * 5 + [_i] + _DCN_SCALARS + [_p]),

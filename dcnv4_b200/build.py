@@ -23,7 +23,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 SOURCES = ("api.cu", "dcnv4_fwd.cu", "dcnv4_bwd.cu", "dcnv4_bwd_tiled.cu", "dcnv4_fwd_tiled.cu", "dcnv4_fwd_fused.cu", "fda_fwd.cu", "fda_bwd.cu", "aux.cu", "layernorm.cu",
            "linear.cu", "bias_act.cu", "center_scale.cu", "layernorm_train.cu", "layernorm_train_f32_f32.cu",
            "layernorm_train_f16_f16.cu", "layernorm_train_f16_f32.cu", "layernorm_train_bf16_bf16.cu",
-           "layernorm_train_bf16_f32.cu")
+           "layernorm_train_bf16_f32.cu", "newton_schulz.cu")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 NVCC_FLAGS = ("-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr")
 

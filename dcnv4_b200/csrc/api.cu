@@ -435,6 +435,9 @@ int dcnv4b200_layernorm_act_fwd(const void* x, const void* gamma, const void* be
                                    static_cast<cudaStream_t>(stream));
 }
 
+// Limits of the Newton-Schulz entry point: a side of a matrix, matrices per call (a grid dimension), steps.
+constexpr int kNsMaxSide = 65536, kNsMaxBatch = 65535, kNsMaxSteps = 100;
+
 // Checks the two LayerNorm training passes share; fills the arguments they have in common.
 static int fill_ln_train(LnTrainArgs& a, const void* weight, const void* bias, const void* layer_scale,
                          const float* sample_scale, int mode, int dtype, int out_dtype, int param_dtype,
@@ -522,6 +525,29 @@ int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const 
   a.dx = grad_x; a.dx2 = pre ? grad_branch : nullptr; a.partial = static_cast<float*>(workspace);
   a.dw = grad_weight; a.db = grad_bias; a.dgamma = grad_layer_scale;
   return (int)launch_ln_train_bwd(mode, activation, dtype, out_dtype, a, s);
+}
+
+size_t dcnv4b200_newton_schulz_workspace_bytes(long long batch, int m, int n) {
+  if (batch <= 0 || batch > kNsMaxBatch || m <= 0 || n <= 0 || m > kNsMaxSide || n > kNsMaxSide) return 0;
+  return ns_workspace_bytes(batch, m, n);
+}
+
+int dcnv4b200_newton_schulz(const void* x, void* out, void* workspace, size_t workspace_bytes, int dtype,
+                            long long batch, int m, int n, int steps, float a, float b, float c, float eps,
+                            void* stream) {
+  if (!dtype_ok(dtype)) return DCNV4B200_ERR_DTYPE;
+  if (batch < 0 || m <= 0 || n <= 0 || steps < 1) return DCNV4B200_ERR_SHAPE;
+  if (m > kNsMaxSide || n > kNsMaxSide || batch > kNsMaxBatch || steps > kNsMaxSteps) return DCNV4B200_ERR_UNSUPPORTED;
+  if (batch == 0) return 0;
+  if (!x || !out) return DCNV4B200_ERR_NULL;
+  if (((uintptr_t)x & (elem_size(dtype) - 1)) || ((uintptr_t)out & 1) || !aligned16(workspace))
+    return DCNV4B200_ERR_ALIGN;
+  if (!workspace || workspace_bytes < ns_workspace_bytes(batch, m, n)) return DCNV4B200_ERR_WORKSPACE;
+  int* status = nullptr;
+  int sms = 1;
+  if (int rc = status_ptr(&status, &sms)) return rc;
+  return (int)launch_newton_schulz(dtype, x, out, workspace, batch, m, n, steps, a, b, c, eps, sms, status,
+                                   static_cast<cudaStream_t>(stream));
 }
 
 int dcnv4b200_center_scale_blend_fwd(const void* x, const void* x_proj, const void* weight, const void* bias,

@@ -510,6 +510,10 @@ cudaError_t launch_ln_train_fwd(int mode, int act, int xd, int yd, const LnTrain
 cudaError_t launch_ln_train_bwd(int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s);
 size_t ln_train_workspace_bytes(int xd, int rows, int C);
 int ln_train_max_channels();
+// Newton-Schulz orthogonalisation of a stack of (m, n) matrices (newton_schulz.cu).
+size_t ns_workspace_bytes(long long batch, int m, int n);
+cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* workspace, long long batch, int m, int n,
+                                 int steps, float a, float b, float c, float eps, int sms, int* status, cudaStream_t s);
 
 // out = x*(1 - s) + x_proj*s with s = sigmoid(x . weight^T + bias) per row and group (center_scale.cu).
 cudaError_t launch_center_scale_blend(int dtype, int param_dtype, const void* x, const void* xp, const void* w,

@@ -401,6 +401,35 @@ def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor]
                         h.dtype if x_dtype is None else x_dtype, "add_layer_norm_backward")
 
 
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # the quintic published with the Muon optimiser
+
+
+def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, float, float] = NEWTON_SCHULZ_COEFFICIENTS,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """Orthogonalise a matrix or a stack of matrices (..., m, n) by the quintic Newton-Schulz iteration:
+    X = x / (|x|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T.  Contiguous CUDA tensor in
+    float32 / float16 / bfloat16; the result is a new bfloat16 tensor (its rounding is of the size of the
+    iteration's own error).  No autograd.  Deterministic."""
+    _check_tensor(x, "input")
+    if x.dim() < 2:
+        raise RuntimeError("input must be a matrix or a stack of matrices (..., m, n)")
+    a, b, c = (float(v) for v in coefficients)
+    code = _code(x)
+    m, n = x.shape[-2:]
+    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+    if out.numel() == 0:
+        return out
+    batch = out.numel() // (m * n)
+    L = _lib.lib()
+    ws_bytes = L.dcnv4b200_newton_schulz_workspace_bytes(batch, m, n)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = L.dcnv4b200_newton_schulz(x.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes, code, batch, m, n,
+                                       int(steps), a, b, c, float(eps), _stream(x))
+    _lib.check(rc, "newton_schulz")
+    return out
+
+
 def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                    residual: Optional[torch.Tensor] = None, activation: str = "none") -> torch.Tensor:
     """y = act(x @ weight.T + bias) [+ residual] in one tensor-core kernel (forward only; no

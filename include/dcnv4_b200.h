@@ -224,6 +224,24 @@ int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const 
                                   long long rows_per_sample, int activation, void* stream);
 
 /*
+ * Newton-Schulz orthogonalisation of a stack of matrices, the step of the Muon optimiser:
+ *     X = x / (|x|_F + eps);   `steps` times:  A = X X^T,  X <- a X + (b A + c A A) X      (m <= n; else from the right)
+ * which moves the singular values of x towards 1 and keeps its singular vectors.  The reference has no counterpart
+ * (its trainers use stock optimisers); the product of Linear and convolution weights' updates is its use here.
+ *   x    (batch, m, n) in `dtype` (fp32, fp16, bf16), any alignment;  out (batch, m, n) bf16, not overlapping x
+ *   workspace  16-byte aligned, at least dcnv4b200_newton_schulz_workspace_bytes() bytes, private to calls that may
+ *              overlap on the GPU
+ * m, n <= 65536, batch <= 65535, 1 <= steps <= 100 (DCNV4B200_ERR_UNSUPPORTED / _ERR_SHAPE otherwise).  The iteration
+ * runs on fp16 tensor-core products with fp32 accumulation, with X carried in 22 bits until the last two steps; the
+ * coefficients must keep |X| within fp16's range, as those of the published iteration do.  A zero matrix gives zeros,
+ * a matrix with a NaN gives NaN, other matrices of the stack are not affected.  Results repeat bit for bit.
+ */
+size_t dcnv4b200_newton_schulz_workspace_bytes(long long batch, int m, int n);
+int dcnv4b200_newton_schulz(const void* x, void* out, void* workspace, size_t workspace_bytes, int dtype,
+                            long long batch, int m, int n, int steps, float a, float b, float c, float eps,
+                            void* stream);
+
+/*
  * Centre-feature-scale blend of the DCNv4 module, forward, in one pass:
  *     s[r, g]   = sigmoid(sum_c x[r, c] * weight[g, c] + bias[g])
  *     out[r, c] = x[r, c] * (1 - s[r, c / D]) + x_proj[r, c] * s[r, c / D]

@@ -70,3 +70,31 @@ def test_functions_refuse_cpu_tensors():
         ops.layer_norm_residual_forward(x, x, w, w, 1e-6)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.add_layer_norm_forward(x, x, w, w, 1e-6)
+
+
+def _ns(lib, x=0x1000, out=0x2000, ws=0x4000, ws_bytes=1 << 40, dtype=0, batch=1, m=64, n=64, steps=5):
+    return lib.dcnv4b200_newton_schulz(x, out, ws, ws_bytes, dtype, batch, m, n, steps, 3.4445, -4.775, 2.0315, 1e-7, None)
+
+
+def test_newton_schulz_refuses(lib):
+    assert _ns(lib, dtype=3) == -2
+    assert _ns(lib, batch=-1) == -3 and _ns(lib, m=0) == -3 and _ns(lib, n=0) == -3 and _ns(lib, steps=0) == -3
+    assert _ns(lib, m=65537) == -6 and _ns(lib, batch=65536) == -6 and _ns(lib, steps=101) == -6
+    assert _ns(lib, batch=0) == 0
+    assert _ns(lib, x=None) == -1 and _ns(lib, out=None) == -1
+    assert _ns(lib, x=0x1002) == -4 and _ns(lib, out=0x2001) == -4 and _ns(lib, ws=0x4008) == -4
+    assert _ns(lib, ws=None) == -5 and _ns(lib, ws_bytes=1000) == -5
+
+
+def test_newton_schulz_workspace(lib):
+    need = lib.dcnv4b200_newton_schulz_workspace_bytes
+    assert need(0, 64, 64) == 0 and need(1, 0, 64) == 0 and need(1, 64, 70000) == 0
+    assert need(3, 65, 129) >= 3 * (4 * 65 * 136 + 2 * 65 * 72) * 2
+    assert need(65535, 65536, 65536) > 1 << 47             # no 32-bit overflow
+
+
+def test_newton_schulz_refuses_cpu_tensors():
+    import torch
+    from dcnv4_b200 import ops
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.newton_schulz(torch.zeros(3, 8))
