@@ -459,7 +459,12 @@ static int fill_ln_train(LnTrainArgs& a, const void* weight, const void* bias, c
   a.w = weight; a.b = bias; a.gamma = mode == DCNV4B200_LN_POST ? layer_scale : nullptr;
   a.s = mode == DCNV4B200_LN_PLAIN ? nullptr : sample_scale;
   a.rows = (int)rows; a.C = C; a.param_f32 = param_dtype == DCNV4B200_F32;
-  a.rows_per_sample = (unsigned)(sample_scale ? rows_per_sample : 1);
+  a.rows_per_sample = (unsigned)(sample_scale && rows > 0 ? rows_per_sample : 1);
+  // division by multiplication, exact for numerators below 2^31: ceil(2^(31 + l) / d) with 2^l >= d
+  int l = 0;
+  while ((1u << l) < a.rows_per_sample) ++l;
+  a.per_shift = 31 + l;
+  a.per_mul = ((1ULL << a.per_shift) + a.rows_per_sample - 1) / a.rows_per_sample;
   return 0;
 }
 static inline bool element_aligned(const void* p, int dtype) { return ((uintptr_t)p & (elem_size(dtype) - 1)) == 0; }
@@ -480,6 +485,7 @@ int dcnv4b200_layernorm_train_fwd(const void* x, const void* residual, const voi
       !element_aligned(h, out_dtype) || !element_aligned(mean, DCNV4B200_F32) || !element_aligned(rstd, DCNV4B200_F32))
     return DCNV4B200_ERR_ALIGN;
   a.x = x; a.res = residual; a.y = y; a.h = h; a.mean = mean; a.rstd = rstd; a.eps = eps;
+  if (int rc = status_ptr(&a.status)) return rc;
   return (int)launch_ln_train_fwd(mode, activation, dtype, out_dtype, a, static_cast<cudaStream_t>(stream));
 }
 
@@ -524,6 +530,7 @@ int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const 
   a.gy = grad_y; a.gh = pre ? grad_h : nullptr; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.dx = grad_x; a.dx2 = pre ? grad_branch : nullptr; a.partial = static_cast<float*>(workspace);
   a.dw = grad_weight; a.db = grad_bias; a.dgamma = grad_layer_scale;
+  if (int rc = status_ptr(&a.status)) return rc;
   return (int)launch_ln_train_bwd(mode, activation, dtype, out_dtype, a, s);
 }
 

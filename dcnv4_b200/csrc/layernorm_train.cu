@@ -3,11 +3,11 @@
 
 namespace dcnb200 {
 
-cudaError_t ln_train_run_f32_f32(bool, int, int, bool, const LnTrainArgs&, cudaStream_t);
-cudaError_t ln_train_run_f16_f16(bool, int, int, bool, const LnTrainArgs&, cudaStream_t);
-cudaError_t ln_train_run_f16_f32(bool, int, int, bool, const LnTrainArgs&, cudaStream_t);
-cudaError_t ln_train_run_bf16_bf16(bool, int, int, bool, const LnTrainArgs&, cudaStream_t);
-cudaError_t ln_train_run_bf16_f32(bool, int, int, bool, const LnTrainArgs&, cudaStream_t);
+cudaError_t ln_train_run_f32_f32(bool, int, int, const ln::Plan&, const LnTrainArgs&, cudaStream_t);
+cudaError_t ln_train_run_f16_f16(bool, int, int, const ln::Plan&, const LnTrainArgs&, cudaStream_t);
+cudaError_t ln_train_run_f16_f32(bool, int, int, const ln::Plan&, const LnTrainArgs&, cudaStream_t);
+cudaError_t ln_train_run_bf16_bf16(bool, int, int, const ln::Plan&, const LnTrainArgs&, cudaStream_t);
+cudaError_t ln_train_run_bf16_f32(bool, int, int, const ln::Plan&, const LnTrainArgs&, cudaStream_t);
 
 namespace {
 
@@ -53,51 +53,45 @@ ln_train_params_kernel(const LnTrainArgs a, int mode) {
 
 }  // namespace
 
-// Whether the 16-byte vectors of the wide instantiation may be used: every row of every tensor starts on 16 bytes.
-static bool vectors_ok(int xd, int yd, const LnTrainArgs& a) {
-  const int ex = xd == 0 ? 4 : 2, ey = yd == 0 ? 4 : 2;
-  const int v = xd == 0 ? 4 : 8;
-  if (a.C % v != 0 || (long long)a.C * ex % 16 != 0 || (long long)a.C * ey % 16 != 0) return false;
-  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  return al(a.x) && al(a.res) && al(a.y) && al(a.h) && al(a.gy) && al(a.gh) && al(a.dx) && al(a.dx2);
-}
-
-static ln::Geometry geometry_of(int xd, int C, bool vec) {
-  const int v = xd == 0 ? 4 : 8;
-  return ln::geometry(vec ? C / v : C, !vec, v == 8 ? 3 : 4);
-}
-
 int ln_train_max_channels() { return ln::kMaxChannels; }
 
-// Partial sums of the backward pass: one (2, C) fp32 block per CTA.  The scalar instantiation's grid is the larger
-// one wherever both exist; the workspace covers either.
+// Element sizes of types 0 fp32, 1 fp16, 2 bf16.
+static int size_of(int d) { return d == 0 ? 4 : 2; }
+
+// Alignment decides the kernel: bulk copies want every loaded tensor on 16 bytes, the vector stores every tensor on the
+// size of a lane's vector (32 bytes where a 16-bit branch stands beside fp32 tensors).
+static ln::Plan plan_of(bool backward, int mode, int xd, int yd, const LnTrainArgs& a) {
+  auto on = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  const bool base = on(a.x, 16) && on(a.res, 16) && on(a.h, 16) && on(a.gy, 16) && on(a.gh, 16);
+  const uintptr_t wide = xd != 0 && yd == 0 ? 32 : 16;
+  const bool vec = on(a.y, wide) && on(a.h, wide) && on(a.dx, wide) && on(a.dx2, 16);
+  return ln::plan_for(backward, mode, size_of(xd), size_of(yd), a.gh != nullptr, base, vec, a.rows, a.C);
+}
+
+// Partial sums of the backward pass: one (2, C) fp32 block per CTA, for whichever kernel the alignment will choose.
 size_t ln_train_workspace_bytes(int xd, int rows, int C) {
-  const int v = xd == 0 ? 4 : 8;
-  int n = ln::grid_for(rows, geometry_of(xd, C, false), ln::kBwdPerSm);
-  if (C % v == 0) {
-    const int m = ln::grid_for(rows, geometry_of(xd, C, true), ln::kBwdPerSm);
-    n = n > m ? n : m;
-  }
+  const int direct = ln::direct_grid(rows, ln::geometry(C, 1, 0).lpr);
+  const int n = direct > ln::kSms ? direct : (rows < ln::kSms ? rows : ln::kSms);
   return (size_t)n * 2 * C * sizeof(float);
 }
 
-// xd / yd: tensor types (0 fp32, 1 fp16, 2 bf16) of the branch input and of residual / result / gradients; yd is
-// xd or fp32.  Parameters are fp32 or of type xd.
-static cudaError_t run(bool backward, int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s) {
-  const bool vec = vectors_ok(xd, yd, a);
-  if (xd == 0) return ln_train_run_f32_f32(backward, mode, act, vec, a, s);
-  if (xd == 1) return yd == 0 ? ln_train_run_f16_f32(backward, mode, act, vec, a, s) : ln_train_run_f16_f16(backward, mode, act, vec, a, s);
-  return yd == 0 ? ln_train_run_bf16_f32(backward, mode, act, vec, a, s) : ln_train_run_bf16_bf16(backward, mode, act, vec, a, s);
+// xd / yd: tensor types of the branch input and of residual / result / gradients; yd is xd or fp32.  Parameters are
+// fp32 or of type xd.
+static cudaError_t run(bool backward, int mode, int act, int xd, int yd, const ln::Plan& p, const LnTrainArgs& a, cudaStream_t s) {
+  if (xd == 0) return ln_train_run_f32_f32(backward, mode, act, p, a, s);
+  if (xd == 1) return yd == 0 ? ln_train_run_f16_f32(backward, mode, act, p, a, s) : ln_train_run_f16_f16(backward, mode, act, p, a, s);
+  return yd == 0 ? ln_train_run_bf16_f32(backward, mode, act, p, a, s) : ln_train_run_bf16_bf16(backward, mode, act, p, a, s);
 }
 
 cudaError_t launch_ln_train_fwd(int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s) {
-  return run(false, mode, act, xd, yd, a, s);
+  return run(false, mode, act, xd, yd, plan_of(false, mode, xd, yd, a), a, s);
 }
 
 cudaError_t launch_ln_train_bwd(int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s) {
-  if (cudaError_t e = run(true, mode, act, xd, yd, a, s)) return e;
+  const ln::Plan p = plan_of(true, mode, xd, yd, a);
+  if (cudaError_t e = run(true, mode, act, xd, yd, p, a, s)) return e;
   LnTrainArgs f = a;
-  f.n_partial = ln::grid_for(a.rows, geometry_of(xd, a.C, vectors_ok(xd, yd, a)), ln::kBwdPerSm);
+  f.n_partial = p.grid;
   const dim3 grid((unsigned)((a.C + kCols - 1) / kCols)), threads(kCols * kSlices);
   if (xd == 1) return launch_overlapped(ln_train_params_kernel<__half>, grid, threads, 0, s, f, mode);
   if (xd == 2) return launch_overlapped(ln_train_params_kernel<__nv_bfloat16>, grid, threads, 0, s, f, mode);

@@ -11,11 +11,19 @@
 //   plain, pre: dw = A, db = B;   post: dw = gamma A, db = gamma B, dgamma = w A + b B
 // so one row kernel and one small reduction over the CTAs' partial (A, B) serve all three.
 //
-// A row belongs to a team of `lpr` lanes: 2..32 lanes of a warp, or a whole CTA of 2..16 warps.  A lane keeps its
-// NV vectors of the row in registers (each element is read once and written once), its slice of the parameters and
-// of A and B for the whole launch; statistics and sums are fp32, two passes over registers (mean, then squared
-// deviations).  Nothing is accumulated with atomics: the order of every sum is fixed by the sizes alone, so
-// results repeat bit for bit.
+// All of them are bound by memory: a few operations per element, each tensor read and written once.  Rows are contiguous,
+// so a tile of rows is one span per tensor, and a ring of such tiles is kept in flight with bulk copies (cp.async.bulk,
+// mbarriers, bounded waits) while the CTA's 8 or 16 warps compute: the bytes in flight do not depend on how many
+// registers a row takes.  A span only has to start on 16 bytes, so rows of any width use the ring; with a width that no
+// vector divides the lanes read shared memory element by element.
+//
+// A row belongs to a team of `lpr` lanes: 2..32 lanes of a warp, or all computing warps of the CTA.  A lane keeps its
+// NV vectors of the row, its slice of the parameters and of A and B in registers; statistics and sums are fp32, two
+// passes over registers (mean, then squared deviations), two elements per instruction (fma.rn.f32x2).  Nothing is
+// accumulated with atomics: the order of every sum is fixed by the sizes alone, so results repeat bit for bit.
+//
+// Tensors that do not start on 16 bytes (a view into the middle of another), and odd rows too wide for the ring, take
+// the element-wise kernels at the end, which load straight from global memory.
 //
 // The reference builds these norms from torch.nn.LayerNorm, layer-scale products, timm's DropPath and residual
 // additions (classification/models/flash_intern_image.py:34-56, 414-432); it has no kernel for them.
@@ -49,9 +57,17 @@ struct LnTrainArgs {
   int lpr;               // lanes of a team (32 * warps when a row takes the whole CTA)
   int param_f32;         // parameters are fp32 (else: the type TP of the instantiation)
   unsigned rows_per_sample;
+  unsigned long long per_mul;  // row / rows_per_sample == (row * per_mul) >> per_shift for row < 2^31
+  int per_shift;
   int n_partial;
   float eps;
+  int* status;           // device status word
+  int tile_rows, stages; // ring: rows of a tile, tiles in flight
 };
+
+__device__ __forceinline__ unsigned sample_of(const LnTrainArgs& a, unsigned row) {
+  return (unsigned)((row * a.per_mul) >> a.per_shift);
+}
 
 namespace ln {
 
@@ -131,7 +147,562 @@ constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143
 
 enum : int { kPlain = 0, kPost = 1, kPre = 2 };
 
-// ------------------------------------------------------------------------------------ forward
+// ------------------------------------------------------------------------------ arithmetic
+
+// Pairs of fp32: one instruction for two elements (sm_100).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Normal distribution function and density of two values, each from one exponential: Phi by formula 7.1.26 of Abramowitz
+// and Stegun (erf to 1.5e-7), the density is that formula's own exp(-z^2 / 2) / sqrt(2 pi).
+__device__ __forceinline__ void normal(float2 z, float2& cdf, float2& density) {
+  const float2 x = mul2(make_float2(fabsf(z.x), fabsf(z.y)), both(kSqrtHalf));
+  const float2 y = mul2(mul2(x, x), both(-1.4426950408889634f));
+  float2 e, t = fma2(x, both(0.3275911f), both(1.f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(y.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(y.y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(t.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(t.y));
+  float2 q = fma2(both(1.061405429f), t, both(-1.453152027f));
+  q = fma2(q, t, both(1.421413741f));
+  q = fma2(q, t, both(-0.284496736f));
+  q = fma2(q, t, both(0.254829592f));
+  // erf|x| = 1 - q t e, hence Phi = 1/2 + sign(z) (1/2 - q t e / 2)
+  const float2 half = fma2(mul2(mul2(q, t), e), both(-0.5f), both(0.5f));
+  cdf = add2(make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y)), both(0.5f));
+  density = mul2(e, both(kInvSqrt2Pi));
+}
+
+// ------------------------------------------------------------------------------ the ring of row tiles
+
+constexpr int kMaxStages = 8;
+constexpr int kRingHeader = 512;    // barriers, abort flag, team sums
+struct RingHeader {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  int abort;
+  int pad;
+  float2 red[2][16];
+};
+static_assert(sizeof(RingHeader) <= kRingHeader, "ring header");
+
+// Warps of a CTA: as many as the registers of NE elements a lane leave room for.  Parameters live in registers up to
+// 16 elements, beyond that in shared memory.
+constexpr int warps_for(int ne) { return ne <= 16 ? 16 : 12; }
+template <int NE> constexpr int ring_warps() { return warps_for(NE); }
+template <int NE> constexpr bool params_in_smem() { return NE > 16; }
+
+__device__ __forceinline__ void ring_wait(uint64_t* bar, uint32_t parity, RingHeader* h, int* status) {
+  if (*(volatile int*)&h->abort) return;
+  if (!mbar_wait_bounded(bar, parity)) { atomicExch(status, kStatusStageTimeout); *(volatile int*)&h->abort = 1; }
+}
+__device__ __forceinline__ void ring_init(RingHeader* h, int stages, int warps) {
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&h->full[s], 1); mbar_init(&h->empty[s], (uint32_t)warps); }
+    h->abort = 0;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void ring_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// One tensor's span of a tile: whole 16-byte units by bulk copy, the last tile's remainder by plain stores, which the
+// arrival that follows makes visible.  Returns the bytes the barrier has to expect.
+__device__ __forceinline__ uint32_t span_bytes(int n, int C, int es) { return (uint32_t)n * (uint32_t)C * (uint32_t)es; }
+template <typename T>
+__device__ __forceinline__ void span_tail(unsigned char* dst, const T* src, uint32_t bytes) {
+  for (uint32_t i = (bytes & ~15u) / sizeof(T); i < bytes / sizeof(T); ++i) reinterpret_cast<T*>(dst)[i] = src[i];
+}
+
+// Fills the ring.  One lane of the first warp asks for a tile of up to three tensors; it refills a slot when it starts the
+// tile after the one the slot held, so it waits for the slowest warp of that tile and no warp does nothing else.
+template <typename T0, typename T1, typename T2>
+struct RingFill {
+  const T0* p0; const T1* p1; const T2* p2;
+  unsigned char* ring;
+  RingHeader* h;
+  int tiles;
+
+  __device__ __forceinline__ uint32_t slot0(const LnTrainArgs& a) const { return span_bytes(a.tile_rows, a.C, sizeof(T0)); }
+  __device__ __forceinline__ uint32_t slot1(const LnTrainArgs& a) const { return p1 ? span_bytes(a.tile_rows, a.C, sizeof(T1)) : 0; }
+  __device__ __forceinline__ uint32_t slot2(const LnTrainArgs& a) const { return p2 ? span_bytes(a.tile_rows, a.C, sizeof(T2)) : 0; }
+
+  // tile `t` into slot `stage`, which is free
+  __device__ void issue(const LnTrainArgs& a, int t, int stage) const {
+    const uint32_t z0 = slot0(a), z1 = slot1(a);
+    const long long row0 = (long long)t * a.tile_rows;
+    const int n = (int)(a.rows - row0 < a.tile_rows ? a.rows - row0 : a.tile_rows);
+    const uint32_t b0 = span_bytes(n, a.C, sizeof(T0)), b1 = p1 ? span_bytes(n, a.C, sizeof(T1)) : 0;
+    const uint32_t b2 = p2 ? span_bytes(n, a.C, sizeof(T2)) : 0;
+    unsigned char* d = ring + (size_t)stage * (z0 + z1 + slot2(a));
+    const T0* s0 = p0 + row0 * a.C;
+    const T1* s1 = p1 ? p1 + row0 * a.C : nullptr;
+    const T2* s2 = p2 ? p2 + row0 * a.C : nullptr;
+    span_tail(d, s0, b0);
+    if (p1) span_tail(d + z0, s1, b1);
+    if (p2) span_tail(d + z0 + z1, s2, b2);
+    mbar_expect_tx(&h->full[stage], (b0 & ~15u) + (b1 & ~15u) + (b2 & ~15u));
+    if (b0 & ~15u) bulk_g2s(d, s0, b0 & ~15u, &h->full[stage]);
+    if (b1 & ~15u) bulk_g2s(d + z0, s1, b1 & ~15u, &h->full[stage]);
+    if (b2 & ~15u) bulk_g2s(d + z0 + z1, s2, b2 & ~15u, &h->full[stage]);
+  }
+  __device__ void start(const LnTrainArgs& a) const {
+    for (int s = 0; s < a.stages; ++s) {
+      const long long t = blockIdx.x + (long long)s * gridDim.x;
+      if (t < tiles) issue(a, (int)t, s);
+    }
+  }
+  // before this CTA's tile `t` (its k-th, k > 0): the slot of the tile before gets the tile `stages` further on
+  __device__ void refill(const LnTrainArgs& a, int t, int stage, uint32_t phase) const {
+    const long long next = (long long)t + (long long)(a.stages - 1) * gridDim.x;
+    if (next >= tiles) return;
+    const int prev = stage == 0 ? a.stages - 1 : stage - 1;
+    ring_wait(&h->empty[prev], stage == 0 ? phase ^ 1 : phase, h, a.status);
+    if (!*(volatile int*)&h->abort) issue(a, (int)next, prev);
+  }
+};
+
+// A lane's elements of a row in shared memory, as pairs.  VEC > 1: vectors sub, sub + lpr, ... of VEC elements; VEC == 1:
+// elements sub, sub + lpr, ...
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void row_load(float2 (&f)[NV * VEC / 2], const T* row, int sub, int lpr, int C, bool live) {
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int v = 0; v < NV; v += 2) {
+      const int c0 = sub + v * lpr, c1 = c0 + lpr;
+      f[v / 2].x = live && c0 < C ? to_f32(row[c0]) : 0.f;
+      f[v / 2].y = live && c1 < C ? to_f32(row[c1]) : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (sub + v * lpr) * VEC;
+      constexpr int W = VEC * (int)sizeof(T) / 4;
+      uint32_t r[W];
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        uint4 t = make_uint4(0u, 0u, 0u, 0u);
+        if (live && c < C) t = reinterpret_cast<const uint4*>(row + c)[i];
+        r[4 * i] = t.x; r[4 * i + 1] = t.y; r[4 * i + 2] = t.z; r[4 * i + 3] = t.w;
+      }
+      float w[VEC];
+      widen(r, w, (const T*)nullptr);
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) f[v * VEC / 2 + e] = make_float2(w[2 * e], w[2 * e + 1]);
+    }
+  }
+}
+// The same from global memory (parameters).
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void row_fetch(float2 (&f)[NV * VEC / 2], const T* row, int sub, int lpr, int C) {
+  row_load<T, VEC, NV>(f, row, sub, lpr, C, true);
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void row_store(T* row, const float2 (&f)[NV * VEC / 2], int sub, int lpr, int C) {
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int v = 0; v < NV; v += 2) {
+      const int c0 = sub + v * lpr, c1 = c0 + lpr;
+      if (c0 < C) row[c0] = from_f32<T>(f[v / 2].x);
+      if (c1 < C) row[c1] = from_f32<T>(f[v / 2].y);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (sub + v * lpr) * VEC;
+      if (c < C) {
+        float w[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) { w[2 * e] = f[v * VEC / 2 + e].x; w[2 * e + 1] = f[v * VEC / 2 + e].y; }
+        uint32_t r[VEC * sizeof(T) / 4];
+        narrow(w, r, (const T*)nullptr);
+        stg_raw(row + c, r);   // 16 or 32 bytes in one instruction
+      }
+    }
+  }
+}
+// Parameter slice in the same order; zero beyond C.
+template <typename P, int VEC, int NV>
+__device__ __forceinline__ void param_load(float2 (&f)[NV * VEC / 2], const void* p, int sub, int lpr, int C, int f32) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int c = (sub + v * lpr) * VEC + e, i = v * VEC + e;
+      const float t = c < C ? param<P>(p, c, f32) : 0.f;
+      if (i & 1) f[i / 2].y = t;
+      else f[i / 2].x = t;
+    }
+}
+// 16-byte loads where the parameters allow it: a launch's first rows wait for these.
+template <typename P, int VEC, int NV>
+__device__ __forceinline__ void param_fetch(float2 (&f)[NV * VEC / 2], const void* p, int sub, int lpr, int C, int f32) {
+  if constexpr (VEC > 1) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      if (f32) { row_fetch<float, VEC, NV>(f, static_cast<const float*>(p), sub, lpr, C); return; }
+      if constexpr (sizeof(P) == 2) { row_fetch<P, VEC, NV>(f, static_cast<const P*>(p), sub, lpr, C); return; }
+    }
+  }
+  param_load<P, VEC, NV>(f, p, sub, lpr, C, f32);
+}
+// One fp32 parameter vector in shared memory, filled by the whole CTA.
+template <typename P>
+__device__ __forceinline__ void param_stage(float* dst, const void* p, const void* factor, int C, int f32) {
+  for (int c = threadIdx.x; c < C; c += blockDim.x)
+    dst[c] = param<P>(p, c, f32) * (factor != nullptr ? param<P>(factor, c, f32) : 1.f);
+}
+// A lane's pair i of a staged parameter vector.
+template <int VEC, int NV>
+__device__ __forceinline__ void param_row(float2 (&f)[NV * VEC / 2], const float* p, int sub, int lpr, int C) {
+  row_load<float, VEC, NV>(f, p, sub, lpr, C, true);
+}
+// Column of a lane's element i.
+template <int VEC> __device__ __forceinline__ int column(int i, int sub, int lpr) { return (sub + i / VEC * lpr) * VEC + i % VEC; }
+
+// Sum of two values over the team.  The warps of a wider team meet at a named barrier of their own, one per call (the
+// slots alternate, so the next call cannot overwrite what a slow warp still reads).
+__device__ __forceinline__ float2 ring_sum(float2 t, int lpr, RingHeader* h, int& flip) {
+#pragma unroll 1
+  for (int o = lpr > 32 ? 16 : lpr >> 1; o > 0; o >>= 1) {
+    const float2 u = make_float2(__shfl_xor_sync(0xffffffffu, t.x, o), __shfl_xor_sync(0xffffffffu, t.y, o));
+    t = add2(t, u);
+  }
+  if (lpr > 32) {
+    float2* slot = h->red[flip];
+    flip ^= 1;
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = t;
+    const int team = threadIdx.x / lpr;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(lpr) : "memory");
+    t = make_float2(0.f, 0.f);
+    for (int i = 0; i < (lpr >> 5); ++i) t = add2(t, slot[team * (lpr >> 5) + i]);
+  }
+  return t;
+}
+
+__device__ __forceinline__ float ring_sum(float t, int lpr, RingHeader* h, int& flip) {
+#pragma unroll 1
+  for (int o = lpr > 32 ? 16 : lpr >> 1; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (lpr > 32) {
+    float2* slot = h->red[flip];
+    flip ^= 1;
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5].x = t;
+    const int team = threadIdx.x / lpr;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(lpr) : "memory");
+    t = 0.f;
+    for (int i = 0; i < (lpr >> 5); ++i) t += slot[team * (lpr >> 5) + i].x;
+  }
+  return t;
+}
+
+template <typename TX, typename TY, int VEC, int NV, int MODE, bool GELU>
+__global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), 1)
+ln_ring_fwd_kernel(const LnTrainArgs a) {
+  using P = TX;
+  constexpr int NE = VEC * NV, W = ring_warps<NE>();
+  extern __shared__ __align__(128) unsigned char smem[];
+  RingHeader* h = reinterpret_cast<RingHeader*>(smem);
+  unsigned char* ring = smem + kRingHeader;
+  const int lpr = a.lpr, C = a.C, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
+  ring_init(h, a.stages, W);
+  pdl_trigger();
+  pdl_wait();
+  const RingFill<TX, TY, TY> fill{static_cast<const TX*>(a.x), MODE == kPlain ? nullptr : static_cast<const TY*>(a.res), nullptr,
+                                  ring, h, tiles};
+  if (threadIdx.x == 0) fill.start(a);
+  {
+    const int sub = (int)threadIdx.x % lpr, team = (int)threadIdx.x / lpr;
+    const int per_pass = W * 32 / lpr;                     // rows of one pass of the CTA
+    const int first = lpr > 32 ? team : warp * (32 / lpr);  // first row of this warp in a pass
+    const int passes = (a.tile_rows + per_pass - 1) / per_pass;
+    const float inv_c = 1.f / (float)C;
+    const uint32_t slot0 = fill.slot0(a), slot = slot0 + fill.slot1(a);
+    int flip = 0;
+    constexpr bool kStaged = params_in_smem<NE>();
+    float2 w[NE / 2], b[NE / 2];
+    float* ws = reinterpret_cast<float*>(ring + (size_t)a.stages * slot);
+    float* bs = ws + (C + 3) / 4 * 4;
+    if constexpr (kStaged) {
+      const void* g = MODE == kPost ? a.gamma : nullptr;
+      param_stage<P>(ws, a.w, g, C, a.param_f32);
+      param_stage<P>(bs, a.b, g, C, a.param_f32);
+      __syncthreads();
+    } else {
+      param_fetch<P, VEC, NV>(w, a.w, sub, lpr, C, a.param_f32);
+      param_fetch<P, VEC, NV>(b, a.b, sub, lpr, C, a.param_f32);
+      if (MODE == kPost && a.gamma != nullptr) {
+        float2 g[NE / 2];
+        param_fetch<P, VEC, NV>(g, a.gamma, sub, lpr, C, a.param_f32);
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) { w[i] = mul2(w[i], g[i]); b[i] = mul2(b[i], g[i]); }
+      }
+    }
+    const bool scaled = MODE != kPlain && a.s != nullptr;
+    auto factor = [&](int t, int pass) {        // s of this team's row, asked for one pass ahead
+      const int lr = pass * per_pass + team;
+      const long long row = (long long)t * a.tile_rows + lr;
+      return t < tiles && lr < a.tile_rows && row < a.rows ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
+    };
+    float s = 1.f, s_next = scaled ? factor(blockIdx.x, 0) : 1.f;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      if (threadIdx.x == 0 && t != (int)blockIdx.x) fill.refill(a, t, stage, phase);
+      __syncwarp();
+      ring_wait(&h->full[stage], phase, h, a.status);
+      const unsigned char* base = ring + (size_t)stage * slot;
+      const int row0 = t * a.tile_rows;
+      const int n = a.rows - row0 < a.tile_rows ? a.rows - row0 : a.tile_rows;
+      for (int pass = 0; pass < passes; ++pass) {
+        if (scaled) {
+          s = s_next;
+          s_next = pass + 1 < passes ? factor(t, pass + 1) : factor(t + gridDim.x, 0);
+        }
+        const int lr = pass * per_pass + team;
+        if (pass * per_pass + first >= n) continue;        // no row of this warp's
+        const bool live = lr < n;
+        const int row = row0 + lr;
+        float2 x[NE / 2], r[MODE == kPlain ? 1 : NE / 2];
+        row_load<TX, VEC, NV>(x, reinterpret_cast<const TX*>(base) + (size_t)lr * C, sub, lpr, C, live);
+        if constexpr (MODE != kPlain) row_load<TY, VEC, NV>(r, reinterpret_cast<const TY*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live);
+        if constexpr (MODE == kPre) {
+#pragma unroll
+          for (int i = 0; i < NE / 2; ++i) x[i] = fma2(both(s), x[i], r[i]);
+          if (live) row_store<TY, VEC, NV>(static_cast<TY*>(a.h) + (long long)row * C, x, sub, lpr, C);
+        }
+        // two chains of additions each: a warp's own latency is what these short rows wait for
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) sum[i & 1] = add2(sum[i & 1], x[i]);
+        sum[0] = add2(sum[0], sum[1]);
+        const float mean = ring_sum(sum[0].x + sum[0].y, lpr, h, flip) * inv_c;
+        float2 sq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) {
+          x[i] = add2(x[i], both(-mean));
+          if (VEC > 1) {
+            if (column<VEC>(2 * i, sub, lpr) < C) sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
+          } else {
+            if (column<VEC>(2 * i, sub, lpr) < C) sq[i & 1].x = fmaf(x[i].x, x[i].x, sq[i & 1].x);
+            if (column<VEC>(2 * i + 1, sub, lpr) < C) sq[i & 1].y = fmaf(x[i].y, x[i].y, sq[i & 1].y);
+          }
+        }
+        sq[0] = add2(sq[0], sq[1]);
+        const float rstd = rsqrtf(ring_sum(sq[0].x + sq[0].y, lpr, h, flip) * inv_c + a.eps);
+        if (!live) continue;
+        if constexpr (kStaged) {
+          param_row<VEC, NV>(w, ws, sub, lpr, C);
+          param_row<VEC, NV>(b, bs, sub, lpr, C);
+        }
+        if (sub == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) {
+          float2 o = fma2(mul2(x[i], both(rstd)), w[i], b[i]);
+          if (GELU) {
+            float2 cdf, density;
+            normal(o, cdf, density);
+            o = mul2(o, cdf);
+          }
+          if constexpr (MODE == kPost) o = fma2(both(s), o, r[i]);
+          x[i] = o;
+        }
+        row_store<TY, VEC, NV>(static_cast<TY*>(a.y) + (long long)row * C, x, sub, lpr, C);
+      }
+      __syncwarp();
+      if (lane == 0) ring_arrive(&h->empty[stage]);
+      if (++stage == a.stages) { stage = 0; phase ^= 1; }
+    }
+  }
+  if (*(volatile int*)&h->abort)       // copies into this CTA's memory may be in flight: give them 20 ms to land
+    for (int i = 0; i < 20000; ++i) __nanosleep(1000);
+}
+
+template <typename TL, typename TG, typename T2, typename P, int VEC, int NV, int MODE, bool GELU>
+__global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), 1)
+ln_ring_bwd_kernel(const LnTrainArgs a) {
+  constexpr int NE = VEC * NV, W = ring_warps<NE>();
+  extern __shared__ __align__(128) unsigned char smem[];
+  RingHeader* h = reinterpret_cast<RingHeader*>(smem);
+  unsigned char* ring = smem + kRingHeader;
+  const int lpr = a.lpr, C = a.C, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
+  const bool with_gh = MODE == kPre && a.gh != nullptr;
+  ring_init(h, a.stages, W);
+  pdl_trigger();
+  pdl_wait();
+  const int sub = (int)threadIdx.x % lpr, team = (int)threadIdx.x / lpr;
+  float2 sa[NE / 2], sb[NE / 2];
+#pragma unroll
+  for (int i = 0; i < NE / 2; ++i) sa[i] = sb[i] = make_float2(0.f, 0.f);
+  const RingFill<TL, TG, TG> fill{static_cast<const TL*>(MODE == kPre ? a.h : a.x), static_cast<const TG*>(a.gy),
+                                  with_gh ? static_cast<const TG*>(a.gh) : nullptr, ring, h, tiles};
+  if (threadIdx.x == 0) fill.start(a);
+  {
+    const int per_pass = W * 32 / lpr;
+    const int first = lpr > 32 ? team : warp * (32 / lpr);
+    const int passes = (a.tile_rows + per_pass - 1) / per_pass;
+    const float inv_c = 1.f / (float)C;
+    const uint32_t slot0 = fill.slot0(a), slot1 = fill.slot1(a), slot = slot0 + slot1 + fill.slot2(a);
+    int flip = 0;
+    constexpr bool kStaged = params_in_smem<NE>();
+    float2 w[NE / 2], b[GELU ? NE / 2 : 1];
+    float* ws = reinterpret_cast<float*>(ring + (size_t)a.stages * slot);
+    float* bs = ws + (C + 3) / 4 * 4;
+    if constexpr (kStaged) {
+      param_stage<P>(ws, a.w, MODE == kPost ? a.gamma : nullptr, C, a.param_f32);
+      if constexpr (GELU) param_stage<P>(bs, a.b, nullptr, C, a.param_f32);
+      __syncthreads();
+    } else {
+      param_fetch<P, VEC, NV>(w, a.w, sub, lpr, C, a.param_f32);
+      if constexpr (GELU) param_fetch<P, VEC, NV>(b, a.b, sub, lpr, C, a.param_f32);
+      if (MODE == kPost && a.gamma != nullptr) {
+        float2 g[NE / 2];
+        param_fetch<P, VEC, NV>(g, a.gamma, sub, lpr, C, a.param_f32);
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) w[i] = mul2(w[i], g[i]);
+      }
+    }
+    const bool scaled = MODE != kPlain && a.s != nullptr;
+    // statistics and factor of this team's row, asked for one pass ahead
+    auto stats = [&](int t, int pass, float& mean, float& rstd, float& s) {
+      const int lr = pass * per_pass + team;
+      const long long row = (long long)t * a.tile_rows + lr;
+      const bool ok = t < tiles && lr < a.tile_rows && row < a.rows;
+      mean = ok ? __ldg(a.mean + row) : 0.f;
+      rstd = ok ? __ldg(a.rstd + row) : 0.f;
+      if (scaled) s = ok ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
+    };
+    float mean_n, rstd_n, s_n = 1.f;
+    stats(blockIdx.x, 0, mean_n, rstd_n, s_n);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      if (threadIdx.x == 0 && t != (int)blockIdx.x) fill.refill(a, t, stage, phase);
+      __syncwarp();
+      ring_wait(&h->full[stage], phase, h, a.status);
+      const unsigned char* base = ring + (size_t)stage * slot;
+      const int row0 = t * a.tile_rows;
+      const int n = a.rows - row0 < a.tile_rows ? a.rows - row0 : a.tile_rows;
+      for (int pass = 0; pass < passes; ++pass) {
+        const float mean = mean_n, rstd = rstd_n, s = s_n;
+        if (pass + 1 < passes) stats(t, pass + 1, mean_n, rstd_n, s_n);
+        else stats(t + gridDim.x, 0, mean_n, rstd_n, s_n);
+        const int lr = pass * per_pass + team;
+        if (pass * per_pass + first >= n) continue;
+        const bool live = lr < n;
+        const int row = row0 + lr;
+        float2 x[NE / 2], g[NE / 2];
+        row_load<TL, VEC, NV>(x, reinterpret_cast<const TL*>(base) + (size_t)lr * C, sub, lpr, C, live);
+        row_load<TG, VEC, NV>(g, reinterpret_cast<const TG*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live);
+        // elements beyond C have g = w = 0 and add nothing to any sum
+        float2 t1[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, t2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if constexpr (kStaged) {
+          param_row<VEC, NV>(w, ws, sub, lpr, C);
+          if constexpr (GELU) param_row<VEC, NV>(b, bs, sub, lpr, C);
+        }
+        const float2 r2 = both(rstd), shift = both(-mean);
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) {
+          x[i] = mul2(add2(x[i], shift), r2);
+          if (MODE == kPost) g[i] = mul2(g[i], both(s));
+          if constexpr (GELU) {
+            const float2 z = fma2(x[i], w[i], b[i]);
+            float2 cdf, density;
+            normal(z, cdf, density);
+            g[i] = mul2(g[i], fma2(z, density, cdf));
+          }
+          sa[i] = fma2(g[i], x[i], sa[i]);
+          sb[i] = add2(sb[i], g[i]);
+          g[i] = mul2(g[i], w[i]);
+          t1[i & 1] = add2(t1[i & 1], g[i]);
+          t2[i & 1] = fma2(g[i], x[i], t2[i & 1]);
+        }
+        t1[0] = add2(t1[0], t1[1]);
+        t2[0] = add2(t2[0], t2[1]);
+        const float2 m = ring_sum(make_float2(t1[0].x + t1[0].y, t2[0].x + t2[0].y), lpr, h, flip);
+        if (!live) continue;
+        const float2 m1 = both(-m.x * inv_c * rstd), m2 = both(-m.y * inv_c * rstd);
+        if constexpr (MODE == kPre) {
+#pragma unroll
+          for (int i = 0; i < NE / 2; ++i) x[i] = fma2(x[i], m2, fma2(g[i], r2, m1));
+          if (with_gh) {
+            row_load<TG, VEC, NV>(g, reinterpret_cast<const TG*>(base + slot0 + slot1) + (size_t)lr * C, sub, lpr, C, true);
+#pragma unroll
+            for (int i = 0; i < NE / 2; ++i) x[i] = add2(x[i], g[i]);
+          }
+          row_store<TL, VEC, NV>(static_cast<TL*>(a.dx) + (long long)row * C, x, sub, lpr, C);
+          if (a.dx2 != nullptr) {
+#pragma unroll
+            for (int i = 0; i < NE / 2; ++i) x[i] = mul2(x[i], both(s));
+            row_store<T2, VEC, NV>(static_cast<T2*>(a.dx2) + (long long)row * C, x, sub, lpr, C);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NE / 2; ++i) x[i] = fma2(x[i], m2, fma2(g[i], r2, m1));
+          row_store<TL, VEC, NV>(static_cast<TL*>(a.dx) + (long long)row * C, x, sub, lpr, C);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ring_arrive(&h->empty[stage]);
+      if (++stage == a.stages) { stage = 0; phase ^= 1; }
+    }
+    // over the teams of each warp
+    for (int o = lpr; o < 32; o <<= 1) {
+#pragma unroll
+      for (int i = 0; i < NE / 2; ++i) {
+        sa[i].x += __shfl_xor_sync(0xffffffffu, sa[i].x, o);
+        sa[i].y += __shfl_xor_sync(0xffffffffu, sa[i].y, o);
+        sb[i].x += __shfl_xor_sync(0xffffffffu, sb[i].x, o);
+        sb[i].y += __shfl_xor_sync(0xffffffffu, sb[i].y, o);
+      }
+    }
+  }
+  if (*(volatile int*)&h->abort)
+    for (int i = 0; i < 20000; ++i) __nanosleep(1000);
+  // over the warps, or the teams of several warps, through the ring's memory: every tile has been consumed
+  __syncthreads();
+  float* acc = reinterpret_cast<float*>(ring);     // [slots][2][C]
+  const int slots = lpr > 32 ? W * 32 / lpr : W, slot = lpr > 32 ? team : warp;
+  if (lpr > 32 || lane < lpr) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int c = column<VEC>(i, sub, lpr);
+      if (c < C) {
+        acc[(slot * 2) * C + c] = i & 1 ? sa[i / 2].y : sa[i / 2].x;
+        acc[(slot * 2 + 1) * C + c] = i & 1 ? sb[i / 2].y : sb[i / 2].x;
+      }
+    }
+  }
+  __syncthreads();
+  float* dst = a.partial + (size_t)blockIdx.x * 2 * C;
+  for (int i = threadIdx.x; i < 2 * C; i += blockDim.x) {
+    float t = 0.f;
+    for (int q = 0; q < slots; ++q) t += acc[q * 2 * C + i];
+    dst[i] = t;
+  }
+}
+
+// ------------------------------------------------------------------------- element-wise kernels
 
 template <typename TX, typename TY, int VEC, int NV, int MODE, bool GELU>
 __global__ void __launch_bounds__(512)
@@ -178,7 +749,7 @@ ln_train_fwd_kernel(const LnTrainArgs a) {
       if (MODE != kPlain) load<TY, VEC>(rr[v], static_cast<const TY*>(a.res) + base + c, live && c < C);
     }
     float s = 1.f;
-    if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + (unsigned)row / a.rows_per_sample) : 0.f;
+    if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
     float xv[NV][VEC];
     float sum = 0.f;
 #pragma unroll
@@ -215,7 +786,7 @@ ln_train_fwd_kernel(const LnTrainArgs a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         o[e] = fmaf((xv[v][e] - mean) * rstd, w[v][e], b[v][e]);
-        if (GELU) o[e] = 0.5f * o[e] * (1.f + erff(o[e] * kSqrtHalf));
+        if (GELU) { float2 cdf, density; normal(both(o[e]), cdf, density); o[e] *= cdf.x; }
         if (MODE == kPost) o[e] = fmaf(s, o[e], rv[e]);
       }
       store<TY, VEC>(static_cast<TY*>(a.y) + base + c, o);
@@ -272,7 +843,7 @@ ln_train_bwd_kernel(const LnTrainArgs a) {
     }
     const float mean = live ? __ldg(a.mean + row) : 0.f, rstd = live ? __ldg(a.rstd + row) : 0.f;
     float s = 1.f;
-    if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + (unsigned)row / a.rows_per_sample) : 0.f;
+    if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
     float xh[NV][VEC], gw[NV][VEC];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -287,8 +858,9 @@ ln_train_bwd_kernel(const LnTrainArgs a) {
         if (MODE == kPost) g[e] *= s;
         if (GELU) {
           const float z = fmaf(xh[v][e], w[v][e], b[v][e]);
-          const float cdf = 0.5f * (1.f + erff(z * kSqrtHalf));
-          g[e] *= fmaf(z * kInvSqrt2Pi, __expf(-0.5f * z * z), cdf);
+          float2 cdf, density;
+          normal(both(z), cdf, density);
+          g[e] *= fmaf(z, density.x, cdf.x);
         }
         sa[v][e] = fmaf(g[e], xh[v][e], sa[v][e]);
         sb[v][e] += g[e];
@@ -363,82 +935,174 @@ ln_train_bwd_kernel(const LnTrainArgs a) {
 
 // --------------------------------------------------------------------------------- dispatch
 
-// Team width and vectors per lane for `n_vec` vectors a row.
+// Team width, elements per lane and computing warps for a row of `n` vectors (or elements).
 struct Geometry {
-  int lpr, nv, threads;
+  int lpr, nv, warps;
   bool ok;
 };
-// NV candidates: 1..4 vectors, or 4 / 16 scalars.  The fewest idle vector slots win; ties go to the wider team
-// (fewer registers).  Teams stop at 512 lanes.
-inline Geometry geometry(int n_vec, bool scalar, int max_nv) {
+// A lane holds 1..max_nv vectors, or 4, 8, 12 or 16 single elements.  A row costs its team's lanes about as much for its
+// bookkeeping as ten more elements a lane would: fewest lanes * (elements + 10) wins.  A team divides the warps of
+// the CTA (16, or 12 where a lane holds more than 16 elements).
+inline Geometry geometry(int n, int vec, int max_nv) {
   Geometry best{0, 0, 0, false};
-  double best_cost = 1e30;
+  long long best_cost = 0;
   for (int lpr = 2; lpr <= 512; lpr *= 2) {
-    int nv = (n_vec + lpr - 1) / lpr;
-    if (scalar) nv = nv <= 4 ? 4 : (nv <= 16 ? 16 : 1000);
-    if (nv > (scalar ? 16 : max_nv)) continue;
-    const double cost = (double)lpr * nv / n_vec;
-    if (cost <= best_cost * 1.0001) { best_cost = cost; best = Geometry{lpr, nv, lpr > 32 ? lpr : 256, true}; }
+    int nv = (n + lpr - 1) / lpr;
+    if (vec == 1) nv = (nv + 3) / 4 * 4;
+    if (nv > (vec == 1 ? 16 : max_nv)) continue;
+    const int warps = warps_for(nv * vec);
+    if (warps * 32 % lpr != 0) continue;
+    const long long cost = (long long)lpr * (nv * vec + 10);
+    if (!best.ok || cost < best_cost) { best_cost = cost; best = Geometry{lpr, nv, warps, true}; }
   }
   return best;
 }
 
-// CTAs of a launch over `rows` rows: what the rows fill, at most `per_sm` per SM.
-inline int grid_for(int rows, const Geometry& g, int per_sm) {
-  const int rows_per_cta = g.lpr > 32 ? 1 : g.threads / g.lpr;
-  const long long need = ((long long)rows + rows_per_cta - 1) / rows_per_cta;
-  const long long cap = (long long)kSms * per_sm;
-  return (int)(need < cap ? (need < 1 ? 1 : need) : cap);
+constexpr size_t kRingBytes = 200 * 1024;   // of 227 KB per SM
+constexpr size_t kTileBytes = 24 * 1024;    // aim of one tile: six or more of them in flight
+
+// Ring of a launch: `row_bytes` of all loaded tensors together, `align` rows make every span a multiple of 16 bytes.
+// False where two tiles do not fit.
+struct Ring { int tile_rows, stages, grid; size_t smem; };
+inline bool ring_for(int rows, const Geometry& g, size_t row_bytes, int align, size_t acc_bytes, size_t param_bytes, Ring* out) {
+  const int per_pass = g.warps * 32 / g.lpr;
+  const size_t room = kRingBytes - param_bytes;
+  if (2 * (size_t)align * row_bytes > room) return false;
+  // whole passes of the CTA up to the aim, at least one; not so many that SMs idle, nor that two do not fit
+  long long r = per_pass;
+  while ((size_t)(r + per_pass) * row_bytes <= kTileBytes) r += per_pass;
+  const long long share = ((long long)rows + kSms - 1) / kSms;
+  if (r > share) r = share;
+  while (r > 1 && 2 * (size_t)r * row_bytes > room) r = (r + 1) / 2;
+  r = (r + align - 1) / align * align;
+  if (2 * (size_t)r * row_bytes > room) r = align;
+  const long long tiles = ((long long)rows + r - 1) / r;
+  out->tile_rows = (int)r;
+  out->grid = (int)(tiles < kSms ? tiles : kSms);
+  long long st = (long long)(room / ((size_t)r * row_bytes));
+  const long long walk = (tiles + out->grid - 1) / out->grid;   // tiles of one CTA
+  if (st > walk) st = walk;
+  if (st > kMaxStages) st = kMaxStages;
+  out->stages = (int)st;
+  size_t bytes = (size_t)st * r * row_bytes + param_bytes;
+  if (bytes < acc_bytes) bytes = acc_bytes;
+  out->smem = kRingHeader + bytes;
+  return true;
+}
+
+// Rows that make rows * C * es a multiple of 16 for the element size (16-bit tensors need the most).
+inline int align_rows(int C, int es_min) {
+  int r = 1;
+  while ((long long)r * C * es_min % 16 != 0) r *= 2;
+  return r;
+}
+
+// CTAs of the element-wise kernels.
+constexpr int kDirectThreads = 256;
+inline int direct_grid(int rows, int lpr) {
+  const int per_cta = lpr > 32 ? 1 : kDirectThreads / lpr;
+  const long long need = ((long long)rows + per_cta - 1) / per_cta, cap = 2LL * kSms;
+  return (int)(need < cap ? need : cap);
+}
+
+// What a launch will do: shared by the launcher and the workspace size.
+struct Plan {
+  Geometry g;
+  Ring ring;
+  int vec;       // elements per vector; 1 element-wise
+  bool direct;
+  int grid;
+};
+inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool base16, bool vec_ok, int rows, int C) {
+  Plan p;
+  const int V = x_es == 4 ? 4 : 8;
+  p.vec = vec_ok && base16 && C % V == 0 ? V : 1;
+  p.g = geometry(p.vec > 1 ? C / V : C, p.vec, V == 8 ? 3 : 4);
+  const int lx = backward && mode == kPre ? y_es : x_es;      // element size of the normalised tensor
+  const size_t row_bytes = (size_t)C * (backward ? lx + y_es * (1 + (mode == kPre && gh)) : x_es + (mode == kPlain ? 0 : y_es));
+  const int es_min = backward ? (lx < y_es ? lx : y_es) : (mode == kPlain || x_es < y_es ? x_es : y_es);
+  const int slots = p.g.lpr > 32 ? p.g.warps * 32 / p.g.lpr : p.g.warps;
+  const size_t acc = backward ? (size_t)slots * 2 * C * sizeof(float) : 0;
+  const size_t params = p.g.nv * p.vec > 16 ? (size_t)2 * ((C + 3) / 4 * 4) * sizeof(float) : 0;
+  p.direct = !base16 || acc > kRingBytes || !ring_for(rows, p.g, row_bytes, align_rows(C, es_min), acc, params, &p.ring);
+  if (p.direct) {
+    p.vec = 1;
+    p.g = geometry(C, 1, 0);
+    if (p.g.nv != 4) p.g.nv = 16;   // the element-wise kernels come with 4 and 16
+  }
+  p.grid = p.direct ? direct_grid(rows, p.g.lpr) : p.ring.grid;
+  return p;
 }
 
 template <typename T> struct FullVec { static constexpr int n = 16 / (int)sizeof(T); };
 
-template <typename TX, typename TY, int VEC, int NV>
-cudaError_t fwd_nv(int mode, int act, const LnTrainArgs& a, int grid, int threads, cudaStream_t s) {
-  const dim3 g((unsigned)grid), t((unsigned)threads);
-  if (mode == kPost) return launch_overlapped(ln_train_fwd_kernel<TX, TY, VEC, NV, kPost, false>, g, t, 0, s, a);
-  if (mode == kPre) return launch_overlapped(ln_train_fwd_kernel<TX, TY, VEC, NV, kPre, false>, g, t, 0, s, a);
-  if (act) return launch_overlapped(ln_train_fwd_kernel<TX, TY, VEC, NV, kPlain, true>, g, t, 0, s, a);
-  return launch_overlapped(ln_train_fwd_kernel<TX, TY, VEC, NV, kPlain, false>, g, t, 0, s, a);
-}
-template <typename TX, typename TY, int VEC, int NV>
-cudaError_t bwd_nv(int mode, int act, const LnTrainArgs& a, int grid, int threads, cudaStream_t s) {
-  const dim3 g((unsigned)grid), t((unsigned)threads);
-  const size_t smem = a.lpr > 32 ? 0 : (size_t)2 * a.C * sizeof(float);
-  if (mode == kPre) return launch_overlapped(ln_train_bwd_kernel<TY, TY, TX, TX, VEC, NV, kPre, false>, g, t, smem, s, a);
-  if (mode == kPost) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPost, false>, g, t, smem, s, a);
-  if (act) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPlain, true>, g, t, smem, s, a);
-  return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPlain, false>, g, t, smem, s, a);
+template <auto Kern>
+cudaError_t launch_ring(const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
+  static int limit[64] = {0};   // dynamic shared memory granted so far, per kernel and device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  dev &= 63;
+  if (limit[dev] == 0) {
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kRingHeader + kRingBytes));
+    if (e != cudaSuccess) return e;
+    limit[dev] = 1;
+  }
+  return launch_overlapped(Kern, dim3((unsigned)p.grid), dim3((unsigned)(32 * p.g.warps)), p.ring.smem, s, a);
 }
 
-// CTAs per SM of the backward grid: enough rows in flight, few enough partial sums.
-constexpr int kFwdPerSm = 8, kBwdPerSm = 2;
+template <typename TX, typename TY, int VEC, int NV>
+cudaError_t ring_run(bool backward, int mode, int act, const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
+  if (!backward) {
+    if (mode == kPost) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPost, false>>(a, p, s);
+    if (mode == kPre) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPre, false>>(a, p, s);
+    if (act) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPlain, true>>(a, p, s);
+    return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPlain, false>>(a, p, s);
+  }
+  if (mode == kPre) return launch_ring<ln_ring_bwd_kernel<TY, TY, TX, TX, VEC, NV, kPre, false>>(a, p, s);
+  if (mode == kPost) return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPost, false>>(a, p, s);
+  if (act) return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPlain, true>>(a, p, s);
+  return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPlain, false>>(a, p, s);
+}
+template <typename TX, typename TY, int NV>
+cudaError_t direct_run(bool backward, int mode, int act, const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
+  const dim3 g((unsigned)p.grid), t((unsigned)(p.g.lpr > 32 ? p.g.lpr : kDirectThreads));
+  if (!backward) {
+    if (mode == kPost) return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPost, false>, g, t, 0, s, a);
+    if (mode == kPre) return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPre, false>, g, t, 0, s, a);
+    if (act) return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPlain, true>, g, t, 0, s, a);
+    return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPlain, false>, g, t, 0, s, a);
+  }
+  const size_t smem = a.lpr > 32 ? 0 : (size_t)2 * a.C * sizeof(float);
+  if (mode == kPre) return launch_overlapped(ln_train_bwd_kernel<TY, TY, TX, TX, 1, NV, kPre, false>, g, t, smem, s, a);
+  if (mode == kPost) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, 1, NV, kPost, false>, g, t, smem, s, a);
+  if (act) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, 1, NV, kPlain, true>, g, t, smem, s, a);
+  return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, 1, NV, kPlain, false>, g, t, smem, s, a);
+}
 
 template <typename TX, typename TY>
-cudaError_t run(bool backward, int mode, int act, bool vec_ok, const LnTrainArgs& a0, cudaStream_t s) {
+cudaError_t run(bool backward, int mode, int act, const Plan& p, const LnTrainArgs& a0, cudaStream_t s) {
   constexpr int V = FullVec<TX>::n;
+  if (!p.g.ok) return cudaErrorInvalidValue;
   LnTrainArgs a = a0;
-  const bool scalar = !vec_ok;
-  const Geometry g = geometry(scalar ? a.C : a.C / V, scalar, V == 8 ? 3 : 4);
-  if (!g.ok) return cudaErrorInvalidValue;
-  a.lpr = g.lpr;
-  const int grid = grid_for(a.rows, g, backward ? kBwdPerSm : kFwdPerSm);
-  a.n_partial = grid;
-#define LN_RUN(VV, NN) \
-  return backward ? bwd_nv<TX, TY, VV, NN>(mode, act, a, grid, g.threads, s) : fwd_nv<TX, TY, VV, NN>(mode, act, a, grid, g.threads, s)
-  if (scalar) {
-    if (g.nv == 4) { LN_RUN(1, 4); }
-    LN_RUN(1, 16);
+  a.lpr = p.g.lpr;
+  if (p.direct) return p.g.nv == 4 ? direct_run<TX, TY, 4>(backward, mode, act, a, p, s) : direct_run<TX, TY, 16>(backward, mode, act, a, p, s);
+  a.tile_rows = p.ring.tile_rows;
+  a.stages = p.ring.stages;
+  if (p.vec == 1) {
+    if (p.g.nv == 4) return ring_run<TX, TY, 1, 4>(backward, mode, act, a, p, s);
+    if (p.g.nv == 8) return ring_run<TX, TY, 1, 8>(backward, mode, act, a, p, s);
+    if (p.g.nv == 12) return ring_run<TX, TY, 1, 12>(backward, mode, act, a, p, s);
+    return ring_run<TX, TY, 1, 16>(backward, mode, act, a, p, s);
   }
-  switch (g.nv) {
-    case 1: LN_RUN(V, 1);
-    case 2: LN_RUN(V, 2);
-    case 3: LN_RUN(V, 3);
+  switch (p.g.nv) {
+    case 1: return ring_run<TX, TY, V, 1>(backward, mode, act, a, p, s);
+    case 2: return ring_run<TX, TY, V, 2>(backward, mode, act, a, p, s);
+    case 3: return ring_run<TX, TY, V, 3>(backward, mode, act, a, p, s);
     default:
-      if constexpr (V == 4) { LN_RUN(V, 4); }
+      if constexpr (V == 4) return ring_run<TX, TY, V, 4>(backward, mode, act, a, p, s);
       return cudaErrorInvalidValue;
   }
-#undef LN_RUN
 }
 
 }  // namespace ln
