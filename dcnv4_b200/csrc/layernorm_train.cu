@@ -36,19 +36,7 @@ ln_train_params_kernel(const LnTrainArgs a, int mode) {
   float sa = 0.f, sb = 0.f;
 #pragma unroll
   for (int i = 0; i < kSlices; ++i) { const float2 u = part[i][threadIdx.x]; sa += u.x; sb += u.y; }
-  auto put = [&](void* dst, float v) {
-    if (a.param_f32) static_cast<float*>(dst)[col] = v;
-    else static_cast<P*>(dst)[col] = from_f32<P>(v);
-  };
-  if (mode == ln::kPost && a.gamma != nullptr) {
-    const float g = ln::param<P>(a.gamma, col, a.param_f32);
-    put(a.dgamma, fmaf(ln::param<P>(a.w, col, a.param_f32), sa, ln::param<P>(a.b, col, a.param_f32) * sb));
-    put(a.dw, g * sa);
-    put(a.db, g * sb);
-  } else {
-    put(a.dw, sa);
-    put(a.db, sb);
-  }
+  ln::finish_column<P>(a, mode == ln::kPost, col, sa, sb);
 }
 
 }  // namespace
@@ -90,6 +78,7 @@ cudaError_t launch_ln_train_fwd(int mode, int act, int xd, int yd, const LnTrain
 cudaError_t launch_ln_train_bwd(int mode, int act, int xd, int yd, const LnTrainArgs& a, cudaStream_t s) {
   const ln::Plan p = plan_of(true, mode, xd, yd, a);
   if (cudaError_t e = run(true, mode, act, xd, yd, p, a, s)) return e;
+  if (!p.direct && p.grid == 1) return cudaSuccess;
   LnTrainArgs f = a;
   f.n_partial = p.grid;
   const dim3 grid((unsigned)((a.C + kCols - 1) / kCols)), threads(kCols * kSlices);

@@ -30,8 +30,22 @@ def _check_tensor(t: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} tensor has to be contiguous")
 
 
+# Handle of a device's current stream without building a Stream object (2 us of a call's 15); the public route otherwise.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _on_device(t: torch.Tensor, fn, *args) -> int:
+    """fn(*args) with the tensor's device current (entered only where it is another one)."""
+    if t.get_device() == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(t.device):
+        return fn(*args)
 
 
 def _check_step(batch: int, im2col_step: int) -> None:
@@ -248,9 +262,8 @@ def layer_norm_train_supported(x: torch.Tensor, weight: torch.Tensor, out_dtype:
             and weight.dtype in (torch.float32, x.dtype) and out_dtype in (None, torch.float32, x.dtype))
 
 
-def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
-    """Argument checks of the training passes; returns (rows, C, rows_per_sample).  `x_dtype` is the dtype of the
-    branch input (x itself, except in the backward pass over a stored sum)."""
+def _refuse_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
+    """Raises for the first thing that is wrong with the arguments of a training pass; returns if nothing is."""
     C = x.shape[-1] if x.dim() else 0
     for t, n in ((x, "input"), (weight, "weight"), (bias, "bias"), (layer_scale, "layer_scale"),
                  (sample_scale, "sample_scale")):
@@ -275,13 +288,37 @@ def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_d
             _check_tensor(t, n)
             if t.shape != x.shape or t.dtype != out_dtype or t.device != x.device:
                 raise RuntimeError(f"{n} must have the shape of the input, dtype {out_dtype}, and its device")
-    rows = x.numel() // C
-    per = rows
     if sample_scale is not None:
         n = sample_scale.numel()
         if sample_scale.dtype != torch.float32 or x.dim() < 2 or (x.shape[0] % n if n else x.shape[0]) != 0:
             raise RuntimeError("sample_scale must be float32 with one factor per sample (its size divides the first "
                                "dimension of the input)")
+
+
+def _plain_cuda(t, device, dtype):
+    return t.device == device and t.dtype == dtype and t.is_contiguous()
+
+
+def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
+    """Argument checks of the training passes; returns (rows, C, rows_per_sample).  `x_dtype` is the dtype of the
+    branch input (x itself, except in the backward pass over a stored sum).  What an ordinary call looks like is
+    accepted at once; anything else goes through the checks one by one."""
+    device, shape, p_dtype = x.device, x.shape, weight.dtype
+    C = shape[-1] if shape else 0
+    if not (x.is_cuda and x.is_contiguous() and C > 0 and x.dtype in _DTYPES
+            and (sample_scale is None or (len(shape) > 1 and _plain_cuda(sample_scale, device, torch.float32)
+                                          and sample_scale.numel() > 0 and shape[0] % sample_scale.numel() == 0))
+            and x_dtype in _DTYPES and (out_dtype == torch.float32 or out_dtype == x_dtype)
+            and (p_dtype == torch.float32 or p_dtype == x_dtype)
+            and _plain_cuda(weight, device, p_dtype) and weight.numel() == C
+            and _plain_cuda(bias, device, p_dtype) and bias.numel() == C
+            and (layer_scale is None or (_plain_cuda(layer_scale, device, p_dtype) and layer_scale.numel() == C))
+            and all(t is None or (_plain_cuda(t, device, out_dtype) and t.shape == shape) for t, _ in others)):
+        _refuse_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype)
+    rows = x.numel() // C
+    per = rows
+    if sample_scale is not None:
+        n = sample_scale.numel()
         per = max(rows // n, 1) if n else 1
     return rows, C, per
 
@@ -292,16 +329,17 @@ def _ptr(t):
 
 def _ln_forward(mode, x, residual, weight, bias, eps, layer_scale, sample_scale, activation, out_dtype, what):
     rows, C, per = _check_ln(x, x.dtype, weight, bias, ((residual, "residual"),), layer_scale, sample_scale, out_dtype)
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    y = torch.empty_like(x) if out_dtype == x.dtype else x.new_empty(x.shape, dtype=out_dtype)
     h = torch.empty_like(y) if mode == _LN_PRE else None
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    with torch.cuda.device(x.device):
-        rc = _lib.lib().dcnv4b200_layernorm_train_fwd(
-            x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale),
-            y.data_ptr(), _ptr(h), mean.data_ptr(), rstd.data_ptr(), mode, _code(x), _DTYPES[out_dtype], _code(weight),
-            rows, C, per, float(eps), 1 if activation == "gelu" else 0, _stream(x))
-    _lib.check(rc, what)
+    mean = x.new_empty(rows, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    rc = _on_device(
+        x, _lib.lib().dcnv4b200_layernorm_train_fwd, x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(),
+        _ptr(layer_scale), _ptr(sample_scale), y.data_ptr(), _ptr(h), mean.data_ptr(), rstd.data_ptr(), mode,
+        _DTYPES[x.dtype], _DTYPES[out_dtype], _DTYPES[weight.dtype], rows, C, per, eps, 1 if activation == "gelu" else 0,
+        _stream(x))
+    if rc:
+        _lib.check(rc, what)
     return y, h, mean, rstd
 
 
@@ -309,30 +347,28 @@ def _ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale,
                  what):
     out_dtype = grad_y.dtype
     pre = mode == _LN_PRE
-    grads = ((grad_y, "grad_y"), (grad_h, "grad_h")) + (((x, "h"),) if pre else ())
+    grads = ((grad_y, "grad_y"), (grad_h, "grad_h"), (x, "h")) if pre else ((grad_y, "grad_y"),)
     rows, C, per = _check_ln(x, x_dtype, weight, bias, grads, layer_scale, sample_scale, out_dtype)
-    for t, n in ((mean, "mean"), (rstd, "rstd")):
-        _check_tensor(t, n)
-        if t.dtype != torch.float32 or t.numel() != rows or t.device != x.device:
-            raise RuntimeError(f"{n} must be the float32 row statistics the forward pass returned")
+    for t in (mean, rstd):
+        if not (_plain_cuda(t, x.device, torch.float32) and t.numel() == rows):
+            raise RuntimeError("mean and rstd must be the float32 row statistics the forward pass returned")
     lib = _lib.lib()
     code = _DTYPES[x_dtype]
     grad_x = torch.empty_like(x)
-    branch = torch.empty(x.shape, dtype=x_dtype, device=x.device) \
-        if pre and (sample_scale is not None or x_dtype != out_dtype) else None
-    params = torch.empty((2 if layer_scale is None else 3, C), dtype=weight.dtype, device=x.device)
+    branch = x.new_empty(x.shape, dtype=x_dtype) if pre and (sample_scale is not None or x_dtype != out_dtype) else None
+    grad_w = torch.empty_like(weight)
+    grad_b = torch.empty_like(bias)
+    grad_s = None if layer_scale is None else torch.empty_like(layer_scale)
     ws_bytes = lib.dcnv4b200_layernorm_train_bwd_workspace_bytes(code, rows, C)
-    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
-    es = params.element_size() * C
-    p0 = params.data_ptr()
-    with torch.cuda.device(x.device):
-        rc = lib.dcnv4b200_layernorm_train_bwd(
-            grad_y.data_ptr(), _ptr(grad_h), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), weight.data_ptr(),
-            bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale), grad_x.data_ptr(), _ptr(branch), p0, p0 + es,
-            None if layer_scale is None else p0 + 2 * es, ws.data_ptr(), ws_bytes, mode, code, _DTYPES[out_dtype],
-            _code(weight), rows, C, per, 1 if activation == "gelu" else 0, _stream(x))
-    _lib.check(rc, what)
-    return (grad_x, branch if branch is not None else grad_x) + params.unbind(0)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    rc = _on_device(
+        x, lib.dcnv4b200_layernorm_train_bwd, grad_y.data_ptr(), _ptr(grad_h), x.data_ptr(), mean.data_ptr(),
+        rstd.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale), grad_x.data_ptr(),
+        _ptr(branch), grad_w.data_ptr(), grad_b.data_ptr(), _ptr(grad_s), ws.data_ptr(), ws_bytes, mode, code,
+        _DTYPES[out_dtype], _DTYPES[weight.dtype], rows, C, per, 1 if activation == "gelu" else 0, _stream(x))
+    if rc:
+        _lib.check(rc, what)
+    return grad_x, grad_x if branch is None else branch, grad_w, grad_b, grad_s
 
 
 def layer_norm_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float,
@@ -354,8 +390,8 @@ def layer_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
     of.  Deterministic."""
     if activation not in ("none", "gelu"):
         raise ValueError("activation must be 'none' or 'gelu'")
-    gx, _, gw, gb = _ln_backward(_LN_PLAIN, grad_y, None, x, mean, rstd, weight, bias, None, None, activation,
-                                 x.dtype, "layer_norm_backward")
+    gx, _, gw, gb, _ = _ln_backward(_LN_PLAIN, grad_y, None, x, mean, rstd, weight, bias, None, None, activation,
+                                    x.dtype, "layer_norm_backward")
     return gx, gw, gb
 
 
@@ -378,7 +414,7 @@ def layer_norm_residual_backward(grad_out: torch.Tensor, x: torch.Tensor, mean: 
     the residual is `grad_out` itself.  Deterministic."""
     g = _ln_backward(_LN_POST, grad_out, None, x, mean, rstd, weight, bias, layer_scale, sample_scale, "none", x.dtype,
                      "layer_norm_residual_backward")
-    return g[0], g[2], g[3], (g[4] if layer_scale is not None else None)
+    return g[0], g[2], g[3], g[4]
 
 
 def add_layer_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
@@ -398,7 +434,7 @@ def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor]
     the dtype of the forward's x (default: that of h).  Without `sample_scale` and with equal dtypes the first two are
     one tensor.  Deterministic."""
     return _ln_backward(_LN_PRE, grad_y, grad_h, h, mean, rstd, weight, weight, None, sample_scale, "none",
-                        h.dtype if x_dtype is None else x_dtype, "add_layer_norm_backward")
+                        h.dtype if x_dtype is None else x_dtype, "add_layer_norm_backward")[:4]
 
 
 NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # the quintic published with the Muon optimiser
@@ -416,16 +452,15 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     a, b, c = (float(v) for v in coefficients)
     code = _code(x)
     m, n = x.shape[-2:]
-    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+    out = x.new_empty(x.shape, dtype=torch.bfloat16)
     if out.numel() == 0:
         return out
     batch = out.numel() // (m * n)
     L = _lib.lib()
     ws_bytes = L.dcnv4b200_newton_schulz_workspace_bytes(batch, m, n)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = L.dcnv4b200_newton_schulz(x.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes, code, batch, m, n,
-                                       int(steps), a, b, c, float(eps), _stream(x))
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    rc = _on_device(x, L.dcnv4b200_newton_schulz, x.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes, code, batch, m, n,
+                    int(steps), a, b, c, float(eps), _stream(x))
     _lib.check(rc, "newton_schulz")
     return out
 
