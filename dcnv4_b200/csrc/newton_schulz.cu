@@ -17,8 +17,13 @@
 // bf16 iteration: 2e-1).  In the last two steps nothing is left to amplify: a is folded into B's diagonal and X is hi.
 // The result is returned in bf16, whose own rounding is of the size of that error.
 //
-// One kernel serves the three products; a persistent CTA per SM, ten warps:
-//   warp 0     TMA loads of the two operand tiles (128 x 64 and BN x 64, 128-byte swizzle) into a ring
+// One persistent kernel runs all products of all steps.  A task is one 128 x BN tile of one product of one matrix; tasks
+// are numbered so that a task only needs earlier ones (step by step, product by product), CTAs take them in that order from
+// a counter, and each matrix counts its finished tiles: a task starts when its matrix has all tiles of the products
+// before.  Nothing waits for a whole product of the whole stack, so one product's last tiles run beside the next one's
+// first, and a single small matrix pays a flag in memory between products instead of a kernel launch.  Every task that is
+// waited for has been taken by a running CTA, so the order of progress needs no co-residency.  Ten warps:
+//   warp 0     takes tasks, waits for what they need, TMA loads of the two operand tiles (64 x 64 boxes, 128-byte swizzle)
 //   warp 1     tcgen05.mma (M 128, N BN, K 16) into one of two accumulators in tensor memory
 //   warps 2-9  epilogue: 32 x 32 units from tensor memory; the previous X (hi, lo) or A arrives by TMA in the staging
 //              buffer that the result leaves from, one unit ahead
@@ -36,16 +41,18 @@ namespace {
 using namespace tc;
 
 constexpr int kBM = 128, kBK = 64;
+constexpr int kBox = 64 * 64 * 2;              // operand box: 64 x 64 fp16
 constexpr int kEpiWarps = 8;
 constexpr int kThreadsNs = 32 * (2 + kEpiWarps);
 constexpr int kUnit = 32 * 64;                 // staging unit: 32 rows x 32 fp16 (64-byte swizzle)
 constexpr int kStagingWarp = 2 * 2 * kUnit;    // two sets of (hi or result, lo or mirror)
-constexpr int kBarBytes = 512;
+constexpr int kBarBytes = 1024;
+constexpr int kQueue = 4;                      // tasks between the warp that takes them and the others
 constexpr float kLoScale = 2048.f;
 
 enum : int { kGram = 0, kPoly = 1, kUpdate = 2 };
 
-template <int BN> constexpr int slot_bytes() { return kBM * kBK * 2 + BN * kBK * 2; }
+template <int BN> constexpr int slot_bytes() { return (2 + BN / 64) * kBox; }
 template <int BN> constexpr int ns_stages() {
   constexpr int room = 227 * 1024 - 1024 - kBarBytes - kEpiWarps * kStagingWarp;
   return room / slot_bytes<BN>() > 6 ? 6 : room / slot_bytes<BN>();
@@ -54,16 +61,24 @@ template <int BN> constexpr size_t ns_smem() {
   return (size_t)ns_stages<BN>() * slot_bytes<BN>() + kEpiWarps * kStagingWarp + kBarBytes + 1024;
 }
 
+// Tensor maps of a call: 64 x 64 boxes of the operands, 32 x 32 boxes of what an epilogue reads and writes.
+struct NsMaps {
+  CUtensorMap x[2], a, b;              // operand boxes
+  CUtensorMap xs[2], ls[2], as, bs;    // epilogue boxes
+  CUtensorMap out;                     // bf16 result
+};
+
 struct NsParams {
-  int M, N, k_blocks;
-  int m_tiles, n_tiles, tiles;   // tiles per matrix (symmetric: the lower triangle)
-  int sym;
-  long long total;               // tiles of the whole stack
+  int m, n, p, q;                // p = min, q = max
+  int tall;
+  int steps, keep;               // steps that carry the pair
+  int batch, group;              // matrices; matrices that go through the steps together
+  int sym_tiles, upd_tiles;      // tiles of a symmetric product, of an update
+  int upd_n;                     // tile columns of an update
+  long long total;
   float a, b, c;
-  int residual;                  // kUpdate: out = a * (hi + lo / 2048) + product; else: product
-  int write_lo;
-  int to_bf16;                   // kUpdate: the result leaves in bf16
-  int fold;                      // kPoly: a on the diagonal
+  unsigned* done;                // [batch] finished tiles, in epilogue warps
+  unsigned long long* ticket;    // next task
   int* status;
 };
 
@@ -88,23 +103,58 @@ __device__ __forceinline__ uint64_t smem_desc_mn(const void* tile) {
   d |= (uint64_t)2 << 61;
   return d;
 }
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
-struct Tile { int bi, mt, nt; };
-__device__ __forceinline__ Tile tile_of(long long t, const NsParams& p) {
-  Tile r;
-  r.bi = (int)(t / p.tiles);
-  const int i = (int)(t - (long long)r.bi * p.tiles);
-  if (p.sym) {  // row mt of the lower triangle starts at mt (mt + 1) / 2
-    int mt = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
-    while ((mt + 1) * (mt + 2) / 2 <= i) ++mt;
-    while (mt * (mt + 1) / 2 > i) --mt;
+// Tile columns of row block i of a symmetric product: those that reach the diagonal or lie left of it.
+template <int BN>
+__host__ __device__ inline int sym_cols(int i, int p) {
+  const int c = (i * kBM + kBM - 1) / BN + 1, most = (p + BN - 1) / BN;
+  return c < most ? c : most;
+}
+
+struct Task { int step, kind, bi, mt, nt; };
+template <int BN>
+__device__ __forceinline__ Task task_of(long long t, const NsParams& p) {
+  Task r;
+  const int per = 2 * p.sym_tiles + p.upd_tiles;
+  const long long per_group = (long long)p.group * p.steps * per;
+  const int g = (int)(t / per_group);
+  long long i = t - (long long)g * per_group;
+  const int left = p.batch - g * p.group, w = left < p.group ? left : p.group;
+  r.step = (int)(i / ((long long)w * per));
+  i -= (long long)r.step * w * per;
+  const long long ws = (long long)w * p.sym_tiles;
+  int tile;
+  if (i < 2 * ws) {
+    r.kind = i < ws ? kGram : kPoly;
+    if (i >= ws) i -= ws;
+    r.bi = (int)(i / p.sym_tiles);
+    tile = (int)(i - (long long)r.bi * p.sym_tiles);
+    int mt = 0;
+    for (int c = sym_cols<BN>(0, p.p); tile >= c; c = sym_cols<BN>(mt, p.p)) { tile -= c; ++mt; }
     r.mt = mt;
-    r.nt = i - mt * (mt + 1) / 2;
+    r.nt = tile;
   } else {
-    r.mt = i / p.n_tiles;
-    r.nt = i - r.mt * p.n_tiles;
+    i -= 2 * ws;
+    r.kind = kUpdate;
+    r.bi = (int)(i / p.upd_tiles);
+    tile = (int)(i - (long long)r.bi * p.upd_tiles);
+    r.mt = tile / p.upd_n;
+    r.nt = tile - r.mt * p.upd_n;
   }
+  r.bi += g * p.group;
   return r;
+}
+// Epilogue warps of the task's matrix that must have finished before it may start.
+__device__ __forceinline__ unsigned needs(const Task& t, const NsParams& p) {
+  const int per = 2 * p.sym_tiles + p.upd_tiles;
+  const int before = t.step * per + (t.kind == kGram ? 0 : t.kind == kPoly ? p.sym_tiles : 2 * p.sym_tiles);
+  return (unsigned)before * kEpiWarps;
 }
 
 __device__ __forceinline__ uint32_t pack_h(float x, float y) {
@@ -117,36 +167,39 @@ __device__ __forceinline__ uint32_t pack_b(float x, float y) {
 }
 __device__ __forceinline__ float2 unpack_h(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-// TA / TB: the operand is MN-major (its rows are the reduction's).
-template <int BN, bool TA, bool TB, int EPI>
+template <int BN>
 __global__ void __launch_bounds__(kThreadsNs, 1)
-ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ CUtensorMap map_r0, const __grid_constant__ CUtensorMap map_r1,
-               const __grid_constant__ CUtensorMap map_o0, const __grid_constant__ CUtensorMap map_o1,
-               const NsParams p) {
+ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int kStages = ns_stages<BN>();
-  constexpr uint32_t kBytesA = kBM * kBK * 2, kBytesB = BN * kBK * 2;
-  unsigned char* ring_a = smem;
-  unsigned char* ring_b = smem + kStages * kBytesA;
-  unsigned char* staging = smem + kStages * (kBytesA + kBytesB);
+  constexpr uint32_t kSlot = slot_bytes<BN>();
+  unsigned char* ring = smem;                      // per slot: A (2 boxes), B (BN / 64 boxes)
+  unsigned char* staging = smem + kStages * kSlot;
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingWarp);
   uint64_t* full = bars;
-  uint64_t* empty = bars + kStages;
-  uint64_t* acc_full = bars + 2 * kStages;
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* res_bars = acc_empty + 2;            // [kEpiWarps][2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_bars + 2 * kEpiWarps);
+  uint64_t* task_full = acc_empty + 2;             // [kQueue]
+  uint64_t* task_empty = task_full + kQueue;
+  uint64_t* res_bars = task_empty + kQueue;        // [kEpiWarps][2]
+  volatile long long* queue = reinterpret_cast<volatile long long*>(res_bars + 2 * kEpiWarps);  // [kQueue], -1 ends
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<long long*>(queue) + kQueue);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t kTmemCols = 2 * BN;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], kEpiWarps); }
-    for (int w = 0; w < 2 * kEpiWarps; ++w) mbar_init(&res_bars[w], 1);
+    auto init = [](uint64_t* bar, uint32_t count) {   // one fence for all of them below
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+    };
+    for (int s = 0; s < kStages; ++s) { init(&full[s], 1); init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { init(&acc_full[a], 1); init(&acc_empty[a], kEpiWarps); }
+    for (int q = 0; q < kQueue; ++q) { init(&task_full[q], 1); init(&task_empty[q], 1 + kEpiWarps); }
+    for (int w = 0; w < 2 * kEpiWarps; ++w) init(&res_bars[w], 1);
     *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
@@ -157,30 +210,56 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   pdl_trigger();
 
   auto give_up = [&] { atomicExch(p.status, kStatusStageTimeout); *abort_flag = 1; };
+  // operand orientation of a task: the tile's rows are the reduction's (MN-major)?
+  auto a_mn = [&](int kind) { return kind == kGram && p.tall; };
+  auto b_mn = [&](int kind) { return kind == kGram ? p.tall != 0 : kind == kUpdate && !p.tall; };
+  auto k_blocks = [&](int kind) { return ((kind == kGram ? p.q : p.p) + kBK - 1) / kBK; };
 
   if (warp == 0) {
     if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
+      int stage = 0, slot = 0;
+      uint32_t phase = 0, qphase = 0;
       pdl_wait();
-      for (long long t = blockIdx.x; t < p.total && !*abort_flag; t += gridDim.x) {
-        const Tile q = tile_of(t, p);
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!mbar_wait_bounded(&empty[stage], phase ^ 1)) { give_up(); break; }
-          mbar_expect_tx(&full[stage], kBytesA + kBytesB);
-          unsigned char* da = ring_a + stage * kBytesA;
-          unsigned char* db = ring_b + stage * kBytesB;
-          if (TA) {
-#pragma unroll
-            for (int i = 0; i < kBM / 64; ++i) tma_load_3d(da + i * 8192, &map_a, q.mt * kBM + i * 64, kb * kBK, q.bi, &full[stage]);
-          } else {
-            tma_load_3d(da, &map_a, kb * kBK, q.mt * kBM, q.bi, &full[stage]);
+      while (!*abort_flag) {
+        long long t = (long long)atomicAdd(p.ticket, 1ULL);
+        if (t >= p.total) t = -1;
+        Task q;
+        if (t >= 0) {
+          q = task_of<BN>(t, p);
+          const unsigned want = needs(q, p);
+          if (want) {
+            int spins = 0;
+            while (load_acquire(p.done + q.bi) < want) {
+              if (*abort_flag || ++spins > (1 << 25)) { give_up(); break; }
+            }
+            if (*abort_flag) break;
           }
-          if (TB) {
+          fence_async();       // what other CTAs stored by TMA is about to be loaded by TMA
+        }
+        if (!mbar_wait_bounded(&task_empty[slot], qphase ^ 1)) { give_up(); break; }
+        queue[slot] = t;
+        mbar_arrive(&task_full[slot]);
+        if (++slot == kQueue) { slot = 0; qphase ^= 1; }
+        if (t < 0) break;
+        const bool ta = a_mn(q.kind), tb = b_mn(q.kind);
+        const CUtensorMap* mx = &maps.x[q.step & 1];
+        const CUtensorMap* ma = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? mx : &maps.b);
+        const CUtensorMap* mb = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? &maps.b : mx);
+        const int kb_n = k_blocks(q.kind);
+        for (int kb = 0; kb < kb_n; ++kb) {
+          if (!mbar_wait_bounded(&empty[stage], phase ^ 1)) { give_up(); break; }
+          mbar_expect_tx(&full[stage], kSlot);
+          unsigned char* da = ring + stage * kSlot;
+          unsigned char* db = da + 2 * kBox;
 #pragma unroll
-            for (int i = 0; i < BN / 64; ++i) tma_load_3d(db + i * 8192, &map_b, q.nt * BN + i * 64, kb * kBK, q.bi, &full[stage]);
-          } else {
-            tma_load_3d(db, &map_b, kb * kBK, q.nt * BN, q.bi, &full[stage]);
+          for (int i = 0; i < 2; ++i) {
+            const int mn = q.mt * kBM + i * 64;
+            tma_load_3d(da + i * kBox, ma, ta ? mn : kb * kBK, ta ? kb * kBK : mn, q.bi, &full[stage]);
+          }
+#pragma unroll
+          for (int i = 0; i < BN / 64; ++i) {
+            const int mn = q.nt * BN + i * 64;
+            tma_load_3d(db + i * kBox, mb, tb ? mn : kb * kBK, tb ? kb * kBK : mn, q.bi, &full[stage]);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -188,21 +267,30 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = instr_desc<__half>(BN) | ((uint32_t)TA << 15) | ((uint32_t)TB << 16);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      for (long long t = blockIdx.x; t < p.total && !*abort_flag; t += gridDim.x) {
+      int stage = 0, acc = 0, slot = 0;
+      uint32_t phase = 0, acc_phase = 0, qphase = 0;
+      while (!*abort_flag) {
+        if (!mbar_wait_bounded(&task_full[slot], qphase)) { give_up(); break; }
+        const long long t = queue[slot];
+        mbar_arrive(&task_empty[slot]);
+        if (++slot == kQueue) { slot = 0; qphase ^= 1; }
+        if (t < 0) break;
+        const int kind = task_of<BN>(t, p).kind;
+        const bool ta = a_mn(kind), tb = b_mn(kind);
+        const uint32_t idesc = instr_desc<__half>(BN) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
+        const uint64_t step_a = ta ? 128 : 2, step_b = tb ? 128 : 2;  // 16 of K: 16 rows of an MN-major box, 32 bytes of a K-major row
+        const int kb_n = k_blocks(kind);
         if (!mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1)) { give_up(); break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = 0; kb < kb_n; ++kb) {
           if (!mbar_wait_bounded(&full[stage], phase)) { give_up(); break; }
           tc_fence_after();
-          const uint64_t da = TA ? smem_desc_mn(ring_a + stage * kBytesA) : smem_desc_sw128(ring_a + stage * kBytesA);
-          const uint64_t db = TB ? smem_desc_mn(ring_b + stage * kBytesB) : smem_desc_sw128(ring_b + stage * kBytesB);
+          unsigned char* da = ring + stage * kSlot;
+          const uint64_t a0 = ta ? smem_desc_mn(da) : smem_desc_sw128(da);
+          const uint64_t b0 = tb ? smem_desc_mn(da + 2 * kBox) : smem_desc_sw128(da + 2 * kBox);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k)  // 16 of K: 32 bytes along a K-major row, 16 rows of an MN-major tile
-            tc_mma_f16(d_tmem, da + (uint64_t)(k * (TA ? 128 : 2)), db + (uint64_t)(k * (TB ? 128 : 2)), idesc, (kb | k) != 0);
+          for (int k = 0; k < kBK / 16; ++k) tc_mma_f16(d_tmem, a0 + k * step_a, b0 + k * step_b, idesc, (kb | k) != 0);
           tc_commit(&empty[stage]);
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -215,47 +303,73 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     constexpr int kCols = BN / 2, kUnits = kCols / 32;  // columns and units of this warp's share of a tile
     unsigned char* buf = staging + (warp - 2) * kStagingWarp;
     uint64_t* res_bar = &res_bars[2 * (warp - 2)];
-    const bool has_res = EPI == kPoly || (EPI == kUpdate && p.residual);
-    uint32_t unit = 0;
+    uint32_t unit = 0, fetch_phase = 0;                  // bit i: phase of set i's next fetch
+    int slot = 0, acc = 0;
+    uint32_t qphase = 0, acc_phase = 0;
     pdl_wait();
-    // ask for the tile of the previous X or A that unit `u` of tile `t` needs
-    auto fetch = [&](long long t, int u, uint32_t k) {
-      const Tile q = tile_of(t, p);
-      const int col = q.nt * BN + group * kCols + u * 32, row = q.mt * kBM + quad * 32;
-      unsigned char* set = buf + (k & 1) * 2 * kUnit;
-      mbar_expect_tx(&res_bar[k & 1], EPI == kUpdate ? 2 * kUnit : kUnit);
-      tma_load_3d(set, &map_r0, col, row, q.bi, &res_bar[k & 1]);
-      if (EPI == kUpdate) tma_load_3d(set + kUnit, &map_r1, col, row, q.bi, &res_bar[k & 1]);
-    };
-    if (has_res && lane == 0 && blockIdx.x < p.total) fetch(blockIdx.x, 0, 0);
-    long long t = blockIdx.x;
-    for (uint32_t it = 0; t < p.total && !*abort_flag; t += gridDim.x, ++it) {
-      const int acc = (int)(it & 1);
-      const Tile q = tile_of(t, p);
-      if (!mbar_wait_bounded(&acc_full[acc], (it >> 1) & 1)) { if (lane == 0) give_up(); break; }
+    while (!*abort_flag) {
+      if (!mbar_wait_bounded(&task_full[slot], qphase)) { if (lane == 0) give_up(); break; }
+      const long long t = queue[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&task_empty[slot]);
+      if (++slot == kQueue) { slot = 0; qphase ^= 1; }
+      if (t < 0) break;
+      const Task q = task_of<BN>(t, p);
+      const int kind = q.kind;
+      const bool pair = q.step < p.keep, last = q.step == p.steps - 1;
+      const bool res = kind == kUpdate && pair;          // a * (hi + lo / 2048) is added
+      const bool has_res = kind == kPoly || res;
+      const bool write_lo = kind == kUpdate && q.step + 1 < p.keep;
+      const bool bf16 = kind == kUpdate && last;
+      const float diag = kind == kPoly && !pair ? p.a : 0.f;  // a folded into B
+      const CUtensorMap* r0 = kind == kPoly ? &maps.as : &maps.xs[q.step & 1];
+      const CUtensorMap* r1 = &maps.ls[q.step & 1];
+      const CUtensorMap* o0 = kind == kGram ? &maps.as : kind == kPoly ? &maps.bs : (last ? &maps.out : &maps.xs[(q.step & 1) ^ 1]);
+      const CUtensorMap* o1 = &maps.ls[(q.step & 1) ^ 1];
+      const int rows = kind == kUpdate ? p.m : p.p, cols = kind == kUpdate ? p.n : p.p;
+      const int row0 = q.mt * kBM + quad * 32, colw = q.nt * BN + group * kCols;
+      const bool rows_in = row0 < rows;                  // else this warp's quarter lies below the matrix
+      // ask for the unit of the previous X or A that unit `u` needs
+      auto fetch = [&](int u, uint32_t k) {
+        unsigned char* set = buf + (k & 1) * 2 * kUnit;
+        mbar_expect_tx(&res_bar[k & 1], res ? 2 * kUnit : kUnit);
+        tma_load_3d(set, r0, colw + u * 32, row0, q.bi, &res_bar[k & 1]);
+        if (res) tma_load_3d(set + kUnit, r1, colw + u * 32, row0, q.bi, &res_bar[k & 1]);
+      };
+      int units = rows_in ? (cols - colw + 31) / 32 : 0;   // units with any column of the matrix
+      units = units < 0 ? 0 : (units > kUnits ? kUnits : units);
+      if (has_res && units > 0 && lane == 0) {
+        fence_async();
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        fetch(0, unit);
+      }
+      if (!mbar_wait_bounded(&acc_full[acc], acc_phase)) { if (lane == 0) give_up(); break; }
       tc_fence_after();
-      const int row0 = q.mt * kBM + quad * 32;
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + group * kCols);
 #pragma unroll 1
-      for (int u = 0; u < kUnits; ++u, ++unit) {
-        const int col0 = q.nt * BN + group * kCols + u * 32;
-        unsigned char* set = buf + (unit & 1) * 2 * kUnit;
+      for (int u = 0; u < units; ++u, ++unit) {
+        const int col0 = colw + u * 32;
+        const int set_i = (int)(unit & 1);
+        unsigned char* set = buf + set_i * 2 * kUnit;
         uint32_t v[32];
         tmem_ld_32x32(taddr + (uint32_t)(u * 32), v);
         if (lane == 0) {
           if (has_res) {
             // the other set is free once the store of the previous unit has read it
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            if (u + 1 < kUnits) fetch(t, u + 1, unit + 1);
-            else if (t + gridDim.x < p.total) fetch(t + gridDim.x, 0, unit + 1);
+            if (u + 1 < units) fetch(u + 1, unit + 1);
           } else {
             asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
           }
         }
         __syncwarp();
-        if (has_res && !mbar_wait_bounded(&res_bar[unit & 1], (unit >> 1) & 1)) { if (lane == 0) give_up(); }
+        if (has_res) {
+          if (!mbar_wait_bounded(&res_bar[set_i], (fetch_phase >> set_i) & 1)) { if (lane == 0) give_up(); }
+          fetch_phase ^= 1u << set_i;
+        }
         tmem_ld_wait();
-        const bool mirror = EPI != kUpdate && p.sym && q.mt != q.nt;
+        // a unit below the diagonal whose mirror image no tile computes is stored there as well
+        const bool mirror = kind != kUpdate && row0 > col0 && row0 / BN >= sym_cols<BN>(col0 / kBM, p.p);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           // 64-byte swizzle: 16-byte piece index xor bits 1-2 of the row
@@ -263,7 +377,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v[j + e]);
-          if (EPI == kPoly) {
+          if (kind == kPoly) {
             const uint4 r = *reinterpret_cast<const uint4*>(set + off);
             const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -272,13 +386,13 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
               x[2 * e] = fmaf(p.c, x[2 * e], p.b * f.x);
               x[2 * e + 1] = fmaf(p.c, x[2 * e + 1], p.b * f.y);
             }
-            if (p.fold && row0 + lane >= col0 + j && row0 + lane < col0 + j + 8) {
+            if (row0 + lane >= col0 + j && row0 + lane < col0 + j + 8) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                if (row0 + lane == col0 + j + e) x[e] += p.a;
+                if (row0 + lane == col0 + j + e) x[e] += diag;
             }
           }
-          if (EPI == kUpdate && p.residual) {
+          if (res) {
             const uint4 h = *reinterpret_cast<const uint4*>(set + off);
             const uint4 l = *reinterpret_cast<const uint4*>(set + kUnit + off);
             const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
@@ -290,7 +404,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
           }
           uint32_t o[4];
-          if (EPI == kUpdate && p.to_bf16) {
+          if (bf16) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = pack_b(x[2 * e], x[2 * e + 1]);
           } else {
@@ -298,7 +412,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             for (int e = 0; e < 4; ++e) o[e] = pack_h(x[2 * e], x[2 * e + 1]);
           }
           *reinterpret_cast<uint4*>(set + off) = make_uint4(o[0], o[1], o[2], o[3]);
-          if (EPI == kUpdate && p.write_lo) {
+          if (write_lo) {
             uint32_t l[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -319,17 +433,23 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-          if (row0 < p.M && col0 < p.N) {
-            tma_store_3d(&map_o0, set, col0, row0, q.bi);
-            if (EPI == kUpdate && p.write_lo) tma_store_3d(&map_o1, set + kUnit, col0, row0, q.bi);
-            if (mirror) tma_store_3d(&map_o0, set + kUnit, row0, col0, q.bi);
-          }
+          tma_store_3d(o0, set, col0, row0, q.bi);
+          if (write_lo) tma_store_3d(o1, set + kUnit, col0, row0, q.bi);
+          if (mirror) tma_store_3d(o0, set + kUnit, row0, col0, q.bi);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (lane == 0) {
+        mbar_arrive(&acc_empty[acc]);
+        // the tile's stores are complete, hence visible, before the matrix counts this warp
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        fence_async();
+        __threadfence();
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + q.bi) : "memory");
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -357,10 +477,15 @@ template <typename T> __device__ __forceinline__ float load1(const T* p) { retur
 // Sum of squares of one slice of one matrix, in 64 bits (fp32 squares of large gradients would overflow).
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
-ns_square_kernel(const T* __restrict__ x, double* __restrict__ partial, long long per, long long chunk, int vec) {
+ns_square_kernel(const T* __restrict__ x, double* __restrict__ partial, long long per, long long chunk, int vec,
+                 unsigned* __restrict__ done, unsigned long long* __restrict__ ticket) {
   __shared__ double part[kNormThreads / 32];
   pdl_trigger();
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {   // the counters of the kernel after next
+    done[blockIdx.y] = 0;
+    if (blockIdx.y == 0) *ticket = 0;
+  }
   const T* src = x + (long long)blockIdx.y * per;
   const long long lo = (long long)blockIdx.x * chunk;
   const long long hi = lo + chunk < per ? lo + chunk : per;
@@ -472,46 +597,11 @@ bool map3(CUtensorMap* m, bool bf16, const void* base, long long batch, long lon
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct Mat { const void* p; long long rows; int cols, ld; };
-
-template <int BN, bool TA, bool TB, int EPI>
-cudaError_t launch_gemm(const Mat& A, const Mat& B, const Mat& r0, const Mat& r1, const Mat& o0, const Mat& o1,
-                        long long batch, NsParams p, int M, int N, int K, bool sym, int sms, cudaStream_t s) {
-  static std::once_flag once[64];
-  static cudaError_t attr_err[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  dev = dev < 0 || dev >= 64 ? 0 : dev;
-  std::call_once(once[dev], [&] {
-    attr_err[dev] = cudaFuncSetAttribute(ns_gemm_kernel<BN, TA, TB, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)ns_smem<BN>());
-  });
-  if (attr_err[dev] != cudaSuccess) return attr_err[dev];
-  CUtensorMap ma, mb, m0, m1, n0, n1;
-  if (!map3(&ma, false, A.p, batch, A.rows, A.cols, A.ld, TA ? 64 : kBM, 64) ||
-      !map3(&mb, false, B.p, batch, B.rows, B.cols, B.ld, TB ? 64 : BN, 64) ||
-      !map3(&m0, false, r0.p, batch, r0.rows, r0.cols, r0.ld, 32, 32) ||
-      !map3(&m1, false, r1.p, batch, r1.rows, r1.cols, r1.ld, 32, 32) ||
-      !map3(&n0, p.to_bf16 != 0, o0.p, batch, o0.rows, o0.cols, o0.ld, 32, 32) ||
-      !map3(&n1, false, o1.p, batch, o1.rows, o1.cols, o1.ld, 32, 32))
-    return cudaErrorNotSupported;
-  p.M = M; p.N = N;
-  p.k_blocks = (K + kBK - 1) / kBK;
-  p.m_tiles = (M + kBM - 1) / kBM;
-  p.n_tiles = (N + BN - 1) / BN;
-  p.sym = sym;
-  p.tiles = sym ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles;
-  p.total = batch * p.tiles;
-  const unsigned grid = (unsigned)(p.total < sms ? p.total : sms);
-  return launch_overlapped(ns_gemm_kernel<BN, TA, TB, EPI>, dim3(grid), dim3(kThreadsNs), ns_smem<BN>(), s, ma, mb, m0,
-                           m1, n0, n1, p);
-}
-
 inline long long pad8(long long v) { return (v + 7) / 8 * 8; }
 inline size_t pad1k(size_t v) { return (v + 1023) / 1024 * 1024; }
 
 struct Layout {
-  size_t x[2], l[2], a, b, norm, total;
+  size_t x[2], l[2], a, b, norm, done, ticket, total;
   int ldn, ldp;
 };
 Layout layout_of(long long batch, int m, int n) {
@@ -526,8 +616,36 @@ Layout layout_of(long long batch, int m, int n) {
   w.a = at; at += ab;
   w.b = at; at += ab;
   w.norm = at; at += pad1k((size_t)batch * kMaxChunks * sizeof(double));
+  w.ticket = at;                   // 8 bytes, the per-matrix counts behind them
+  w.done = at + 8; at += pad1k(8 + (size_t)batch * sizeof(unsigned));
   w.total = at;
   return w;
+}
+
+#ifndef DCNB200_NS_BN
+#define DCNB200_NS_BN 0
+#endif
+
+template <int BN>
+cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev = dev < 0 || dev >= 64 ? 0 : dev;
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(ns_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ns_smem<BN>());
+  });
+  if (attr_err[dev] != cudaSuccess) return attr_err[dev];
+  p.sym_tiles = 0;
+  for (int i = 0; i < (p.p + kBM - 1) / kBM; ++i) p.sym_tiles += sym_cols<BN>(i, p.p);
+  p.upd_n = (p.n + BN - 1) / BN;
+  p.upd_tiles = (p.m + kBM - 1) / kBM * p.upd_n;
+  p.total = (long long)p.batch * p.steps * (2 * p.sym_tiles + p.upd_tiles);
+  // more CTAs than a product has tiles would only wait
+  const long long most = (long long)p.batch * (p.sym_tiles > p.upd_tiles ? p.sym_tiles : p.upd_tiles);
+  const unsigned grid = (unsigned)(most < sms ? most : sms);
+  return launch_overlapped(ns_kernel<BN>, dim3(grid), dim3(kThreadsNs), ns_smem<BN>(), s, maps, p);
 }
 
 template <typename T>
@@ -546,7 +664,8 @@ cudaError_t prepare(const void* x, const Layout& w, unsigned char* ws, long long
   double* partial = reinterpret_cast<double*>(ws + w.norm);
   const T* src = static_cast<const T*>(x);
   cudaError_t e = launch_overlapped(ns_square_kernel<T>, dim3((unsigned)chunks, (unsigned)batch), dim3(kNormThreads), 0, s,
-                                    src, partial, per, chunk, (int)vec);
+                                    src, partial, per, chunk, (int)vec, reinterpret_cast<unsigned*>(ws + w.done),
+                                    reinterpret_cast<unsigned long long*>(ws + w.ticket));
   if (e != cudaSuccess) return e;
   long long blocks = (8LL * sms + batch - 1) / batch;
   if (blocks > most) blocks = most;
@@ -567,34 +686,37 @@ cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* work
   cudaError_t e = dtype == 0   ? prepare<float>(x, w, ws, batch, m, n, eps, sms, s)
                   : dtype == 1 ? prepare<__half>(x, w, ws, batch, m, n, eps, sms, s)
                                : prepare<__nv_bfloat16>(x, w, ws, batch, m, n, eps, sms, s);
-  const bool tall = m > n;
-  const int pd = tall ? n : m, qd = tall ? m : n;
-  const Mat A{ws + w.a, pd, pd, w.ldp}, B{ws + w.b, pd, pd, w.ldp};
+  if (e != cudaSuccess) return e;
   const bool direct = n % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const int keep = steps - 2;      // steps that carry the pair
-  for (int k = 0; k < steps && e == cudaSuccess; ++k) {
-    const int cur = k & 1, nxt = cur ^ 1;
-    const Mat X{ws + w.x[cur], m, n, w.ldn}, L{ws + w.l[cur], m, n, w.ldn};
-    const bool last = k == steps - 1;
-    Mat O{ws + w.x[nxt], m, n, w.ldn};
-    const Mat OL{ws + w.l[nxt], m, n, w.ldn};
-    if (last && direct) O = Mat{out, m, n, n};
-    NsParams p = {};
-    p.a = a; p.b = b; p.c = c; p.status = status;
-    p.residual = k < keep;
-    p.fold = !p.residual;
-    p.write_lo = k + 1 < keep;
-    if (tall) e = launch_gemm<128, true, true, kGram>(X, X, A, A, A, A, batch, p, pd, pd, qd, true, sms, s);
-    else e = launch_gemm<128, false, false, kGram>(X, X, A, A, A, A, batch, p, pd, pd, qd, true, sms, s);
-    if (e != cudaSuccess) break;
-    e = launch_gemm<128, false, false, kPoly>(A, A, A, A, B, B, batch, p, pd, pd, pd, true, sms, s);
-    if (e != cudaSuccess) break;
-    p.to_bf16 = last;
-    if (tall) e = n > 128 ? launch_gemm<256, false, false, kUpdate>(X, B, X, L, O, OL, batch, p, m, n, pd, false, sms, s)
-                          : launch_gemm<128, false, false, kUpdate>(X, B, X, L, O, OL, batch, p, m, n, pd, false, sms, s);
-    else e = n > 128 ? launch_gemm<256, false, true, kUpdate>(B, X, X, L, O, OL, batch, p, m, n, pd, false, sms, s)
-                     : launch_gemm<128, false, true, kUpdate>(B, X, X, L, O, OL, batch, p, m, n, pd, false, sms, s);
+  NsParams p = {};
+  p.m = m; p.n = n; p.tall = m > n;
+  p.p = p.tall ? n : m; p.q = p.tall ? m : n;
+  p.steps = steps; p.keep = steps - 2;
+  p.batch = (int)batch; p.group = (int)batch;
+  p.a = a; p.b = b; p.c = c;
+  p.done = reinterpret_cast<unsigned*>(ws + w.done);
+  p.ticket = reinterpret_cast<unsigned long long*>(ws + w.ticket);
+  p.status = status;
+  NsMaps maps;
+  bool ok = true;
+  for (int i = 0; i < 2; ++i) {
+    ok = ok && map3(&maps.x[i], false, ws + w.x[i], batch, m, n, w.ldn, 64, 64);
+    ok = ok && map3(&maps.xs[i], false, ws + w.x[i], batch, m, n, w.ldn, 32, 32);
+    ok = ok && map3(&maps.ls[i], false, ws + w.l[i], batch, m, n, w.ldn, 32, 32);
   }
+  ok = ok && map3(&maps.a, false, ws + w.a, batch, p.p, p.p, w.ldp, 64, 64) &&
+       map3(&maps.b, false, ws + w.b, batch, p.p, p.p, w.ldp, 64, 64) &&
+       map3(&maps.as, false, ws + w.a, batch, p.p, p.p, w.ldp, 32, 32) &&
+       map3(&maps.bs, false, ws + w.b, batch, p.p, p.p, w.ldp, 32, 32);
+  // a result whose rows 16-byte stores cannot address goes through the padded buffer the last step does not read
+  ok = ok && (direct ? map3(&maps.out, true, out, batch, m, n, n, 32, 32)
+                     : map3(&maps.out, true, ws + w.x[steps & 1], batch, m, n, w.ldn, 32, 32));
+  if (!ok) return cudaErrorNotSupported;
+  // Tile width: the widest whose update still gives every SM a tile.
+  const long long rows = (m + kBM - 1) / kBM;
+  const int width = DCNB200_NS_BN ? DCNB200_NS_BN
+                    : batch * rows * ((n + 255) / 256) >= sms ? 256 : batch * rows * ((n + 127) / 128) >= sms ? 128 : 64;
+  e = width == 256 ? launch_ns<256>(maps, p, sms, s) : width == 128 ? launch_ns<128>(maps, p, sms, s) : launch_ns<64>(maps, p, sms, s);
   if (e == cudaSuccess && !direct) {
     const long long total = batch * (long long)m * n;
     long long blocks = (total + kNormThreads - 1) / kNormThreads;
