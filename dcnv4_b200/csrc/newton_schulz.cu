@@ -22,11 +22,12 @@
 // a counter, and each matrix counts its finished tiles: a task starts when its matrix has all tiles of the products
 // before.  Nothing waits for a whole product of the whole stack, so one product's last tiles run beside the next one's
 // first, and a single small matrix pays a flag in memory between products instead of a kernel launch.  Every task that is
-// waited for has been taken by a running CTA, so the order of progress needs no co-residency.  Ten warps:
+// waited for has been taken by a running CTA, so the order of progress needs no co-residency.  Warps:
 //   warp 0     takes tasks, waits for what they need, TMA loads of the two operand tiles (64 x 64 boxes, 128-byte swizzle)
 //   warp 1     tcgen05.mma (M 128, N BN, K 16) into one of two accumulators in tensor memory
-//   warps 2-9  epilogue: 32 x 32 units from tensor memory; the previous X (hi, lo) or A arrives by TMA in the staging
-//              buffer that the result leaves from, one unit ahead
+//   last warp  counts the finished tiles
+//   others     epilogue: 32 x 32 units from tensor memory; the previous X (hi, lo) or A arrives by TMA
+//              in the staging buffer that the result leaves from
 // Every mbarrier wait is bounded; one that runs out sets the device status word and the CTA winds down.
 //
 // The reference has no optimiser kernels; its trainers use stock AdamW (classification/optimizer.py).
@@ -42,23 +43,25 @@ using namespace tc;
 
 constexpr int kBM = 128, kBK = 64;
 constexpr int kBox = 64 * 64 * 2;              // operand box: 64 x 64 fp16
-constexpr int kEpiWarps = 8;
-constexpr int kThreadsNs = 32 * (2 + kEpiWarps);
+// Epilogue warps: four quarters of the accumulator's rows, each in up to four column groups of at least 32.
+template <int BN> constexpr int epi_groups() { return BN / 32 < 4 ? BN / 32 : 4; }
+template <int BN> constexpr int epi_warps() { return 4 * epi_groups<BN>(); }
+template <int BN> constexpr int ns_threads() { return 32 * (3 + epi_warps<BN>()); }
 constexpr int kUnit = 32 * 64;                 // staging unit: 32 rows x 32 fp16 (64-byte swizzle)
-constexpr int kStagingWarp = 2 * 2 * kUnit;    // two sets of (hi or result, lo or mirror)
+constexpr int kStagingWarp = 2 * kUnit;        // hi or result, and lo or mirror
 constexpr int kBarBytes = 1024;
-constexpr int kQueue = 4;                      // tasks between the warp that takes them and the others
+constexpr int kQueue = 4;                      // tasks between the warp that takes them and the others, tiles to be counted
 constexpr float kLoScale = 2048.f;
 
 enum : int { kGram = 0, kPoly = 1, kUpdate = 2 };
 
 template <int BN> constexpr int slot_bytes() { return (2 + BN / 64) * kBox; }
 template <int BN> constexpr int ns_stages() {
-  constexpr int room = 227 * 1024 - 1024 - kBarBytes - kEpiWarps * kStagingWarp;
+  constexpr int room = 227 * 1024 - 1024 - kBarBytes - epi_warps<BN>() * kStagingWarp;
   return room / slot_bytes<BN>() > 6 ? 6 : room / slot_bytes<BN>();
 }
 template <int BN> constexpr size_t ns_smem() {
-  return (size_t)ns_stages<BN>() * slot_bytes<BN>() + kEpiWarps * kStagingWarp + kBarBytes + 1024;
+  return (size_t)ns_stages<BN>() * slot_bytes<BN>() + epi_warps<BN>() * kStagingWarp + kBarBytes + 1024;
 }
 
 // Tensor maps of a call: 64 x 64 boxes of the operands, 32 x 32 boxes of what an epilogue reads and writes.
@@ -72,13 +75,13 @@ struct NsParams {
   int m, n, p, q;                // p = min, q = max
   int tall;
   int steps, keep;               // steps that carry the pair
-  int batch, group;              // matrices; matrices that go through the steps together
+  int batch;
   int sym_tiles, upd_tiles;      // tiles of a symmetric product, of an update
   int upd_n;                     // tile columns of an update
-  long long total;
+  unsigned total;                // tasks
   float a, b, c;
-  unsigned* done;                // [batch] finished tiles, in epilogue warps
-  unsigned long long* ticket;    // next task
+  unsigned* done;                // [batch] finished tiles
+  unsigned* ticket;              // next task
   int* status;
 };
 
@@ -108,7 +111,22 @@ __device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+// One lane of a converged warp.  The tensor-core and TMA instructions take their operands from uniform registers: behind
+// a plain `lane == 0` the compiler cannot tell that one lane is left and serialises each of them (measured: 0.38 us for
+// every 64 of K, whatever the tile's width).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {   // without suspending, unlike try_wait
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Global memory written through the async proxy elsewhere and known through a flag is about to be read through it here.
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 // Tile columns of row block i of a symmetric product: those that reach the diagonal or lie left of it.
 template <int BN>
@@ -118,43 +136,37 @@ __host__ __device__ inline int sym_cols(int i, int p) {
 }
 
 struct Task { int step, kind, bi, mt, nt; };
+// Task order: step by step, product by product, matrix by matrix.  (Groups of matrices a product apart, so that long and
+// short products run side by side, were slower: 733 against 677 us for 22 x 640x2560.  CTAs take tasks in order and the
+// distance between a matrix' product and its next one shrinks.)
 template <int BN>
-__device__ __forceinline__ Task task_of(long long t, const NsParams& p) {
+__device__ __forceinline__ Task task_of(unsigned t, const NsParams& p) {
   Task r;
-  const int per = 2 * p.sym_tiles + p.upd_tiles;
-  const long long per_group = (long long)p.group * p.steps * per;
-  const int g = (int)(t / per_group);
-  long long i = t - (long long)g * per_group;
-  const int left = p.batch - g * p.group, w = left < p.group ? left : p.group;
-  r.step = (int)(i / ((long long)w * per));
-  i -= (long long)r.step * w * per;
-  const long long ws = (long long)w * p.sym_tiles;
-  int tile;
-  if (i < 2 * ws) {
-    r.kind = i < ws ? kGram : kPoly;
-    if (i >= ws) i -= ws;
+  const unsigned sym = p.batch * p.sym_tiles, per_step = 2 * sym + p.batch * p.upd_tiles;
+  r.step = (int)(t / per_step);
+  unsigned i = t - r.step * per_step;
+  if (i < 2 * sym) {
+    r.kind = i < sym ? kGram : kPoly;
+    if (i >= sym) i -= sym;
     r.bi = (int)(i / p.sym_tiles);
-    tile = (int)(i - (long long)r.bi * p.sym_tiles);
-    int mt = 0;
+    int tile = (int)(i - r.bi * p.sym_tiles), mt = 0;
     for (int c = sym_cols<BN>(0, p.p); tile >= c; c = sym_cols<BN>(mt, p.p)) { tile -= c; ++mt; }
     r.mt = mt;
     r.nt = tile;
   } else {
-    i -= 2 * ws;
+    i -= 2 * sym;
     r.kind = kUpdate;
     r.bi = (int)(i / p.upd_tiles);
-    tile = (int)(i - (long long)r.bi * p.upd_tiles);
-    r.mt = tile / p.upd_n;
-    r.nt = tile - r.mt * p.upd_n;
+    const unsigned tile = i - r.bi * p.upd_tiles;
+    r.mt = (int)(tile / p.upd_n);
+    r.nt = (int)(tile - r.mt * p.upd_n);
   }
-  r.bi += g * p.group;
   return r;
 }
-// Epilogue warps of the task's matrix that must have finished before it may start.
+// Tiles of the task's matrix that must be finished before it may start.
 __device__ __forceinline__ unsigned needs(const Task& t, const NsParams& p) {
   const int per = 2 * p.sym_tiles + p.upd_tiles;
-  const int before = t.step * per + (t.kind == kGram ? 0 : t.kind == kPoly ? p.sym_tiles : 2 * p.sym_tiles);
-  return (unsigned)before * kEpiWarps;
+  return (unsigned)(t.step * per + (t.kind == kGram ? 0 : t.kind == kPoly ? p.sym_tiles : 2 * p.sym_tiles));
 }
 
 __device__ __forceinline__ uint32_t pack_h(float x, float y) {
@@ -168,12 +180,13 @@ __device__ __forceinline__ uint32_t pack_b(float x, float y) {
 __device__ __forceinline__ float2 unpack_h(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
 template <int BN>
-__global__ void __launch_bounds__(kThreadsNs, 1)
+__global__ void __launch_bounds__(ns_threads<BN>(), 1)
 ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int kStages = ns_stages<BN>();
   constexpr uint32_t kSlot = slot_bytes<BN>();
+  constexpr int kEpiWarps = epi_warps<BN>();
   unsigned char* ring = smem;                      // per slot: A (2 boxes), B (BN / 64 boxes)
   unsigned char* staging = smem + kStages * kSlot;
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingWarp);
@@ -183,9 +196,12 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* task_full = acc_empty + 2;             // [kQueue]
   uint64_t* task_empty = task_full + kQueue;
-  uint64_t* res_bars = task_empty + kQueue;        // [kEpiWarps][2]
-  volatile long long* queue = reinterpret_cast<volatile long long*>(res_bars + 2 * kEpiWarps);  // [kQueue], -1 ends
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<long long*>(queue) + kQueue);
+  uint64_t* tile_done = task_empty + kQueue;       // [kQueue] all stores of a tile complete
+  uint64_t* tile_free = tile_done + kQueue;
+  uint64_t* res_bars = tile_free + kQueue;         // [kEpiWarps]
+  int4* queue = reinterpret_cast<int4*>(res_bars + kEpiWarps);  // [kQueue]: step * 4 + kind (-1: no more), matrix, tile
+  volatile int* tile_matrix = reinterpret_cast<volatile int*>(queue + kQueue);   // [kQueue], -1: no more
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(tile_matrix) + kQueue);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t kTmemCols = 2 * BN;
@@ -196,8 +212,8 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
     };
     for (int s = 0; s < kStages; ++s) { init(&full[s], 1); init(&empty[s], 1); }
     for (int a = 0; a < 2; ++a) { init(&acc_full[a], 1); init(&acc_empty[a], kEpiWarps); }
-    for (int q = 0; q < kQueue; ++q) { init(&task_full[q], 1); init(&task_empty[q], 1 + kEpiWarps); }
-    for (int w = 0; w < 2 * kEpiWarps; ++w) init(&res_bars[w], 1);
+    for (int q = 0; q < kQueue; ++q) { init(&task_full[q], 1); init(&task_empty[q], 1 + kEpiWarps); init(&tile_done[q], kEpiWarps); init(&tile_free[q], 1); }
+    for (int w = 0; w < kEpiWarps; ++w) init(&res_bars[w], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -209,45 +225,49 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();
 
-  auto give_up = [&] { atomicExch(p.status, kStatusStageTimeout); *abort_flag = 1; };
+  // Waits and their outcome are a warp's, not a lane's: all lanes leave a loop together.
+  auto give_up = [&] { if (lane == 0) { atomicExch(p.status, kStatusStageTimeout); *abort_flag = 1; } };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; };
+  auto aborted = [&] { return __any_sync(0xffffffffu, *abort_flag) != 0; };
   // operand orientation of a task: the tile's rows are the reduction's (MN-major)?
   auto a_mn = [&](int kind) { return kind == kGram && p.tall; };
   auto b_mn = [&](int kind) { return kind == kGram ? p.tall != 0 : kind == kUpdate && !p.tall; };
   auto k_blocks = [&](int kind) { return ((kind == kGram ? p.q : p.p) + kBK - 1) / kBK; };
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, slot = 0;
-      uint32_t phase = 0, qphase = 0;
-      pdl_wait();
-      while (!*abort_flag) {
-        long long t = (long long)atomicAdd(p.ticket, 1ULL);
-        if (t >= p.total) t = -1;
-        Task q;
-        if (t >= 0) {
-          q = task_of<BN>(t, p);
-          const unsigned want = needs(q, p);
-          if (want) {
-            int spins = 0;
-            while (load_acquire(p.done + q.bi) < want) {
-              if (*abort_flag || ++spins > (1 << 25)) { give_up(); break; }
-            }
-            if (*abort_flag) break;
-          }
-          fence_async();       // what other CTAs stored by TMA is about to be loaded by TMA
-        }
-        if (!mbar_wait_bounded(&task_empty[slot], qphase ^ 1)) { give_up(); break; }
-        queue[slot] = t;
+    int stage = 0, slot = 0;
+    uint32_t phase = 0, qphase = 0;
+    pdl_wait();
+    unsigned next = 0;                 // lane 0: the next ticket, asked for when the current task's last loads go out
+    if (lane == 0) next = atomicAdd(p.ticket, 1u);
+    while (!aborted()) {
+      const unsigned t = __shfl_sync(0xffffffffu, next, 0);
+      Task q{-1, 3, 0, 0, 0};          // step * 4 + kind == -1: the end
+      if (t < p.total) {
+        q = task_of<BN>(t, p);
+        const unsigned want = needs(q, p);
+        bool ready = want == 0;
+        for (int spins = 0; !ready && spins < (1 << 25); ++spins) ready = load_acquire(p.done + q.bi) >= want;
+        if (!__all_sync(0xffffffffu, ready)) { give_up(); break; }
+        fence_async();                 // for this warp's loads and, by way of the queue, the epilogue's
+      }
+      if (!wait(&task_empty[slot], qphase ^ 1)) { give_up(); break; }
+      if (lane == 0) {
+        queue[slot] = make_int4(q.step * 4 + q.kind, q.bi, q.mt, q.nt);
         mbar_arrive(&task_full[slot]);
-        if (++slot == kQueue) { slot = 0; qphase ^= 1; }
-        if (t < 0) break;
-        const bool ta = a_mn(q.kind), tb = b_mn(q.kind);
-        const CUtensorMap* mx = &maps.x[q.step & 1];
-        const CUtensorMap* ma = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? mx : &maps.b);
-        const CUtensorMap* mb = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? &maps.b : mx);
-        const int kb_n = k_blocks(q.kind);
-        for (int kb = 0; kb < kb_n; ++kb) {
-          if (!mbar_wait_bounded(&empty[stage], phase ^ 1)) { give_up(); break; }
+      }
+      if (++slot == kQueue) { slot = 0; qphase ^= 1; }
+      if (t >= p.total) break;
+      const bool ta = a_mn(q.kind), tb = b_mn(q.kind);
+      const CUtensorMap* mx = &maps.x[q.step & 1];
+      const CUtensorMap* ma = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? mx : &maps.b);
+      const CUtensorMap* mb = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? &maps.b : mx);
+      const int kb_n = k_blocks(q.kind);
+      __syncwarp();
+      for (int kb = 0; kb < kb_n; ++kb) {
+        if (kb == kb_n - 1 && lane == 0) next = atomicAdd(p.ticket, 1u);
+        if (!wait(&empty[stage], phase ^ 1)) { give_up(); break; }
+        if (elect_one()) {
           mbar_expect_tx(&full[stage], kSlot);
           unsigned char* da = ring + stage * kSlot;
           unsigned char* db = da + 2 * kBox;
@@ -261,60 +281,102 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
             const int mn = q.nt * BN + i * 64;
             tma_load_3d(db + i * kBox, mb, tb ? mn : kb * kBK, tb ? kb * kBK : mn, q.bi, &full[stage]);
           }
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
+        __syncwarp();
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, acc = 0, slot = 0;
-      uint32_t phase = 0, acc_phase = 0, qphase = 0;
-      while (!*abort_flag) {
-        if (!mbar_wait_bounded(&task_full[slot], qphase)) { give_up(); break; }
-        const long long t = queue[slot];
-        mbar_arrive(&task_empty[slot]);
-        if (++slot == kQueue) { slot = 0; qphase ^= 1; }
-        if (t < 0) break;
-        const int kind = task_of<BN>(t, p).kind;
-        const bool ta = a_mn(kind), tb = b_mn(kind);
-        const uint32_t idesc = instr_desc<__half>(BN) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
-        const uint64_t step_a = ta ? 128 : 2, step_b = tb ? 128 : 2;  // 16 of K: 16 rows of an MN-major box, 32 bytes of a K-major row
-        const int kb_n = k_blocks(kind);
-        if (!mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1)) { give_up(); break; }
+    int stage = 0, acc = 0, slot = 0;
+    uint32_t phase = 0, acc_phase = 0, qphase = 0;
+    while (!aborted()) {
+      if (!wait(&task_full[slot], qphase)) { give_up(); break; }
+      const int code = queue[slot].x, kind = code & 3;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&task_empty[slot]);
+      if (++slot == kQueue) { slot = 0; qphase ^= 1; }
+      if (code < 0) break;
+      const bool ta = a_mn(kind), tb = b_mn(kind);
+      const uint32_t idesc = instr_desc<__half>(BN) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
+      const uint64_t step_a = ta ? 128 : 2, step_b = tb ? 128 : 2;  // 16 of K: 16 rows of an MN-major box, 32 bytes of a K-major row
+      const int kb_n = k_blocks(kind);
+      if (!wait(&acc_empty[acc], acc_phase ^ 1)) { give_up(); break; }
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+      for (int kb = 0; kb < kb_n; ++kb) {
+        if (!wait(&full[stage], phase)) { give_up(); break; }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-        for (int kb = 0; kb < kb_n; ++kb) {
-          if (!mbar_wait_bounded(&full[stage], phase)) { give_up(); break; }
-          tc_fence_after();
+        if (elect_one()) {
           unsigned char* da = ring + stage * kSlot;
           const uint64_t a0 = ta ? smem_desc_mn(da) : smem_desc_sw128(da);
           const uint64_t b0 = tb ? smem_desc_mn(da + 2 * kBox) : smem_desc_sw128(da + 2 * kBox);
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) tc_mma_f16(d_tmem, a0 + k * step_a, b0 + k * step_b, idesc, (kb | k) != 0);
           tc_commit(&empty[stage]);
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (kb == kb_n - 1) tc_commit(&acc_full[acc]);
         }
-        tc_commit(&acc_full[acc]);
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        __syncwarp();
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  } else if (warp == 2 + kEpiWarps) {
+    // Counts finished tiles: the release makes a whole CTA's stores visible and takes a microsecond or two, which the
+    // epilogue warps do not wait for.
+    int slot = 0;
+    uint32_t phase = 0;
+    for (;;) {
+      if (!wait(&tile_done[slot], phase)) {
+        if (aborted()) break;
+        continue;                        // long dependencies elsewhere; the waits that matter give up by themselves
+      }
+      const int bi = tile_matrix[slot];
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&tile_free[slot]);
+        if (bi >= 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + bi) : "memory");
+      }
+      if (bi < 0) break;
+      if (++slot == kQueue) { slot = 0; phase ^= 1; }
     }
   } else {
     const int quad = warp & 3, group = (warp - 2) >> 2;
-    constexpr int kCols = BN / 2, kUnits = kCols / 32;  // columns and units of this warp's share of a tile
-    unsigned char* buf = staging + (warp - 2) * kStagingWarp;
-    uint64_t* res_bar = &res_bars[2 * (warp - 2)];
-    uint32_t unit = 0, fetch_phase = 0;                  // bit i: phase of set i's next fetch
+    constexpr int kCols = BN / epi_groups<BN>(), kUnits = kCols / 32;  // columns and units of this warp's share of a tile
+    unsigned char* set = staging + (warp - 2) * kStagingWarp;
+    uint64_t* res_bar = &res_bars[warp - 2];
+    uint32_t fetch_phase = 0;
     int slot = 0, acc = 0;
     uint32_t qphase = 0, acc_phase = 0;
+    // A tile counts for its matrix once its stores are complete, some microseconds after they were issued.  With another
+    // task at hand the warp goes on and reports the tile a task later; without one it waits, since that task may wait
+    // for this tile.
+    int pending = -1;                                    // matrix of the tile not yet reported
+    int tslot = 0;
+    uint32_t tphase = 0;
+    auto report = [&](int bi) {                          // the whole warp; this warp's stores of the tile are complete
+      if (warp == 2) {                                   // one warp names the matrix
+        if (!wait(&tile_free[tslot], tphase ^ 1)) give_up();
+        if (lane == 0) tile_matrix[tslot] = bi;
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(&tile_done[tslot]);
+      if (++tslot == kQueue) { tslot = 0; tphase ^= 1; }
+    };
     pdl_wait();
-    while (!*abort_flag) {
-      if (!mbar_wait_bounded(&task_full[slot], qphase)) { if (lane == 0) give_up(); break; }
-      const long long t = queue[slot];
+    while (!aborted()) {
+      if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&task_full[slot], qphase))) {
+        if (elect_one()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+        report(pending);
+        pending = -1;
+      }
+      if (!wait(&task_full[slot], qphase)) { give_up(); break; }
+      const int4 code = queue[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&task_empty[slot]);
       if (++slot == kQueue) { slot = 0; qphase ^= 1; }
-      if (t < 0) break;
-      const Task q = task_of<BN>(t, p);
+      if (code.x < 0) break;
+      const Task q{code.x >> 2, code.x & 3, code.y, code.z, code.w};
       const int kind = q.kind;
       const bool pair = q.step < p.keep, last = q.step == p.steps - 1;
       const bool res = kind == kUpdate && pair;          // a * (hi + lo / 2048) is added
@@ -329,43 +391,33 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       const int rows = kind == kUpdate ? p.m : p.p, cols = kind == kUpdate ? p.n : p.p;
       const int row0 = q.mt * kBM + quad * 32, colw = q.nt * BN + group * kCols;
       const bool rows_in = row0 < rows;                  // else this warp's quarter lies below the matrix
-      // ask for the unit of the previous X or A that unit `u` needs
-      auto fetch = [&](int u, uint32_t k) {
-        unsigned char* set = buf + (k & 1) * 2 * kUnit;
-        mbar_expect_tx(&res_bar[k & 1], res ? 2 * kUnit : kUnit);
-        tma_load_3d(set, r0, colw + u * 32, row0, q.bi, &res_bar[k & 1]);
-        if (res) tma_load_3d(set + kUnit, r1, colw + u * 32, row0, q.bi, &res_bar[k & 1]);
+      // make the staging buffer free and ask for the unit of the previous X or A that unit `u` needs
+      auto fetch = [&](int u) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        if (!has_res) return;
+        mbar_expect_tx(res_bar, res ? 2 * kUnit : kUnit);
+        tma_load_3d(set, r0, colw + u * 32, row0, q.bi, res_bar);
+        if (res) tma_load_3d(set + kUnit, r1, colw + u * 32, row0, q.bi, res_bar);
       };
       int units = rows_in ? (cols - colw + 31) / 32 : 0;   // units with any column of the matrix
       units = units < 0 ? 0 : (units > kUnits ? kUnits : units);
-      if (has_res && units > 0 && lane == 0) {
-        fence_async();
-        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        fetch(0, unit);
-      }
-      if (!mbar_wait_bounded(&acc_full[acc], acc_phase)) { if (lane == 0) give_up(); break; }
+      if (units > 0 && elect_one()) fetch(0);
+      __syncwarp();
+      if (!wait(&acc_full[acc], acc_phase)) { give_up(); break; }
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + group * kCols);
 #pragma unroll 1
-      for (int u = 0; u < units; ++u, ++unit) {
+      for (int u = 0; u < units; ++u) {
         const int col0 = colw + u * 32;
-        const int set_i = (int)(unit & 1);
-        unsigned char* set = buf + set_i * 2 * kUnit;
         uint32_t v[32];
         tmem_ld_32x32(taddr + (uint32_t)(u * 32), v);
-        if (lane == 0) {
-          if (has_res) {
-            // the other set is free once the store of the previous unit has read it
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            if (u + 1 < units) fetch(u + 1, unit + 1);
-          } else {
-            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          }
+        if (u > 0) {
+          if (elect_one()) fetch(u);
+          __syncwarp();
         }
-        __syncwarp();
         if (has_res) {
-          if (!mbar_wait_bounded(&res_bar[set_i], (fetch_phase >> set_i) & 1)) { if (lane == 0) give_up(); }
-          fetch_phase ^= 1u << set_i;
+          if (!wait(res_bar, fetch_phase)) give_up();
+          fetch_phase ^= 1;
         }
         tmem_ld_wait();
         // a unit below the diagonal whose mirror image no tile computes is stored there as well
@@ -432,7 +484,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) {
+        if (elect_one()) {
           tma_store_3d(o0, set, col0, row0, q.bi);
           if (write_lo) tma_store_3d(o1, set + kUnit, col0, row0, q.bi);
           if (mirror) tma_store_3d(o0, set + kUnit, row0, col0, q.bi);
@@ -441,17 +493,22 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
+      if (elect_one()) {
         mbar_arrive(&acc_empty[acc]);
-        // the tile's stores are complete, hence visible, before the matrix counts this warp
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        fence_async();
-        __threadfence();
-        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + q.bi) : "memory");
+        for (int u = units; u < kUnits; ++u) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group %0;" ::"n"(kUnits) : "memory");   // all but this tile's
       }
+      __syncwarp();
+      if (pending >= 0) report(pending);
+      pending = q.bi;
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (elect_one()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+    if (!aborted()) {
+      if (pending >= 0) report(pending);
+      report(-1);
+    }
   }
 
   tc_fence_before();
@@ -478,7 +535,7 @@ template <typename T> __device__ __forceinline__ float load1(const T* p) { retur
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
 ns_square_kernel(const T* __restrict__ x, double* __restrict__ partial, long long per, long long chunk, int vec,
-                 unsigned* __restrict__ done, unsigned long long* __restrict__ ticket) {
+                 unsigned* __restrict__ done, unsigned* __restrict__ ticket) {
   __shared__ double part[kNormThreads / 32];
   pdl_trigger();
   pdl_wait();
@@ -641,11 +698,13 @@ cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
   for (int i = 0; i < (p.p + kBM - 1) / kBM; ++i) p.sym_tiles += sym_cols<BN>(i, p.p);
   p.upd_n = (p.n + BN - 1) / BN;
   p.upd_tiles = (p.m + kBM - 1) / kBM * p.upd_n;
-  p.total = (long long)p.batch * p.steps * (2 * p.sym_tiles + p.upd_tiles);
+  const long long total = (long long)p.batch * p.steps * (2LL * p.sym_tiles + p.upd_tiles);
+  if (total >= (1LL << 31)) return cudaErrorInvalidValue;
+  p.total = (unsigned)total;
   // more CTAs than a product has tiles would only wait
   const long long most = (long long)p.batch * (p.sym_tiles > p.upd_tiles ? p.sym_tiles : p.upd_tiles);
   const unsigned grid = (unsigned)(most < sms ? most : sms);
-  return launch_overlapped(ns_kernel<BN>, dim3(grid), dim3(kThreadsNs), ns_smem<BN>(), s, maps, p);
+  return launch_overlapped(ns_kernel<BN>, dim3(grid), dim3(ns_threads<BN>()), ns_smem<BN>(), s, maps, p);
 }
 
 template <typename T>
@@ -665,7 +724,7 @@ cudaError_t prepare(const void* x, const Layout& w, unsigned char* ws, long long
   const T* src = static_cast<const T*>(x);
   cudaError_t e = launch_overlapped(ns_square_kernel<T>, dim3((unsigned)chunks, (unsigned)batch), dim3(kNormThreads), 0, s,
                                     src, partial, per, chunk, (int)vec, reinterpret_cast<unsigned*>(ws + w.done),
-                                    reinterpret_cast<unsigned long long*>(ws + w.ticket));
+                                    reinterpret_cast<unsigned*>(ws + w.ticket));
   if (e != cudaSuccess) return e;
   long long blocks = (8LL * sms + batch - 1) / batch;
   if (blocks > most) blocks = most;
@@ -692,10 +751,10 @@ cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* work
   p.m = m; p.n = n; p.tall = m > n;
   p.p = p.tall ? n : m; p.q = p.tall ? m : n;
   p.steps = steps; p.keep = steps - 2;
-  p.batch = (int)batch; p.group = (int)batch;
+  p.batch = (int)batch;
   p.a = a; p.b = b; p.c = c;
   p.done = reinterpret_cast<unsigned*>(ws + w.done);
-  p.ticket = reinterpret_cast<unsigned long long*>(ws + w.ticket);
+  p.ticket = reinterpret_cast<unsigned*>(ws + w.ticket);
   p.status = status;
   NsMaps maps;
   bool ok = true;
