@@ -838,7 +838,12 @@ def run_train_l(args):
                                                           gradient_as_bucket_view=True,
                                                           bucket_cap_mb=args.bucket_cap_mb)
         hooked = ddp_hooks.register(model, args.grad_compress)
-    opt = torch.optim.AdamW(model.parameters(), lr=1e-4, weight_decay=0.05)
+    if args.optimizer == "muon":       # the matrices; AdamW keeps norms, biases, layer scales and the classifier
+        from dcnv4_b200.muon import Muon, split_parameters
+        matrices, others = split_parameters(model)
+        opts = [Muon(matrices, lr=1e-4, weight_decay=0.05), torch.optim.AdamW(others, lr=1e-4, weight_decay=0.05)]
+    else:
+        opts = [torch.optim.AdamW(model.parameters(), lr=1e-4, weight_decay=0.05)]
     g = torch.Generator(device="cpu").manual_seed(100 + rank)
     images = torch.randn(batch, 3, res, res, generator=g).to(dev)
     labels = torch.randint(0, 1000, (batch,), generator=g).to(dev)
@@ -846,13 +851,15 @@ def run_train_l(args):
     import contextlib
 
     def step(sync=True):
-        opt.zero_grad(set_to_none=True)
+        for opt in opts:
+            opt.zero_grad(set_to_none=True)
         ctx = contextlib.nullcontext() if (sync or world == 1) else model.no_sync()
         with ctx:
             with torch.autocast("cuda", dtype=torch.bfloat16):
                 loss = F.cross_entropy(model(images).float(), labels)
             loss.backward()
-        opt.step()
+        for opt in opts:
+            opt.step()
         return loss
 
     def barrier():
@@ -894,7 +901,8 @@ def run_train_l(args):
             "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16 autocast",
             "data": "synthetic", "loss": float(loss.detach()),
             "config": {"workload": f"FlashInternImage-{size.upper()} training step, {res}x{res}, batch {batch}/GPU, "
-                                   "AdamW, activation checkpointing, DDP all-reduce",
+                                   f"{'Muon + AdamW' if args.optimizer == 'muon' else 'AdamW'}, "
+                                   "activation checkpointing, DDP all-reduce",
                        "global_batch": batch * world, "parallelism": f"dp{world}",
                        "grad_compress": args.grad_compress if hooked else "none",
                        "bucket_cap_mb": args.bucket_cap_mb if world > 1 else None},
@@ -932,6 +940,9 @@ def main():
                     help="DDP gradient bucket size of --workload train_l (measured at 2 GPUs: 25 MB 147.8 ms per "
                          "step, 100 MB 138.3 ms, 400 MB 139.7 ms)")
     ap.add_argument("--train-res", type=int, default=1024)
+    ap.add_argument("--optimizer", default="adamw", choices=("adamw", "muon"),
+                    help="optimiser of --workload train_l: AdamW for everything as the reference, or Muon for the weight "
+                         "matrices and AdamW for the rest")
     args = ap.parse_args()
     if args.impl == "reference":
         return run_reference(args)

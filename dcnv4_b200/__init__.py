@@ -7,8 +7,11 @@ functions.  Importing the package does not touch the GPU; the CUDA library is lo
 first use and its absence is an error (there is no CPU path).
 """
 from . import ops as ext
-from .functions import DCNv4Function, FlashDeformAttnFunction
+from .functions import (AddLayerNormFunction, DCNv4Function, FlashDeformAttnFunction, LayerNormFunction,
+                        LayerNormResidualFunction)
 from .modules import DCNv4, FlashDeformAttn
+from .muon import Muon
 
-__all__ = ["DCNv4Function", "FlashDeformAttnFunction", "DCNv4", "FlashDeformAttn", "ext"]
+__all__ = ["DCNv4Function", "FlashDeformAttnFunction", "DCNv4", "FlashDeformAttn", "ext", "AddLayerNormFunction",
+           "LayerNormFunction", "LayerNormResidualFunction", "Muon"]
 __version__ = "0.1.0"

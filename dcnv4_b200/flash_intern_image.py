@@ -20,6 +20,8 @@ from torch import nn
 from torch.utils import checkpoint
 
 from . import ops
+from .functions.layer_norm_func import (AddLayerNormFunction, LayerNormFunction, LayerNormResidualFunction,
+                                        kernels_apply)
 from .modules import DCNv4
 
 
@@ -34,14 +36,36 @@ class _ToChannelsLast(nn.Module):
 
 
 class LayerNorm(nn.LayerNorm):
-    """torch.nn.LayerNorm (same parameters, same state-dict keys) whose inference forward on CUDA
-    runs the library's channels-last kernel: the model normalises millions of rows of 64-512
-    channels, which the stock kernel handles one thread block per row.  Whenever autograd needs
-    the operation (training) or the kernel does not cover the input, the stock path runs."""
+    """torch.nn.LayerNorm (same parameters, same state-dict keys) that runs the library's channels-last
+    kernels on CUDA: the model normalises millions of rows of 64-512 channels, which the stock kernel
+    handles one thread block per row.  Inference takes the forward kernel, training the pair with
+    saved row statistics (float32 results under autocast, as the stock module gives); the stock path
+    runs where the kernels do not cover the input."""
 
     use_library_kernel = True   # class-wide switch (benchmarks turn it off to time the stock path)
 
+    def train_out_dtype(self, x):
+        """Result dtype of the training kernels for this input, or None where the stock path has to run."""
+        if not (self.use_library_kernel and self.elementwise_affine and self.bias is not None and x.is_cuda
+                and len(self.normalized_shape) == 1 and x.dim() > 0 and x.shape[-1] == self.normalized_shape[0]
+                and kernels_apply(x, self.weight, self.bias)):
+            return None
+        autocast = torch.is_autocast_enabled("cuda")
+        if not autocast and self.weight.dtype != x.dtype:
+            return None                                   # the stock module refuses mixed types: leave that to it
+        out = torch.float32 if autocast else x.dtype
+        return out if ops.layer_norm_train_supported(x if x.is_contiguous() else x.contiguous(), self.weight, out) else None
+
+    def forward_act(self, x, activation="none"):
+        """act(self(x)) by the training kernels, or None where they do not apply."""
+        needs_grad = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad)
+        out = self.train_out_dtype(x) if needs_grad else None
+        return None if out is None else LayerNormFunction.apply(x, self.weight, self.bias, self.eps, activation, out)
+
     def forward(self, x):
+        y = self.forward_act(x)
+        if y is not None:
+            return y
         needs_grad = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad)
         if (self.use_library_kernel and not needs_grad and self.elementwise_affine and self.bias is not None
                 and len(self.normalized_shape) == 1 and not torch.is_autocast_enabled()
@@ -92,9 +116,17 @@ class DropPath(nn.Module):
     def forward(self, x):
         if self.drop_prob == 0.0 or not self.training:
             return x
-        keep = 1.0 - self.drop_prob
-        mask = x.new_empty((x.shape[0],) + (1,) * (x.dim() - 1)).bernoulli_(keep)
-        return x * mask / keep
+        return x * self._mask(x) / (1.0 - self.drop_prob)
+
+    def _mask(self, x):
+        return x.new_empty((x.shape[0],) + (1,) * (x.dim() - 1)).bernoulli_(1.0 - self.drop_prob)
+
+    def sample_scale(self, x):
+        """The factor of each sample (float32, one per element of the first dimension), or None when
+        inactive: for kernels that apply it themselves.  Draws the mask `forward(x)` would draw."""
+        if self.drop_prob == 0.0 or not self.training:
+            return None
+        return self._mask(x).float().flatten() / (1.0 - self.drop_prob)
 
 
 class StemLayer(nn.Module):
@@ -112,13 +144,16 @@ class StemLayer(nn.Module):
         self.norm2 = build_norm_layer(out_chans, norm_layer, "channels_first", "channels_last")
 
     def _fused_norm_act(self, x):
-        """LayerNorm + GELU over the channels of a channels-last activation in one pass (inference):
+        """LayerNorm + GELU over the channels of a channels-last activation in one pass:
         the convolution's (N,C,H,W) result in channels_last memory is the contiguous (N,H,W,C) tensor
         the kernel wants, and so is its input view for the next convolution."""
         ln = self.norm1[1] if len(self.norm1) == 3 and isinstance(self.norm1[1], LayerNorm) else None
-        if (ln is None or not isinstance(self.act, nn.GELU) or self.act.approximate != "none"
-                or torch.is_grad_enabled() and (x.requires_grad or ln.weight.requires_grad)
-                or torch.is_autocast_enabled() or not LayerNorm.use_library_kernel):
+        if ln is None or not isinstance(self.act, nn.GELU) or self.act.approximate != "none":
+            return None
+        if torch.is_grad_enabled() and (x.requires_grad or ln.weight.requires_grad):
+            y = ln.forward_act(x.permute(0, 2, 3, 1), "gelu")
+            return None if y is None else y.permute(0, 3, 1, 2)
+        if torch.is_autocast_enabled() or not LayerNorm.use_library_kernel:
             return None
         t = x.permute(0, 2, 3, 1)
         if not (t.is_contiguous() and ops.layer_norm_supported(t, ln.weight)):
@@ -164,6 +199,39 @@ def _single_layer_norm(module) -> Optional[nn.LayerNorm]:
     if isinstance(module, nn.Sequential) and len(module) == 1 and isinstance(module[0], nn.LayerNorm):
         return module[0]
     return None
+
+
+def _has_hooks(*modules) -> bool:
+    """Hooks see a module's call, so a module that has some is called."""
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+
+
+def _post_norm(norm_layer, x, residual, layer_scale, drop_path):
+    """residual + drop_path(layer_scale * norm(x)) for the tail of a post-norm branch: one kernel forward and one
+    backward in training, the stock operations otherwise."""
+    norm = _single_layer_norm(norm_layer)
+    if (torch.is_grad_enabled() and isinstance(norm, LayerNorm) and norm.weight.requires_grad
+            and not _has_hooks(norm_layer, norm, drop_path)):
+        out = norm.train_out_dtype(x)
+        if (out is not None and residual.dtype == out and residual.shape == x.shape and kernels_apply(residual, layer_scale)
+                and (layer_scale is None or layer_scale.dtype == norm.weight.dtype)):
+            scale = drop_path.sample_scale(residual) if isinstance(drop_path, DropPath) else None
+            return LayerNormResidualFunction.apply(x, residual, norm.weight, norm.bias, norm.eps, layer_scale, scale)
+    a = norm_layer(x)
+    return residual + drop_path(a if layer_scale is None else layer_scale * a)
+
+
+def _pre_norm(norm_layer, branch, residual, drop_path):
+    """(h, norm(h)) with h = residual + drop_path(branch) for the seam between two pre-norm branches, fused in training."""
+    norm = _single_layer_norm(norm_layer)
+    if (torch.is_grad_enabled() and isinstance(norm, LayerNorm) and norm.weight.requires_grad
+            and not _has_hooks(norm_layer, norm, drop_path)):
+        out = norm.train_out_dtype(branch)
+        if out is not None and residual.dtype == out and residual.shape == branch.shape and kernels_apply(residual):
+            scale = drop_path.sample_scale(branch) if isinstance(drop_path, DropPath) else None
+            return AddLayerNormFunction.apply(branch, residual, norm.weight, norm.bias, norm.eps, scale)
+    h = residual + drop_path(branch)
+    return h, norm_layer(h)
 
 
 class _ConvAsLinear:
@@ -221,18 +289,24 @@ class InternImageLayer(nn.Module):
 
     def _inner(self, x, shape):
         if self.post_norm:
-            a = self.norm1(self.dcn(x, shape))
-            x = x + self.drop_path(self.gamma1 * a if self.layer_scale else a)
-            m = self.norm2(self.mlp(x, shape))
-            x = x + self.drop_path(self.gamma2 * m if self.layer_scale else m)
+            x = _post_norm(self.norm1, self.dcn(x, shape), x, self.gamma1 if self.layer_scale else None, self.drop_path)
+            x = _post_norm(self.norm2, self.mlp(x, shape), x, self.gamma2 if self.layer_scale else None, self.drop_path)
         elif self._plain_residual():
             x = self._chained(x, shape, None, None)[0]
         else:
-            a = self.dcn(self.norm1(x), shape)
-            x = x + self.drop_path(self.gamma1 * a if self.layer_scale else a)
-            m = self.mlp(self.norm2(x), shape)
-            x = x + self.drop_path(self.gamma2 * m if self.layer_scale else m)
+            x = self._pre_normed(x, shape, None, None)[0]
         return x
+
+    def _pre_normed(self, x, shape, normed, next_norm):
+        """Pre-norm layer with layer scale or stochastic depth: each sum and the LayerNorm that follows it are one
+        step.  Returns (result, next_norm(result) or None)."""
+        a = self.dcn(normed if normed is not None else self.norm1(x), shape)
+        x, m_in = _pre_norm(self.norm2, self.gamma1 * a if self.layer_scale else a, x, self.drop_path)
+        m = self.mlp(m_in, shape)
+        m = self.gamma2 * m if self.layer_scale else m
+        if next_norm is None:
+            return x + self.drop_path(m), None
+        return _pre_norm(next_norm, m, x, self.drop_path)
 
     def _plain_residual(self) -> bool:
         """Pre-norm layer whose two branches are added as they are (no layer scale, no active
@@ -245,9 +319,11 @@ class InternImageLayer(nn.Module):
         previous layer already produced it, `next_norm` the LayerNorm that will be applied to
         this layer's result.  Returns (result, next_norm(result) or None).  At inference each
         LayerNorm is computed in the epilogue of the matrix product that precedes it."""
-        if not self._plain_residual() or (self.with_cp and x.requires_grad):
+        if self.post_norm or (self.with_cp and x.requires_grad):
             x = self.forward(x, shape)
             return x, (None if next_norm is None else next_norm(x))
+        if not self._plain_residual():
+            return self._pre_normed(x, shape, normed, next_norm)
         return self._chained(x, shape, normed, next_norm)
 
     def _chained(self, x, shape, normed, next_norm):

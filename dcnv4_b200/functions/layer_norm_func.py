@@ -2,15 +2,45 @@
 
 The reference composes these from torch.nn.LayerNorm, the layer-scale product, timm's DropPath and residual additions
 (classification/models/flash_intern_image.py:34-56, 414-432).  Each function below is one kernel forward and one
-(plus a small reduction) backward; gradients come out in the dtype of their inputs.
+(plus a small reduction) backward; gradients come out in the dtype of their inputs.  Under `create_graph=True` the
+backward pass is composed of PyTorch operations instead, so second derivatives work as with the stock modules.
 """
 from __future__ import annotations
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from .. import ops
+
+
+def kernels_apply(*tensors) -> bool:
+    """Whether an autograd function over a foreign kernel may take these tensors: not inside a torch.func transform or
+    forward-mode AD, which only the stock operations support."""
+    wrapped = getattr(torch._C, "_functorch", None)
+    is_wrapped = getattr(wrapped, "is_functorch_wrapped_tensor", None)
+    if is_wrapped is not None and any(t is not None and is_wrapped(t) for t in tensors):
+        return False
+    return getattr(torch.autograd.forward_ad, "_current_level", -1) < 0
+
+
+def _layer_norm(x, weight, bias, eps, dtype):
+    return torch.nn.functional.layer_norm(x.to(dtype), (x.shape[-1],), weight.to(dtype), bias.to(dtype), eps)
+
+
+def _per_sample(sample_scale, x):
+    return sample_scale.view((-1,) + (1,) * (x.dim() - 1)).repeat_interleave(x.shape[0] // sample_scale.numel(), 0)
+
+
+def _differentiable(fn, inputs, grads):
+    """Gradients of fn(*inputs) that can be differentiated again; None where an input needs none."""
+    with torch.enable_grad():
+        out = fn(*inputs)
+        out = out if isinstance(out, tuple) else (out,)
+        pairs = [(o, g) for o, g in zip(out, grads) if g is not None]
+        wanted = [t for t in inputs if t is not None and t.requires_grad]
+        got = iter(torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs], create_graph=True,
+                                       allow_unused=True))
+        return [next(got) if t is not None and t.requires_grad else None for t in inputs]
 
 
 class LayerNormFunction(Function):
@@ -18,17 +48,21 @@ class LayerNormFunction(Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, activation="none", out_dtype=None):
-        x = x.contiguous()
-        y, mean, rstd = ops.layer_norm_train_forward(x, weight, bias, eps, activation, out_dtype)
-        ctx.activation = activation
+        xc = x.contiguous()
+        y, mean, rstd = ops.layer_norm_train_forward(xc, weight, bias, eps, activation, out_dtype)
+        ctx.eps, ctx.activation = eps, activation
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
         x, weight, bias, mean, rstd = ctx.saved_tensors
-        gx, gw, gb = ops.layer_norm_backward(grad_y.contiguous(), x, mean, rstd, weight, bias, ctx.activation)
+        if torch.is_grad_enabled():
+            def plain(x_, w_, b_):
+                y = _layer_norm(x_, w_, b_, ctx.eps, grad_y.dtype)
+                return torch.nn.functional.gelu(y) if ctx.activation == "gelu" else y
+            return (*_differentiable(plain, (x, weight, bias), (grad_y,)), None, None, None)
+        gx, gw, gb = ops.layer_norm_backward(grad_y.contiguous(), x.contiguous(), mean, rstd, weight, bias, ctx.activation)
         return gx, gw, gb, None, None, None
 
 
@@ -38,17 +72,23 @@ class LayerNormResidualFunction(Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, layer_scale=None, sample_scale=None):
-        x = x.contiguous()
-        out, mean, rstd = ops.layer_norm_residual_forward(x, residual.contiguous(), weight, bias, eps, layer_scale,
-                                                          sample_scale)
+        out, mean, rstd = ops.layer_norm_residual_forward(x.contiguous(), residual.contiguous(), weight, bias, eps,
+                                                          layer_scale, sample_scale)
+        ctx.eps = eps
         ctx.save_for_backward(x, weight, bias, mean, rstd, layer_scale, sample_scale)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
         x, weight, bias, mean, rstd, layer_scale, sample_scale = ctx.saved_tensors
-        gx, gw, gb, gs = ops.layer_norm_residual_backward(grad_out.contiguous(), x, mean, rstd, weight, bias,
+        if torch.is_grad_enabled():
+            def plain(x_, w_, b_, s_):
+                z = _layer_norm(x_, w_, b_, ctx.eps, grad_out.dtype)
+                z = z if s_ is None else z * s_.to(z.dtype)
+                return z if sample_scale is None else z * _per_sample(sample_scale, z).to(z.dtype)
+            gx, gw, gb, gs = _differentiable(plain, (x, weight, bias, layer_scale), (grad_out,))
+            return gx, grad_out, gw, gb, None, gs, None
+        gx, gw, gb, gs = ops.layer_norm_residual_backward(grad_out.contiguous(), x.contiguous(), mean, rstd, weight, bias,
                                                           layer_scale, sample_scale)
         return gx, grad_out, gw, gb, None, gs, None
 
@@ -62,16 +102,25 @@ class AddLayerNormFunction(Function):
         ctx.set_materialize_grads(False)
         h, y, mean, rstd = ops.add_layer_norm_forward(x.contiguous(), residual.contiguous(), weight, bias, eps,
                                                       sample_scale)
-        ctx.x_dtype = x.dtype
-        ctx.save_for_backward(h, weight, mean, rstd, sample_scale)
+        ctx.eps, ctx.x_dtype = eps, x.dtype
+        ctx.save_for_backward(h, weight, bias, mean, rstd, sample_scale)   # h alone: x and residual may be freed
         return h, y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_h, grad_y):
-        h, weight, mean, rstd, sample_scale = ctx.saved_tensors
+        h, weight, bias, mean, rstd, sample_scale = ctx.saved_tensors
         if grad_h is None and grad_y is None:
             return (None,) * 6
+        if torch.is_grad_enabled():     # through h, an output of this node and so part of the graph
+            gr = grad_h
+            gw = gb = None
+            if grad_y is not None:
+                def plain(h_, w_, b_):
+                    return _layer_norm(h_, w_, b_, ctx.eps, h_.dtype)
+                through, gw, gb = _differentiable(plain, (h, weight, bias), (grad_y,))
+                gr = through if gr is None else gr + through
+            gx = (gr if sample_scale is None else gr * _per_sample(sample_scale, gr).to(gr.dtype)).to(ctx.x_dtype)
+            return gx, gr, gw, gb, None, None
         grad_y = torch.zeros_like(h) if grad_y is None else grad_y.contiguous()
         grad_h = None if grad_h is None else grad_h.contiguous()
         gr, gx, gw, gb = ops.add_layer_norm_backward(grad_y, grad_h, h, mean, rstd, weight, sample_scale, ctx.x_dtype)
