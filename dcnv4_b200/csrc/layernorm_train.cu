@@ -46,13 +46,11 @@ int ln_train_max_channels() { return ln::kMaxChannels; }
 // Element sizes of types 0 fp32, 1 fp16, 2 bf16.
 static int size_of(int d) { return d == 0 ? 4 : 2; }
 
-// Alignment decides the kernel: bulk copies want every loaded tensor on 16 bytes, the vector stores every tensor on the
-// size of a lane's vector (32 bytes where a 16-bit branch stands beside fp32 tensors).
+// Alignment decides the kernel: bulk copies want every loaded tensor on 16 bytes, the vector stores every stored one.
 static ln::Plan plan_of(bool backward, int mode, int xd, int yd, const LnTrainArgs& a) {
   auto on = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const bool base = on(a.x, 16) && on(a.res, 16) && on(a.h, 16) && on(a.gy, 16) && on(a.gh, 16);
-  const uintptr_t wide = xd != 0 && yd == 0 ? 32 : 16;
-  const bool vec = on(a.y, wide) && on(a.h, wide) && on(a.dx, wide) && on(a.dx2, 16);
+  const bool vec = on(a.y, 16) && on(a.h, 16) && on(a.dx, 16) && on(a.dx2, 16);
   return ln::plan_for(backward, mode, size_of(xd), size_of(yd), a.gh != nullptr, base, vec, a.rows, a.C);
 }
 

@@ -208,6 +208,10 @@ static_assert(sizeof(RingHeader) <= kRingHeader, "ring header");
 // Warps of a CTA: as many as the registers of NE elements a lane leave room for.  Parameters live in registers up to
 // 16 elements, beyond that in shared memory.
 constexpr int warps_for(int ne) { return ne <= 16 ? 16 : 12; }
+// CTAs per SM of the forward kernels: where parameters are in shared memory two fit (200704 x 80 bf16, post-norm: 21.4
+// against 23.5 us with one; 131072 x 160 bf16 to fp32: 26.5 against 28.6), elsewhere the registers would spill (2048 x 4096
+// fp32: 33 against 23 us).
+constexpr int fwd_ctas(int ne) { return ne > 16 ? 2 : 1; }
 template <int NE> constexpr int ring_warps() { return warps_for(NE); }
 template <int VEC, int NV> constexpr bool params_in_smem() { return VEC * NV > 16 || (VEC == 1 && NV > 8); }
 
@@ -301,6 +305,11 @@ __device__ __forceinline__ void row_load(float2 (&f)[NV * VEC / 2], const T* row
       const int c = (sub + v * lpr) * VEC;
       constexpr int W = VEC * (int)sizeof(T) / 4;
       uint32_t r[W];
+      if constexpr (W == 2) {
+        uint2 t = make_uint2(0u, 0u);
+        if (live && (v + 1 < NV || c < C)) t = *reinterpret_cast<const uint2*>(row + c);
+        r[0] = t.x; r[1] = t.y;
+      }
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
         uint4 t = make_uint4(0u, 0u, 0u, 0u);
@@ -367,16 +376,34 @@ __device__ __forceinline__ void param_fetch(float2 (&f)[NV * VEC / 2], const voi
   }
   param_load<P, VEC, NV>(f, p, sub, lpr, C, f32);
 }
-// One fp32 parameter vector in shared memory, filled by the whole CTA.
-template <typename P>
+// One fp32 parameter vector in shared memory, filled by the whole CTA.  For vectors of 8 their halves lie in two arrays, so
+// that the 16-byte loads of neighbouring lanes are neighbours (interleaved, they would meet in the same banks).
+template <int VEC>
+__device__ __forceinline__ int staged_at(int c, int C) {
+  return VEC == 8 ? (c & 4) / 4 * (C / 2) + c / 8 * 4 + (c & 3) : c;
+}
+template <typename P, int VEC>
 __device__ __forceinline__ void param_stage(float* dst, const void* p, const void* factor, int C, int f32) {
   for (int c = threadIdx.x; c < C; c += blockDim.x)
-    dst[c] = param<P>(p, c, f32) * (factor != nullptr ? param<P>(factor, c, f32) : 1.f);
+    dst[staged_at<VEC>(c, C)] = param<P>(p, c, f32) * (factor != nullptr ? param<P>(factor, c, f32) : 1.f);
 }
-// A lane's pair i of a staged parameter vector.
 template <int VEC, int NV>
 __device__ __forceinline__ void param_row(float2 (&f)[NV * VEC / 2], const float* p, int sub, int lpr, int C) {
-  row_load<float, VEC, NV>(f, p, sub, lpr, C, true);
+  if constexpr (VEC == 8) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int k = sub + v * lpr;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (v + 1 < NV || k * 8 < C) t = reinterpret_cast<const float4*>(p + h * (C / 2))[k];
+        f[v * 4 + 2 * h] = make_float2(t.x, t.y);
+        f[v * 4 + 2 * h + 1] = make_float2(t.z, t.w);
+      }
+    }
+  } else {
+    row_load<float, VEC, NV>(f, p, sub, lpr, C, true);
+  }
 }
 // Parameter gradients of one column from its sums.
 template <typename P>
@@ -434,7 +461,7 @@ __device__ __forceinline__ float ring_sum(float t, int lpr, RingHeader* h, int& 
 }
 
 template <typename TX, typename TY, int VEC, int NV, int MODE, bool GELU>
-__global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), 1)
+__global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), fwd_ctas(VEC * NV))
 ln_ring_fwd_kernel(const LnTrainArgs a) {
   using P = TX;
   constexpr int NE = VEC * NV, W = ring_warps<NE>();
@@ -464,8 +491,8 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
     float* bs = ws + (C + 3) / 4 * 4;
     if constexpr (kStaged) {
       const void* g = MODE == kPost ? a.gamma : nullptr;
-      param_stage<P>(ws, a.w, g, C, a.param_f32);
-      param_stage<P>(bs, a.b, g, C, a.param_f32);
+      param_stage<P, VEC>(ws, a.w, g, C, a.param_f32);
+      param_stage<P, VEC>(bs, a.b, g, C, a.param_f32);
     } else {
       param_fetch<P, VEC, NV>(w, a.w, sub, lpr, C, a.param_f32);
       param_fetch<P, VEC, NV>(b, a.b, sub, lpr, C, a.param_f32);
@@ -589,8 +616,8 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
     float* ws = reinterpret_cast<float*>(ring + (size_t)a.stages * slot);
     float* bs = ws + (C + 3) / 4 * 4;
     if constexpr (kStaged) {
-      param_stage<P>(ws, a.w, MODE == kPost ? a.gamma : nullptr, C, a.param_f32);
-      if constexpr (GELU) param_stage<P>(bs, a.b, nullptr, C, a.param_f32);
+      param_stage<P, VEC>(ws, a.w, MODE == kPost ? a.gamma : nullptr, C, a.param_f32);
+      if constexpr (GELU) param_stage<P, VEC>(bs, a.b, nullptr, C, a.param_f32);
     } else {
       param_fetch<P, VEC, NV>(w, a.w, sub, lpr, C, a.param_f32);
       if constexpr (GELU) param_fetch<P, VEC, NV>(b, a.b, sub, lpr, C, a.param_f32);
@@ -968,7 +995,7 @@ struct Geometry {
   int lpr, nv, warps;
   bool ok;
 };
-// A lane holds 1..max_nv vectors, or 4, 8, 12 or 16 single elements.  A row costs its team's lanes about as much for its
+// A lane holds 1..max_nv vectors (of 8 elements up to 3, of 4 up to 6), or 4, 8, 12 or 16 single elements.  A row costs its team's lanes about as much for its
 // bookkeeping as ten more elements a lane would: fewest lanes * (elements + 10) wins.  A team divides the warps of
 // the CTA (16, or 12 where a lane holds more than 16 elements).
 inline Geometry geometry(int n, int vec, int max_nv) {
@@ -987,8 +1014,7 @@ inline Geometry geometry(int n, int vec, int max_nv) {
 }
 
 constexpr size_t kRingBytes = 200 * 1024;   // of 227 KB per SM
-// Aim of one tile: several passes of the CTA, whose bookkeeping per tile then counts less (16 / 32 / 64 KB: 26 / 26 / 23.6 us
-// for the post-norm forward over 200704 x 80 bf16), and still three of them in flight.
+// Most of one tile, so that three of them are in flight.
 constexpr size_t kTileBytes = 64 * 1024;
 // A backward pass this small stays in one CTA and needs no second kernel for the parameter gradients: measured 4.0 against
 // 5.8 us at 32 KB, 4.5 against 5.7 at 64 KB, 8.0 against 5.7 at 196 KB.
@@ -997,23 +1023,32 @@ constexpr size_t kAloneBytes = 64 * 1024;
 // Ring of a launch: `row_bytes` of all loaded tensors together, `align` rows make every span a multiple of 16 bytes.
 // False where two tiles do not fit.
 struct Ring { int tile_rows, stages, grid; size_t smem; };
-inline bool ring_for(int rows, const Geometry& g, size_t row_bytes, int align, size_t acc_bytes, size_t param_bytes, Ring* out) {
+inline bool ring_for(int rows, const Geometry& g, size_t row_bytes, int align, size_t acc_bytes, size_t param_bytes, int per_sm, Ring* out) {
   const int per_pass = g.warps * 32 / g.lpr;
-  const size_t room = kRingBytes - param_bytes;
+  // what two CTAs share, unless it is too small for two tiles
+  size_t room = kRingBytes / per_sm - param_bytes;
+  if (per_sm > 1 && (param_bytes > kRingBytes / per_sm || 2 * (size_t)align * row_bytes > room)) { per_sm = 1; room = kRingBytes - param_bytes; }
+  const size_t tile_bytes = kTileBytes / per_sm;
+  const int ctas = kSms * per_sm;
   if (2 * (size_t)align * row_bytes > room) return false;
-  // whole passes of the CTA up to the aim, at least one; not so many that SMs idle, nor that two do not fit
-  long long r = per_pass;
-  while ((size_t)(r + per_pass) * row_bytes <= kTileBytes) r += per_pass;
-  // a backward pass of a few rows stays in one CTA, which then needs no second kernel for the parameter gradients
+  // A backward pass of a few rows stays in one CTA, which then needs no second kernel for the parameter gradients.
   const bool alone = acc_bytes > 0 && (size_t)rows * row_bytes <= kAloneBytes;
-  const long long share = alone ? rows : ((long long)rows + kSms - 1) / kSms;
-  if (r > share) r = share;
+  const long long share = alone ? rows : ((long long)rows + ctas - 1) / ctas;
+  // Tiles are whole passes of the CTA: `j` of them cost j + 0.5 a tile (its bookkeeping), times the rounds of tiles that the
+  // busiest CTA walks, plus j for the first load and the last computation, which nothing overlaps.
+  long long r = share < per_pass ? share : per_pass;
+  double best = 1e30;
+  for (long long j = 1; share >= per_pass && (j == 1 || (size_t)(j * per_pass) * row_bytes <= tile_bytes); ++j) {
+    const long long tiles = ((long long)rows + j * per_pass - 1) / (j * per_pass);
+    const double cost = (double)((tiles + ctas - 1) / ctas) * (j + 0.5) + j;
+    if (cost < best * 0.99) { best = cost; r = j * per_pass; }
+  }
   while (r > 1 && 2 * (size_t)r * row_bytes > room) r = (r + 1) / 2;
   r = (r + align - 1) / align * align;
   if (2 * (size_t)r * row_bytes > room) r = align;
   const long long tiles = ((long long)rows + r - 1) / r;
   out->tile_rows = (int)r;
-  out->grid = alone ? 1 : (int)(tiles < kSms ? tiles : kSms);
+  out->grid = alone ? 1 : (int)(tiles < ctas ? tiles : ctas);
   long long st = (long long)(room / ((size_t)r * row_bytes));
   const long long walk = (tiles + out->grid - 1) / out->grid;   // tiles of one CTA
   if (st > walk) st = walk;
@@ -1050,16 +1085,16 @@ struct Plan {
 };
 inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool base16, bool vec_ok, int rows, int C) {
   Plan p;
-  const int V = x_es == 4 ? 4 : 8;
+  const int V = x_es == 4 || y_es == 4 ? 4 : 8;
   p.vec = vec_ok && base16 && C % V == 0 ? V : 1;
-  p.g = geometry(p.vec > 1 ? C / V : C, p.vec, V == 8 ? 3 : 4);
+  p.g = geometry(p.vec > 1 ? C / V : C, p.vec, V == 8 ? 3 : 6);
   const int lx = backward && mode == kPre ? y_es : x_es;      // element size of the normalised tensor
   const size_t row_bytes = (size_t)C * (backward ? lx + y_es * (1 + (mode == kPre && gh)) : x_es + (mode == kPlain ? 0 : y_es));
   const int es_min = backward ? (lx < y_es ? lx : y_es) : (mode == kPlain || x_es < y_es ? x_es : y_es);
   const int slots = p.g.lpr > 32 ? p.g.warps * 32 / p.g.lpr : p.g.warps;
   const size_t acc = backward ? (size_t)slots * 2 * C * sizeof(float) : 0;
   const size_t params = p.g.nv * p.vec > 16 || (p.vec == 1 && p.g.nv > 8) ? (size_t)2 * ((C + 3) / 4 * 4) * sizeof(float) : 0;
-  p.direct = !base16 || acc > kRingBytes || !ring_for(rows, p.g, row_bytes, align_rows(C, es_min), acc, params, &p.ring);
+  p.direct = !base16 || acc > kRingBytes || !ring_for(rows, p.g, row_bytes, align_rows(C, es_min), acc, params, backward ? 1 : fwd_ctas(p.g.nv * p.vec), &p.ring);
   if (p.direct) {
     p.vec = 1;
     p.g = geometry(C, 1, 0);
@@ -1069,7 +1104,9 @@ inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool 
   return p;
 }
 
-template <typename T> struct FullVec { static constexpr int n = 16 / (int)sizeof(T); };
+// Elements of a vector: 16 bytes of the wider tensor type (a 16-bit branch beside fp32 tensors takes 8 bytes: with 8
+// elements a lane's fp32 pieces would be 32 bytes apart and meet in the same banks).
+template <typename TX, typename TY> struct FullVec { static constexpr int n = sizeof(TX) == 4 || sizeof(TY) == 4 ? 4 : 8; };
 
 template <auto Kern>
 cudaError_t launch_ring(const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
@@ -1117,7 +1154,7 @@ cudaError_t direct_run(bool backward, int mode, int act, const LnTrainArgs& a, c
 
 template <typename TX, typename TY>
 cudaError_t run(bool backward, int mode, int act, const Plan& p, const LnTrainArgs& a0, cudaStream_t s) {
-  constexpr int V = FullVec<TX>::n;
+  constexpr int V = FullVec<TX, TY>::n;
   if (!p.g.ok) return cudaErrorInvalidValue;
   LnTrainArgs a = a0;
   a.lpr = p.g.lpr;
@@ -1135,7 +1172,11 @@ cudaError_t run(bool backward, int mode, int act, const Plan& p, const LnTrainAr
     case 2: return ring_run<TX, TY, V, 2>(backward, mode, act, a, p, s);
     case 3: return ring_run<TX, TY, V, 3>(backward, mode, act, a, p, s);
     default:
-      if constexpr (V == 4) return ring_run<TX, TY, V, 4>(backward, mode, act, a, p, s);
+      if constexpr (V == 4) {
+        if (p.g.nv == 4) return ring_run<TX, TY, V, 4>(backward, mode, act, a, p, s);
+        if (p.g.nv == 5) return ring_run<TX, TY, V, 5>(backward, mode, act, a, p, s);
+        if (p.g.nv == 6) return ring_run<TX, TY, V, 6>(backward, mode, act, a, p, s);
+      }
       return cudaErrorInvalidValue;
   }
 }
