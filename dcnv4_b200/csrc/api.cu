@@ -549,7 +549,8 @@ int dcnv4b200_newton_schulz(const void* x, void* out, void* workspace, size_t wo
   if (!x || !out) return DCNV4B200_ERR_NULL;
   if (((uintptr_t)x & (elem_size(dtype) - 1)) || ((uintptr_t)out & 1) || !aligned16(workspace))
     return DCNV4B200_ERR_ALIGN;
-  if (!workspace || workspace_bytes < ns_workspace_bytes(batch, m, n)) return DCNV4B200_ERR_WORKSPACE;
+  const size_t need = ns_workspace_bytes(batch, m, n);
+  if (need && (!workspace || workspace_bytes < need)) return DCNV4B200_ERR_WORKSPACE;
   int* status = nullptr;
   int sms = 1;
   if (int rc = status_ptr(&status, &sms)) return rc;

@@ -30,6 +30,11 @@
 //              in the staging buffer that the result leaves from
 // Every mbarrier wait is bounded; one that runs out sets the device status word and the CTA winds down.
 //
+// Matrices with p <= 128 and q <= 256 take another kernel: one CTA holds a whole matrix (X and A, B as fp16 operands in shared
+// memory, X in fp32 in tensor memory) and runs all steps without leaving the SM, in one launch that includes the norm.
+// What bounds it is the chain of 3 * steps products, each a commit, a barrier and a pass of eight warps over the
+// accumulator: 64 x 64 takes 22 us, where the tiled kernel's flags and round trips to L2 made it 54.
+//
 // The reference has no optimiser kernels; its trainers use stock AdamW (classification/optimizer.py).
 #include <mutex>
 
@@ -524,6 +529,202 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
   }
 }
 
+// ------------------------------------------------------------------- whole matrices in one CTA
+
+constexpr int kSmallP = 128, kSmallQ = 256;
+constexpr int kSmallThreads = 256;
+constexpr int kBlock = 128 * 64 * 2;           // 128 rows x 64 columns of fp16: one swizzled column block
+
+struct SmallParams {
+  const void* x;
+  void* out;
+  int m, n, p, q, tall;
+  int steps, keep;
+  float a, b, c, eps;
+  int tmem_cols, acc_col;      // tensor memory: X (fp32) from column 0, the accumulator from acc_col
+  int* status;
+};
+
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Where 16-byte piece `piece` of row `row` lies in a column block (128-byte swizzle).
+__device__ __forceinline__ uint32_t block_at(int row, int piece) {
+  return (uint32_t)row * 128 + (uint32_t)((piece ^ (row & 7)) << 4);
+}
+// 32 consecutive columns (from c0, a multiple of 32) of a thread's row into a matrix of column blocks, as fp16.
+__device__ __forceinline__ void put_row(unsigned char* mat, int row, int c0, const float (&v)[32]) {
+  unsigned char* blk = mat + (c0 >> 6) * kBlock;
+#pragma unroll
+  for (int j = 0; j < 32; j += 8)
+    *reinterpret_cast<uint4*>(blk + block_at(row, ((c0 & 63) + j) >> 3)) =
+        make_uint4(pack_h(v[j], v[j + 1]), pack_h(v[j + 2], v[j + 3]), pack_h(v[j + 4], v[j + 5]), pack_h(v[j + 6], v[j + 7]));
+}
+
+// X is kept wide, (p, q), whatever the matrix' own orientation: element (r, c) is x[r][c] or, for tall ones, x[c][r].  A
+// thread owns a row (as tensor memory is read) and one half of the columns.
+template <typename T>
+__global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallParams p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ double part[kSmallThreads / 32];
+  unsigned char* sx = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int qb = (p.q + 63) / 64, pb = (p.p + 63) / 64;    // column blocks
+  unsigned char* sa = sx + qb * kBlock;
+  unsigned char* sb = sa + pb * kBlock;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, half = warp >> 2;
+  const int row = quad * 32 + lane;
+  const int n_gram = (p.p + 15) / 16 * 16, n_upd = (p.q + 15) / 16 * 16;
+  if (threadIdx.x == 0) { mbar_init(&bar, 1); asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+  if (warp == 0) { tmem_alloc(&tmem_slot, (uint32_t)p.tmem_cols); tmem_relinquish(); }
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tx = tmem_slot + ((uint32_t)(quad * 32) << 16), ta = tx + (uint32_t)p.acc_col;
+  const uint32_t acc = tmem_slot + (uint32_t)p.acc_col;
+  pdl_wait();
+  // chunks of 32 columns that this thread's half covers
+  const int xc0 = half ? (qb * 64 / 2 + 31) / 32 * 32 : 0, xc1 = half ? qb * 64 : (qb * 64 / 2 + 31) / 32 * 32;
+  const int ac0 = half ? (pb * 64 / 2 + 31) / 32 * 32 : 0, ac1 = half ? pb * 64 : (pb * 64 / 2 + 31) / 32 * 32;
+
+  // the matrix into tensor memory, and its norm
+  const T* src = static_cast<const T*>(p.x) + (long long)blockIdx.x * p.m * p.n;
+  const long long row_step = p.tall ? 1 : p.n, col_step = p.tall ? p.n : 1;
+  double sum = 0.0;
+  for (int c0 = xc0; c0 < xc1; c0 += 32) {
+    uint32_t v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const bool in = row < p.p && c0 + j < p.q;
+      const float f = in ? to_f32(src[row * row_step + (c0 + j) * col_step]) : 0.f;
+      v[j] = __float_as_uint(f);
+      sum = fma((double)f, (double)f, sum);
+    }
+    tmem_st_32x32(tx + (uint32_t)c0, v);
+  }
+  tmem_st_wait();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int i = 0; i < kSmallThreads / 32; ++i) sum += part[i];
+  const float inv = (float)(1.0 / (sqrt(sum) + (double)p.eps));
+  for (int c0 = xc0; c0 < xc1; c0 += 32) {
+    uint32_t v[32];
+    float f[32];
+    tmem_ld_32x32(tx + (uint32_t)c0, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) { f[j] = __uint_as_float(v[j]) * inv; v[j] = __float_as_uint(f[j]); }
+    tmem_st_32x32(tx + (uint32_t)c0, v);
+    put_row(sx, row, c0, f);
+  }
+  tmem_st_wait();
+
+  uint32_t phase = 0;
+  // every thread's operand writes are visible, the product runs, every thread sees the accumulator
+  auto product = [&](const unsigned char* ma, const unsigned char* mb, bool b_mn, int n, int k) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0 && elect_one()) {
+      const uint32_t idesc = instr_desc<__half>(n) | ((uint32_t)b_mn << 16);
+      for (int i = 0; i < k; i += 16) {
+        const uint64_t da = smem_desc_sw128(ma + (i >> 6) * kBlock) + (uint64_t)((i & 63) * 2 / 16);
+        // as MN-major: 16 rows of K are 2048 bytes, the next 64 columns one block further
+        uint64_t db = smem_desc_sw128(mb + (b_mn ? i * 128 : (i >> 6) * kBlock)) + (uint64_t)(b_mn ? 0 : (i & 63) * 2 / 16);
+        if (b_mn) db = (db & ~((uint64_t)0x3fff << 16)) | (uint64_t)(kBlock >> 4) << 16;
+        tc_mma_f16(acc, da, db, idesc, i != 0);
+      }
+      tc_commit(&bar);
+    }
+    __syncwarp();
+    if (!mbar_wait_bounded(&bar, phase)) atomicExch(p.status, kStatusStageTimeout);
+    phase ^= 1;
+    tc_fence_after();
+  };
+  for (int step = 0; step < p.steps; ++step) {
+    const bool pair = step < p.keep, last = step == p.steps - 1;
+    product(sx, sx, false, n_gram, n_upd);                       // A = X X^T
+    for (int c0 = ac0; c0 < ac1; c0 += 32) {
+      uint32_t v[32];
+      float f[32];
+      tmem_ld_32x32(ta + (uint32_t)c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = row < p.p && c0 + j < p.p ? __uint_as_float(v[j]) : 0.f;
+      put_row(sa, row, c0, f);
+    }
+    product(sa, sa, false, n_gram, n_gram);                      // A A
+    for (int c0 = ac0; c0 < ac1; c0 += 32) {                     // B = b A + c A A (+ a on the diagonal)
+      uint32_t v[32];
+      float f[32];
+      tmem_ld_32x32(ta + (uint32_t)c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        const uint4 r = *reinterpret_cast<const uint4*>(sa + (c0 >> 6) * kBlock + block_at(row, ((c0 & 63) + j) >> 3));
+        const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 h = unpack_h(rr[e >> 1]);
+          const bool in = row < p.p && c0 + j + e < p.p;
+          f[j + e] = in ? fmaf(p.c, __uint_as_float(v[j + e]), p.b * (e & 1 ? h.y : h.x)) : 0.f;
+          if (!pair && in && row == c0 + j + e) f[j + e] += p.a;
+        }
+      }
+      put_row(sb, row, c0, f);
+    }
+    product(sb, sx, true, n_upd, n_gram);                        // B X
+    for (int c0 = xc0; c0 < xc1; c0 += 32) {
+      uint32_t v[32], w[32];
+      float f[32];
+      tmem_ld_32x32(ta + (uint32_t)c0, v);
+      if (pair) tmem_ld_32x32(tx + (uint32_t)c0, w);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        f[j] = row < p.p && c0 + j < p.q ? __uint_as_float(v[j]) : 0.f;
+        if (pair) f[j] = row < p.p && c0 + j < p.q ? fmaf(p.a, __uint_as_float(w[j]), f[j]) : 0.f;
+      }
+      if (last) {
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (long long)blockIdx.x * p.m * p.n;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (row < p.p && c0 + j < p.q) dst[row * row_step + (c0 + j) * col_step] = __float2bfloat16_rn(f[j]);
+      } else {
+        put_row(sx, row, c0, f);
+        if (step + 1 < p.keep) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(f[j]);
+          tmem_st_32x32(tx + (uint32_t)c0, w);
+        }
+      }
+    }
+    tmem_st_wait();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem_slot, (uint32_t)p.tmem_cols);
+  }
+}
+
 // ------------------------------------------------------------------- norm and scaling
 
 constexpr int kNormThreads = 256;
@@ -733,13 +934,44 @@ cudaError_t prepare(const void* x, const Layout& w, unsigned char* ws, long long
                            reinterpret_cast<__half*>(ws + w.l[0]), m, n, w.ldn, (int)chunks, eps, (int)vec);
 }
 
+bool small(int m, int n) { return (m < n ? m : n) <= kSmallP && (m < n ? n : m) <= kSmallQ; }
+
+template <typename T>
+cudaError_t launch_small(SmallParams p, long long batch, size_t smem, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev = dev < 0 || dev >= 64 ? 0 : dev;
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(ns_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (kSmallQ / 64 + 2 * kSmallP / 64) * kBlock + 1024);
+  });
+  if (attr_err[dev] != cudaSuccess) return attr_err[dev];
+  return launch_overlapped(ns_small_kernel<T>, dim3((unsigned)batch), dim3(kSmallThreads), smem, s, p);
+}
+
 }  // namespace
 
-size_t ns_workspace_bytes(long long batch, int m, int n) { return layout_of(batch, m, n).total; }
+size_t ns_workspace_bytes(long long batch, int m, int n) { return small(m, n) ? 0 : layout_of(batch, m, n).total; }
 
 // dtype: 0 fp32, 1 fp16, 2 bf16 of x; out is bf16.
 cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* workspace, long long batch, int m, int n,
                                  int steps, float a, float b, float c, float eps, int sms, int* status, cudaStream_t s) {
+  if (small(m, n)) {
+    SmallParams p = {};
+    p.x = x; p.out = out; p.m = m; p.n = n; p.tall = m > n;
+    p.p = p.tall ? n : m; p.q = p.tall ? m : n;
+    p.steps = steps; p.keep = steps - 2;
+    p.a = a; p.b = b; p.c = c; p.eps = eps; p.status = status;
+    const int qb = (p.q + 63) / 64, pb = (p.p + 63) / 64;
+    p.acc_col = qb * 64;
+    p.tmem_cols = 128;
+    while (p.tmem_cols < 2 * qb * 64) p.tmem_cols *= 2;       // X, and an accumulator as wide (p <= q)
+    const size_t smem = (size_t)(qb + 2 * pb) * kBlock + 1024;
+    return dtype == 0 ? launch_small<float>(p, batch, smem, s)
+           : dtype == 1 ? launch_small<__half>(p, batch, smem, s) : launch_small<__nv_bfloat16>(p, batch, smem, s);
+  }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const Layout w = layout_of(batch, m, n);
   cudaError_t e = dtype == 0   ? prepare<float>(x, w, ws, batch, m, n, eps, sms, s)

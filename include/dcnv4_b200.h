@@ -230,7 +230,7 @@ int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const 
  * (its trainers use stock optimisers); the product of Linear and convolution weights' updates is its use here.
  *   x    (batch, m, n) in `dtype` (fp32, fp16, bf16), any alignment;  out (batch, m, n) bf16, not overlapping x
  *   workspace  16-byte aligned, at least dcnv4b200_newton_schulz_workspace_bytes() bytes, private to calls that may
- *              overlap on the GPU
+ *              overlap on the GPU; NULL where that is 0 (matrices of at most 128 x 256, either way round)
  * m, n <= 65536, batch <= 65535, 1 <= steps <= 100 (DCNV4B200_ERR_UNSUPPORTED / _ERR_SHAPE otherwise).  The iteration
  * runs on fp16 tensor-core products with fp32 accumulation, with X carried in 22 bits until the last two steps; the
  * coefficients must keep |X| within fp16's range, as those of the published iteration do.  A zero matrix gives zeros,
