@@ -81,6 +81,7 @@ struct NsParams {
   int tall;
   int steps, keep;               // steps that carry the pair
   int batch;
+  int group1, group2;            // matrices of the task order's first two groups
   int sym_tiles, upd_tiles;      // tiles of a symmetric product, of an update
   int upd_n;                     // tile columns of an update
   unsigned total;                // tasks
@@ -141,30 +142,46 @@ __host__ __device__ inline int sym_cols(int i, int p) {
 }
 
 struct Task { int step, kind, bi, mt, nt; };
-// Task order: step by step, product by product, matrix by matrix.  (Groups of matrices a product apart, so that long and
-// short products run side by side, were slower: 733 against 677 us for 22 x 640x2560.  CTAs take tasks in order and the
-// distance between a matrix' product and its next one shrinks.)
+// Task order.  CTAs take tasks in order, so a task whose matrix is not ready holds up its CTA: the distance between a
+// matrix' product and its next one should be a wave of tasks or more.  A = X X^T has the fewest and longest tiles; the
+// matrices beyond its first wave of CTAs (group 3) finish it a whole tile later than the others.  So a step goes
+//   A of all | A A of groups 1, 2 | B X of 1 | A A of 3 | B X of 2 | B X of 3
+// with groups 1 and 2 the halves of the first wave.  (One product after the other for all matrices: CTAs waited 26 % of
+// the time at 22 x 640x2560.  Taking ready tiles of any matrix instead, from counters, cost more than it saved.)
 template <int BN>
 __device__ __forceinline__ Task task_of(unsigned t, const NsParams& p) {
   Task r;
-  const unsigned sym = p.batch * p.sym_tiles, per_step = 2 * sym + p.batch * p.upd_tiles;
+  const unsigned sym = p.sym_tiles, upd = p.upd_tiles;
+  const unsigned per_step = p.batch * (2 * sym + upd);
   r.step = (int)(t / per_step);
   unsigned i = t - r.step * per_step;
-  if (i < 2 * sym) {
-    r.kind = i < sym ? kGram : kPoly;
-    if (i >= sym) i -= sym;
-    r.bi = (int)(i / p.sym_tiles);
-    int tile = (int)(i - r.bi * p.sym_tiles), mt = 0;
+  const unsigned g1 = p.group1, g12 = p.group1 + p.group2, g3 = p.batch - g12;
+  unsigned first = 0;
+  if (i < p.batch * sym) {
+    r.kind = kGram;
+  } else if ((i -= p.batch * sym) < g12 * sym) {
+    r.kind = kPoly;
+  } else if ((i -= g12 * sym) < g1 * upd) {
+    r.kind = kUpdate;
+  } else if ((i -= g1 * upd) < g3 * sym) {
+    r.kind = kPoly;
+    first = g12;
+  } else {           // groups 2 and 3 follow one another
+    i -= g3 * sym;
+    r.kind = kUpdate;
+    first = g1;
+  }
+  const unsigned per = r.kind == kUpdate ? upd : sym, of = i / per;
+  int tile = (int)(i - of * per);
+  r.bi = (int)(first + of);
+  if (r.kind == kUpdate) {
+    r.mt = tile / p.upd_n;
+    r.nt = tile - r.mt * p.upd_n;
+  } else {
+    int mt = 0;
     for (int c = sym_cols<BN>(0, p.p); tile >= c; c = sym_cols<BN>(mt, p.p)) { tile -= c; ++mt; }
     r.mt = mt;
     r.nt = tile;
-  } else {
-    i -= 2 * sym;
-    r.kind = kUpdate;
-    r.bi = (int)(i / p.upd_tiles);
-    const unsigned tile = i - r.bi * p.upd_tiles;
-    r.mt = (int)(tile / p.upd_n);
-    r.nt = (int)(tile - r.mt * p.upd_n);
   }
   return r;
 }
@@ -902,6 +919,10 @@ cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
   const long long total = (long long)p.batch * p.steps * (2LL * p.sym_tiles + p.upd_tiles);
   if (total >= (1LL << 31)) return cudaErrorInvalidValue;
   p.total = (unsigned)total;
+  // the matrices whose A fits one wave of CTAs, in two halves; the rest are the third group
+  const int wave = sms / p.sym_tiles < p.batch ? sms / p.sym_tiles : p.batch;
+  p.group1 = (wave + 1) / 2;
+  p.group2 = wave - p.group1;
   // more CTAs than a product has tiles would only wait
   const long long most = (long long)p.batch * (p.sym_tiles > p.upd_tiles ? p.sym_tiles : p.upd_tiles);
   const unsigned grid = (unsigned)(most < sms ? most : sms);
