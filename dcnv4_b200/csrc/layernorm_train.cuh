@@ -15,7 +15,7 @@
 // so a tile of rows is one span per tensor, and a ring of such tiles is kept in flight with bulk copies (cp.async.bulk,
 // mbarriers, bounded waits) while the CTA's 8 or 16 warps compute: the bytes in flight do not depend on how many
 // registers a row takes.  A span only has to start on 16 bytes, so rows of any width use the ring; with a width that no
-// vector divides the lanes read shared memory element by element.
+// vector divides, teams keep to rows that start at the same distance from a vector boundary.
 //
 // A row belongs to a team of `lpr` lanes: 2..32 lanes of a warp, or all computing warps of the CTA.  A lane keeps its
 // NV vectors of the row, its slice of the parameters and of A and B in registers; statistics and sums are fp32, two
@@ -288,10 +288,23 @@ struct RingFill {
   }
 };
 
+// Widths that no vector divides.  Row r then starts r * C mod VEC elements behind a vector boundary, a pattern that repeats
+// after VEC / gcd(C, VEC) rows.  A team that takes rows of one residue only meets one shift: it reads and writes whole
+// vectors on the boundaries, its lanes own columns k * VEC + e - shift, and only the first and the last vector of a row
+// hold elements of the neighbouring rows, which are masked.
+// Word i of a vector whose elements [lo, hi) belong to the row.
+template <typename T>
+__device__ __forceinline__ uint32_t word_mask(int i, int lo, int hi) {
+  if constexpr (sizeof(T) == 4) return i >= lo && i < hi ? 0xffffffffu : 0u;
+  else return (2 * i >= lo && 2 * i < hi ? 0x0000ffffu : 0u) | (2 * i + 1 >= lo && 2 * i + 1 < hi ? 0xffff0000u : 0u);
+}
+
 // A lane's elements of a row in shared memory, as pairs.  VEC > 1: vectors sub, sub + lpr, ... of VEC elements, of which
-// only the last can lie beyond C (NV is the least that covers a row); VEC == 1: elements sub, sub + lpr, ...
-template <typename T, int VEC, int NV>
-__device__ __forceinline__ void row_load(float2 (&f)[NV * VEC / 2], const T* row, int sub, int lpr, int C, bool live) {
+// only the last can lie beyond C (NV is the least that covers a row; with a shift, the last two, and the first is
+// partial); VEC == 1: elements sub, sub + lpr, ...
+template <typename T, int VEC, int NV, bool SHIFT = false>
+__device__ __forceinline__ void row_load(float2 (&f)[NV * VEC / 2], const T* row, int sub, int lpr, int C, bool live,
+                                         int shift = 0) {
   if constexpr (VEC == 1) {
 #pragma unroll
     for (int v = 0; v < NV; v += 2) {
@@ -302,19 +315,25 @@ __device__ __forceinline__ void row_load(float2 (&f)[NV * VEC / 2], const T* row
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (sub + v * lpr) * VEC;
+      const int c = (sub + v * lpr) * VEC - (SHIFT ? shift : 0);
+      const bool edge = SHIFT && (v == 0 || v + 2 >= NV);
       constexpr int W = VEC * (int)sizeof(T) / 4;
+      const bool in = live && ((v + 1 < NV && !edge) || c < C);
       uint32_t r[W];
       if constexpr (W == 2) {
         uint2 t = make_uint2(0u, 0u);
-        if (live && (v + 1 < NV || c < C)) t = *reinterpret_cast<const uint2*>(row + c);
+        if (in) t = *reinterpret_cast<const uint2*>(row + c);
         r[0] = t.x; r[1] = t.y;
       }
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
         uint4 t = make_uint4(0u, 0u, 0u, 0u);
-        if (live && (v + 1 < NV || c < C)) t = reinterpret_cast<const uint4*>(row + c)[i];
+        if (in) t = reinterpret_cast<const uint4*>(row + c)[i];
         r[4 * i] = t.x; r[4 * i + 1] = t.y; r[4 * i + 2] = t.z; r[4 * i + 3] = t.w;
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) r[i] &= word_mask<T>(i, -c, C - c);
       }
       float w[VEC];
       widen(r, w, (const T*)nullptr);
@@ -328,8 +347,8 @@ template <typename T, int VEC, int NV>
 __device__ __forceinline__ void row_fetch(float2 (&f)[NV * VEC / 2], const T* row, int sub, int lpr, int C) {
   row_load<T, VEC, NV>(f, row, sub, lpr, C, true);
 }
-template <typename T, int VEC, int NV>
-__device__ __forceinline__ void row_store(T* row, const float2 (&f)[NV * VEC / 2], int sub, int lpr, int C) {
+template <typename T, int VEC, int NV, bool SHIFT = false>
+__device__ __forceinline__ void row_store(T* row, const float2 (&f)[NV * VEC / 2], int sub, int lpr, int C, int shift = 0) {
   if constexpr (VEC == 1) {
 #pragma unroll
     for (int v = 0; v < NV; v += 2) {
@@ -340,41 +359,48 @@ __device__ __forceinline__ void row_store(T* row, const float2 (&f)[NV * VEC / 2
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (sub + v * lpr) * VEC;
-      if (v + 1 < NV || c < C) {
-        float w[VEC];
+      const int c = (sub + v * lpr) * VEC - (SHIFT ? shift : 0);
+      const bool edge = SHIFT && (v == 0 || v + 2 >= NV);
+      float w[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC / 2; ++e) { w[2 * e] = f[v * VEC / 2 + e].x; w[2 * e + 1] = f[v * VEC / 2 + e].y; }
+      for (int e = 0; e < VEC / 2; ++e) { w[2 * e] = f[v * VEC / 2 + e].x; w[2 * e + 1] = f[v * VEC / 2 + e].y; }
+      if (edge ? c >= 0 && c + VEC <= C : v + 1 < NV || c < C) {
         uint32_t r[VEC * sizeof(T) / 4];
         narrow(w, r, (const T*)nullptr);
-        stg_raw(row + c, r);   // 16 or 32 bytes in one instruction
+        stg_raw(row + c, r);   // 8 or 16 bytes in one instruction
+      } else if (edge) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (c + e >= 0 && c + e < C) row[c + e] = from_f32<T>(w[e]);
       }
     }
   }
 }
-// Parameter slice in the same order; zero beyond C.
+// Parameter slice in the same order; zero outside the row.
 template <typename P, int VEC, int NV>
-__device__ __forceinline__ void param_load(float2 (&f)[NV * VEC / 2], const void* p, int sub, int lpr, int C, int f32) {
+__device__ __forceinline__ void param_load(float2 (&f)[NV * VEC / 2], const void* p, int sub, int lpr, int C, int f32,
+                                           int shift = 0) {
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int c = (sub + v * lpr) * VEC + e, i = v * VEC + e;
-      const float t = c < C ? param<P>(p, c, f32) : 0.f;
+      const int c = (sub + v * lpr) * VEC + e - shift, i = v * VEC + e;
+      const float t = c >= 0 && c < C ? param<P>(p, c, f32) : 0.f;
       if (i & 1) f[i / 2].y = t;
       else f[i / 2].x = t;
     }
 }
 // 16-byte loads where the parameters allow it: a launch's first rows wait for these.
-template <typename P, int VEC, int NV>
-__device__ __forceinline__ void param_fetch(float2 (&f)[NV * VEC / 2], const void* p, int sub, int lpr, int C, int f32) {
-  if constexpr (VEC > 1) {
+template <typename P, int VEC, int NV, bool SHIFT>
+__device__ __forceinline__ void param_fetch(float2 (&f)[NV * VEC / 2], const void* p, int sub, int lpr, int C, int f32,
+                                            int shift) {
+  if constexpr (VEC > 1 && !SHIFT) {
     if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
       if (f32) { row_fetch<float, VEC, NV>(f, static_cast<const float*>(p), sub, lpr, C); return; }
       if constexpr (sizeof(P) == 2) { row_fetch<P, VEC, NV>(f, static_cast<const P*>(p), sub, lpr, C); return; }
     }
   }
-  param_load<P, VEC, NV>(f, p, sub, lpr, C, f32);
+  param_load<P, VEC, NV>(f, p, sub, lpr, C, f32, shift);
 }
 // One fp32 parameter vector in shared memory, filled by the whole CTA.  For vectors of 8 their halves lie in two arrays, so
 // that the 16-byte loads of neighbouring lanes are neighbours (interleaved, they would meet in the same banks).
@@ -460,7 +486,7 @@ __device__ __forceinline__ float ring_sum(float t, int lpr, RingHeader* h, int& 
   return t;
 }
 
-template <typename TX, typename TY, int VEC, int NV, int MODE, bool GELU>
+template <typename TX, typename TY, int VEC, int NV, bool SHIFT, int MODE, bool GELU>
 __global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), fwd_ctas(VEC * NV))
 ln_ring_fwd_kernel(const LnTrainArgs a) {
   using P = TX;
@@ -481,6 +507,7 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
     const int sub = (int)threadIdx.x % lpr, team = (int)threadIdx.x / lpr;
     const int per_pass = W * 32 / lpr;                     // rows of one pass of the CTA
     const int first = lpr > 32 ? team : warp * (32 / lpr);  // first row of this warp in a pass
+    const int shift = SHIFT ? (int)((unsigned)team * (unsigned)C % VEC) : 0;
     const int passes = (a.tile_rows + per_pass - 1) / per_pass;
     const float inv_c = 1.f / (float)C;
     const uint32_t slot0 = fill.slot0(a), slot = slot0 + fill.slot1(a);
@@ -494,11 +521,11 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
       param_stage<P, VEC>(ws, a.w, g, C, a.param_f32);
       param_stage<P, VEC>(bs, a.b, g, C, a.param_f32);
     } else {
-      param_fetch<P, VEC, NV>(w, a.w, sub, lpr, C, a.param_f32);
-      param_fetch<P, VEC, NV>(b, a.b, sub, lpr, C, a.param_f32);
+      param_fetch<P, VEC, NV, SHIFT>(w, a.w, sub, lpr, C, a.param_f32, shift);
+      param_fetch<P, VEC, NV, SHIFT>(b, a.b, sub, lpr, C, a.param_f32, shift);
       if (MODE == kPost && a.gamma != nullptr) {
         float2 g[NE / 2];
-        param_fetch<P, VEC, NV>(g, a.gamma, sub, lpr, C, a.param_f32);
+        param_fetch<P, VEC, NV, SHIFT>(g, a.gamma, sub, lpr, C, a.param_f32, shift);
 #pragma unroll
         for (int i = 0; i < NE / 2; ++i) { w[i] = mul2(w[i], g[i]); b[i] = mul2(b[i], g[i]); }
       }
@@ -530,12 +557,12 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
         const bool live = lr < n;
         const int row = row0 + lr;
         float2 x[NE / 2], r[MODE == kPlain ? 1 : NE / 2];
-        row_load<TX, VEC, NV>(x, reinterpret_cast<const TX*>(base) + (size_t)lr * C, sub, lpr, C, live);
-        if constexpr (MODE != kPlain) row_load<TY, VEC, NV>(r, reinterpret_cast<const TY*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live);
+        row_load<TX, VEC, NV, SHIFT>(x, reinterpret_cast<const TX*>(base) + (size_t)lr * C, sub, lpr, C, live, shift);
+        if constexpr (MODE != kPlain) row_load<TY, VEC, NV, SHIFT>(r, reinterpret_cast<const TY*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live, shift);
         if constexpr (MODE == kPre) {
 #pragma unroll
           for (int i = 0; i < NE / 2; ++i) x[i] = fma2(both(s), x[i], r[i]);
-          if (live) row_store<TY, VEC, NV>(static_cast<TY*>(a.h) + (long long)row * C, x, sub, lpr, C);
+          if (live) row_store<TY, VEC, NV, SHIFT>(static_cast<TY*>(a.h) + (long long)row * C, x, sub, lpr, C, shift);
         }
         // two chains of additions each: a warp's own latency is what these short rows wait for
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -547,11 +574,14 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
 #pragma unroll
         for (int i = 0; i < NE / 2; ++i) {
           x[i] = add2(x[i], both(-mean));
-          if (VEC > 1) {
-            if (2 * i / VEC + 1 < NV || column<VEC>(2 * i, sub, lpr) < C) sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
-          } else {
-            if (column<VEC>(2 * i, sub, lpr) < C) sq[i & 1].x = fmaf(x[i].x, x[i].x, sq[i & 1].x);
-            if (column<VEC>(2 * i + 1, sub, lpr) < C) sq[i & 1].y = fmaf(x[i].y, x[i].y, sq[i & 1].y);
+          if (VEC > 1 && (SHIFT ? 2 * i / VEC != 0 && 2 * i / VEC + 2 < NV : 2 * i / VEC + 1 < NV)) {
+            sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
+          } else if (VEC > 1 && !SHIFT) {
+            if (column<VEC>(2 * i, sub, lpr) < C) sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
+          } else {      // the elements of a pair may differ in whether they belong to the row
+            const int c0 = column<VEC>(2 * i, sub, lpr) - shift, c1 = column<VEC>(2 * i + 1, sub, lpr) - shift;
+            if (c0 >= 0 && c0 < C) sq[i & 1].x = fmaf(x[i].x, x[i].x, sq[i & 1].x);
+            if (c1 >= 0 && c1 < C) sq[i & 1].y = fmaf(x[i].y, x[i].y, sq[i & 1].y);
           }
         }
         sq[0] = add2(sq[0], sq[1]);
@@ -573,7 +603,7 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
           if constexpr (MODE == kPost) o = fma2(both(s), o, r[i]);
           x[i] = o;
         }
-        row_store<TY, VEC, NV>(static_cast<TY*>(a.y) + (long long)row * C, x, sub, lpr, C);
+        row_store<TY, VEC, NV, SHIFT>(static_cast<TY*>(a.y) + (long long)row * C, x, sub, lpr, C, shift);
       }
       __syncwarp();
       if (lane == 0) ring_arrive(&h->empty[stage]);
@@ -584,7 +614,7 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
     for (int i = 0; i < 20000; ++i) __nanosleep(1000);
 }
 
-template <typename TL, typename TG, typename T2, typename P, int VEC, int NV, int MODE, bool GELU>
+template <typename TL, typename TG, typename T2, typename P, int VEC, int NV, bool SHIFT, int MODE, bool GELU>
 __global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), 1)
 ln_ring_bwd_kernel(const LnTrainArgs a) {
   constexpr int NE = VEC * NV, W = ring_warps<NE>();
@@ -595,6 +625,7 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
   const int tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
   const bool with_gh = MODE == kPre && a.gh != nullptr;
   const int sub = (int)threadIdx.x % lpr, team = (int)threadIdx.x / lpr;
+  const int shift = SHIFT ? (int)((unsigned)team * (unsigned)C % VEC) : 0;
   float2 sa[NE / 2], sb[NE / 2];
 #pragma unroll
   for (int i = 0; i < NE / 2; ++i) sa[i] = sb[i] = make_float2(0.f, 0.f);
@@ -619,11 +650,11 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
       param_stage<P, VEC>(ws, a.w, MODE == kPost ? a.gamma : nullptr, C, a.param_f32);
       if constexpr (GELU) param_stage<P, VEC>(bs, a.b, nullptr, C, a.param_f32);
     } else {
-      param_fetch<P, VEC, NV>(w, a.w, sub, lpr, C, a.param_f32);
-      if constexpr (GELU) param_fetch<P, VEC, NV>(b, a.b, sub, lpr, C, a.param_f32);
+      param_fetch<P, VEC, NV, SHIFT>(w, a.w, sub, lpr, C, a.param_f32, shift);
+      if constexpr (GELU) param_fetch<P, VEC, NV, SHIFT>(b, a.b, sub, lpr, C, a.param_f32, shift);
       if (MODE == kPost && a.gamma != nullptr) {
         float2 g[NE / 2];
-        param_fetch<P, VEC, NV>(g, a.gamma, sub, lpr, C, a.param_f32);
+        param_fetch<P, VEC, NV, SHIFT>(g, a.gamma, sub, lpr, C, a.param_f32, shift);
 #pragma unroll
         for (int i = 0; i < NE / 2; ++i) w[i] = mul2(w[i], g[i]);
       }
@@ -659,18 +690,18 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
         const bool live = lr < n;
         const int row = row0 + lr;
         float2 x[NE / 2], g[NE / 2];
-        row_load<TL, VEC, NV>(x, reinterpret_cast<const TL*>(base) + (size_t)lr * C, sub, lpr, C, live);
-        row_load<TG, VEC, NV>(g, reinterpret_cast<const TG*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live);
+        row_load<TL, VEC, NV, SHIFT>(x, reinterpret_cast<const TL*>(base) + (size_t)lr * C, sub, lpr, C, live, shift);
+        row_load<TG, VEC, NV, SHIFT>(g, reinterpret_cast<const TG*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live, shift);
         // elements beyond C have g = w = 0 and add nothing to any sum
         float2 t1[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, t2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if constexpr (kStaged) {
           param_row<VEC, NV>(w, ws, sub, lpr, C);
           if constexpr (GELU) param_row<VEC, NV>(b, bs, sub, lpr, C);
         }
-        const float2 r2 = both(rstd), shift = both(-mean);
+        const float2 r2 = both(rstd), minus_mean = both(-mean);
 #pragma unroll
         for (int i = 0; i < NE / 2; ++i) {
-          x[i] = mul2(add2(x[i], shift), r2);
+          x[i] = mul2(add2(x[i], minus_mean), r2);
           if (MODE == kPost) g[i] = mul2(g[i], both(s));
           if constexpr (GELU) {
             const float2 z = fma2(x[i], w[i], b[i]);
@@ -693,28 +724,28 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
 #pragma unroll
           for (int i = 0; i < NE / 2; ++i) x[i] = fma2(x[i], m2, fma2(g[i], r2, m1));
           if (with_gh) {
-            row_load<TG, VEC, NV>(g, reinterpret_cast<const TG*>(base + slot0 + slot1) + (size_t)lr * C, sub, lpr, C, true);
+            row_load<TG, VEC, NV, SHIFT>(g, reinterpret_cast<const TG*>(base + slot0 + slot1) + (size_t)lr * C, sub, lpr, C, true, shift);
 #pragma unroll
             for (int i = 0; i < NE / 2; ++i) x[i] = add2(x[i], g[i]);
           }
-          row_store<TL, VEC, NV>(static_cast<TL*>(a.dx) + (long long)row * C, x, sub, lpr, C);
+          row_store<TL, VEC, NV, SHIFT>(static_cast<TL*>(a.dx) + (long long)row * C, x, sub, lpr, C, shift);
           if (a.dx2 != nullptr) {
 #pragma unroll
             for (int i = 0; i < NE / 2; ++i) x[i] = mul2(x[i], both(s));
-            row_store<T2, VEC, NV>(static_cast<T2*>(a.dx2) + (long long)row * C, x, sub, lpr, C);
+            row_store<T2, VEC, NV, SHIFT>(static_cast<T2*>(a.dx2) + (long long)row * C, x, sub, lpr, C, shift);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < NE / 2; ++i) x[i] = fma2(x[i], m2, fma2(g[i], r2, m1));
-          row_store<TL, VEC, NV>(static_cast<TL*>(a.dx) + (long long)row * C, x, sub, lpr, C);
+          row_store<TL, VEC, NV, SHIFT>(static_cast<TL*>(a.dx) + (long long)row * C, x, sub, lpr, C, shift);
         }
       }
       __syncwarp();
       if (lane == 0) ring_arrive(&h->empty[stage]);
       if (++stage == a.stages) { stage = 0; phase ^= 1; }
     }
-    // over the teams of each warp
-    for (int o = lpr; o < 32; o <<= 1) {
+    // over the teams of each warp (which own the same columns, unless they are shifted)
+    for (int o = SHIFT ? 32 : lpr; o < 32; o <<= 1) {
 #pragma unroll
       for (int i = 0; i < NE / 2; ++i) {
         sa[i].x += __shfl_xor_sync(0xffffffffu, sa[i].x, o);
@@ -729,12 +760,13 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
   // over the warps, or the teams of several warps, through the ring's memory: every tile has been consumed
   __syncthreads();
   float* acc = reinterpret_cast<float*>(ring);     // [slots][2][C]
-  const int slots = lpr > 32 ? W * 32 / lpr : W, slot = lpr > 32 ? team : warp;
-  if (lpr > 32 || lane < lpr) {
+  const bool by_team = SHIFT || lpr > 32;
+  const int slots = by_team ? W * 32 / lpr : W, slot = by_team ? team : warp;
+  if (by_team || lane < lpr) {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int c = column<VEC>(i, sub, lpr);
-      if (c < C) {
+      const int c = column<VEC>(i, sub, lpr) - shift;
+      if (c >= 0 && c < C) {
         acc[(slot * 2) * C + c] = i & 1 ? sa[i / 2].y : sa[i / 2].x;
         acc[(slot * 2 + 1) * C + c] = i & 1 ? sb[i / 2].y : sb[i / 2].x;
       }
@@ -998,7 +1030,7 @@ struct Geometry {
 // A lane holds 1..max_nv vectors (of 8 elements up to 3, of 4 up to 6), or 4, 8, 12 or 16 single elements.  A row costs its team's lanes about as much for its
 // bookkeeping as ten more elements a lane would: fewest lanes * (elements + 10) wins.  A team divides the warps of
 // the CTA (16, or 12 where a lane holds more than 16 elements).
-inline Geometry geometry(int n, int vec, int max_nv) {
+inline Geometry geometry(int n, int vec, int max_nv, int period = 1) {
   Geometry best{0, 0, 0, false};
   long long best_cost = 0;
   for (int lpr = 2; lpr <= 512; lpr *= 2) {
@@ -1006,7 +1038,7 @@ inline Geometry geometry(int n, int vec, int max_nv) {
     if (vec == 1) nv = (nv + 3) / 4 * 4;
     if (nv > (vec == 1 ? 16 : max_nv)) continue;
     const int warps = warps_for(nv * vec);
-    if (warps * 32 % lpr != 0) continue;
+    if (warps * 32 % lpr != 0 || warps * 32 / lpr % period != 0) continue;   // shifted rows: a team keeps its residue
     const long long cost = (long long)lpr * (nv * vec + 10);
     if (!best.ok || cost < best_cost) { best_cost = cost; best = Geometry{lpr, nv, warps, true}; }
   }
@@ -1080,23 +1112,32 @@ struct Plan {
   Geometry g;
   Ring ring;
   int vec;       // elements per vector; 1 element-wise
+  bool shift;    // vectors of rows that start between boundaries
   bool direct;
   int grid;
 };
 inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool base16, bool vec_ok, int rows, int C) {
   Plan p;
   const int V = x_es == 4 || y_es == 4 ? 4 : 8;
-  p.vec = vec_ok && base16 && C % V == 0 ? V : 1;
-  p.g = geometry(p.vec > 1 ? C / V : C, p.vec, V == 8 ? 3 : 6);
+  p.vec = vec_ok && base16 ? V : 1;
+  p.shift = p.vec > 1 && C % V != 0;
+  if (p.shift) {   // up to V - 1 elements in front of a row's first; 16 elements a lane, whose parameters are in registers
+    int period = V;
+    for (int c = C; c % 2 == 0; c /= 2) period /= 2;
+    p.g = geometry((C + 2 * V - 2) / V, V, 16 / V, period);
+    if (!p.g.ok) { p.shift = false; p.vec = 1; }
+  }
+  if (!p.shift) p.g = geometry(p.vec > 1 ? C / V : C, p.vec, V == 8 ? 3 : 6);
   const int lx = backward && mode == kPre ? y_es : x_es;      // element size of the normalised tensor
   const size_t row_bytes = (size_t)C * (backward ? lx + y_es * (1 + (mode == kPre && gh)) : x_es + (mode == kPlain ? 0 : y_es));
   const int es_min = backward ? (lx < y_es ? lx : y_es) : (mode == kPlain || x_es < y_es ? x_es : y_es);
-  const int slots = p.g.lpr > 32 ? p.g.warps * 32 / p.g.lpr : p.g.warps;
+  const int slots = p.shift || p.g.lpr > 32 ? p.g.warps * 32 / p.g.lpr : p.g.warps;
   const size_t acc = backward ? (size_t)slots * 2 * C * sizeof(float) : 0;
   const size_t params = p.g.nv * p.vec > 16 || (p.vec == 1 && p.g.nv > 8) ? (size_t)2 * ((C + 3) / 4 * 4) * sizeof(float) : 0;
   p.direct = !base16 || acc > kRingBytes || !ring_for(rows, p.g, row_bytes, align_rows(C, es_min), acc, params, backward ? 1 : fwd_ctas(p.g.nv * p.vec), &p.ring);
   if (p.direct) {
     p.vec = 1;
+    p.shift = false;
     p.g = geometry(C, 1, 0);
     if (p.g.nv != 4) p.g.nv = 16;   // the element-wise kernels come with 4 and 16
   }
@@ -1123,18 +1164,18 @@ cudaError_t launch_ring(const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
   return launch_overlapped(Kern, dim3((unsigned)p.grid), dim3((unsigned)(32 * p.g.warps)), p.ring.smem, s, a);
 }
 
-template <typename TX, typename TY, int VEC, int NV>
+template <typename TX, typename TY, int VEC, int NV, bool SHIFT = false>
 cudaError_t ring_run(bool backward, int mode, int act, const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
   if (!backward) {
-    if (mode == kPost) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPost, false>>(a, p, s);
-    if (mode == kPre) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPre, false>>(a, p, s);
-    if (act) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPlain, true>>(a, p, s);
-    return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, kPlain, false>>(a, p, s);
+    if (mode == kPost) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, SHIFT, kPost, false>>(a, p, s);
+    if (mode == kPre) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, SHIFT, kPre, false>>(a, p, s);
+    if (act) return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, SHIFT, kPlain, true>>(a, p, s);
+    return launch_ring<ln_ring_fwd_kernel<TX, TY, VEC, NV, SHIFT, kPlain, false>>(a, p, s);
   }
-  if (mode == kPre) return launch_ring<ln_ring_bwd_kernel<TY, TY, TX, TX, VEC, NV, kPre, false>>(a, p, s);
-  if (mode == kPost) return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPost, false>>(a, p, s);
-  if (act) return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPlain, true>>(a, p, s);
-  return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, kPlain, false>>(a, p, s);
+  if (mode == kPre) return launch_ring<ln_ring_bwd_kernel<TY, TY, TX, TX, VEC, NV, SHIFT, kPre, false>>(a, p, s);
+  if (mode == kPost) return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, SHIFT, kPost, false>>(a, p, s);
+  if (act) return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, SHIFT, kPlain, true>>(a, p, s);
+  return launch_ring<ln_ring_bwd_kernel<TX, TY, TX, TX, VEC, NV, SHIFT, kPlain, false>>(a, p, s);
 }
 template <typename TX, typename TY, int NV>
 cudaError_t direct_run(bool backward, int mode, int act, const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
@@ -1166,6 +1207,15 @@ cudaError_t run(bool backward, int mode, int act, const Plan& p, const LnTrainAr
     if (p.g.nv == 8) return ring_run<TX, TY, 1, 8>(backward, mode, act, a, p, s);
     if (p.g.nv == 12) return ring_run<TX, TY, 1, 12>(backward, mode, act, a, p, s);
     return ring_run<TX, TY, 1, 16>(backward, mode, act, a, p, s);
+  }
+  if (p.shift) {
+    if (p.g.nv == 1) return ring_run<TX, TY, V, 1, true>(backward, mode, act, a, p, s);
+    if (p.g.nv == 2) return ring_run<TX, TY, V, 2, true>(backward, mode, act, a, p, s);
+    if constexpr (V == 4) {
+      if (p.g.nv == 3) return ring_run<TX, TY, V, 3, true>(backward, mode, act, a, p, s);
+      if (p.g.nv == 4) return ring_run<TX, TY, V, 4, true>(backward, mode, act, a, p, s);
+    }
+    return cudaErrorInvalidValue;
   }
   switch (p.g.nv) {
     case 1: return ring_run<TX, TY, V, 1>(backward, mode, act, a, p, s);

@@ -476,3 +476,15 @@ def test_refusals():
         ops.layer_norm_backward(y, x, m[:2].contiguous(), r, w, w)
     with pytest.raises(RuntimeError, match="float64|supports"):
         ops.layer_norm_train_forward(x.double(), w.double(), w.double(), EPS)
+
+
+@pytest.mark.parametrize("tx,ty", PAIRS, ids=IDS)
+@pytest.mark.parametrize("C", [3, 9, 12, 20, 33, 62, 100, 129, 250, 515, 1001, 1004, 1010, 1011, 1018, 2042, 2044, 4094])
+def test_widths_no_vector_divides(C, tx, ty):
+    """Every distance of a row's start from a vector boundary, a last tile that ends inside one, one sample per few rows."""
+    for rows, samples in ((8, 2), (333, 3), (1500 if C < 600 else 40, 4)):
+        d = make(rows, C, tx, ty, F32 if rows % 2 else tx, samples=samples)
+        check_plain(d)
+        check_post(d)
+        check_pre(d)
+    check_plain(make(37, C, tx, ty, F32), "gelu")
