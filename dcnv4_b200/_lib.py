@@ -7,11 +7,13 @@ made without a CUDA tensor, an exception is raised.  Build the library with
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_C", "libdcnv4_b200.so")
+BINDINGS_PATH = os.path.join(HERE, "_C", "dcnv4_b200_bindings.so")
 ABI_VERSION = 1
 
 F32, F16, BF16 = 0, 1, 2
@@ -81,6 +83,27 @@ def lib() -> C.CDLL:
                 raise LibraryError(f"ABI mismatch: library {got}, python {ABI_VERSION}; rebuild the library")
             _lib = handle
     return _lib
+
+
+_bindings = None
+
+
+def bindings():
+    """The binding of the latency-critical entry points (csrc/bindings.cpp), handed the library's functions."""
+    global _bindings
+    handle = lib()
+    with _lock:
+        if _bindings is None:
+            if not os.path.exists(BINDINGS_PATH):
+                raise LibraryError(f"{BINDINGS_PATH} not found: run `python -m dcnv4_b200.build`")
+            spec = importlib.util.spec_from_file_location("dcnv4_b200_bindings", BINDINGS_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.init(*(C.cast(fn, C.c_void_p).value for fn in (
+                handle.dcnv4b200_layernorm_train_fwd, handle.dcnv4b200_layernorm_train_bwd,
+                handle.dcnv4b200_layernorm_train_bwd_workspace_bytes)))
+            _bindings = module
+    return _bindings
 
 
 def check(rc: int, what: str) -> None:

@@ -1,4 +1,5 @@
-"""Build the CUDA library in-tree: dcnv4_b200/csrc/*.cu -> dcnv4_b200/_C/libdcnv4_b200.so.
+"""Build the CUDA library in-tree, dcnv4_b200/csrc/*.cu -> dcnv4_b200/_C/libdcnv4_b200.so, and the Python binding of its
+latency-critical entry points, dcnv4_b200/csrc/bindings.cpp -> dcnv4_b200/_C/dcnv4_b200_bindings.so.
 
     python -m dcnv4_b200.build [--force] [--verbose]
 
@@ -8,16 +9,19 @@ packages.  nvcc cross-compiles without a GPU, so this also runs on a CPU-only bu
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_C")
 LIB = os.path.join(OUT_DIR, "libdcnv4_b200.so")
+BINDINGS = os.path.join(OUT_DIR, "dcnv4_b200_bindings.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ("api.cu", "dcnv4_fwd.cu", "dcnv4_bwd.cu", "dcnv4_bwd_tiled.cu", "dcnv4_fwd_tiled.cu", "dcnv4_fwd_fused.cu", "fda_fwd.cu", "fda_bwd.cu", "aux.cu", "layernorm.cu",
@@ -35,13 +39,28 @@ def _nvcc() -> str:
     return exe
 
 
+def _build_bindings(nvcc: str) -> None:
+    """bindings.cpp uses PyTorch's C++ headers (tensors in, tensors out) and no CUDA code of its own."""
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    inc = os.path.join(torch_dir, "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-I", sysconfig.get_paths()["include"], "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-I", cuda, os.path.join(CSRC, "bindings.cpp"), "-o", BINDINGS, "-L", os.path.join(torch_dir, "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed on bindings.cpp")
+
+
 def _deps_mtime() -> float:
     files = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(INCLUDE, "dcnv4_b200.h")]
     return max(os.path.getmtime(f) for f in files)
 
 
 def is_current() -> bool:
-    return os.path.exists(LIB) and os.path.getmtime(LIB) >= _deps_mtime()
+    return all(os.path.exists(f) and os.path.getmtime(f) >= _deps_mtime() for f in (LIB, BINDINGS))
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -61,8 +80,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError(f"nvcc failed on {src}")
         return obj
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        bindings = ex.submit(_build_bindings, nvcc)
         objs = list(ex.map(compile_one, SOURCES))
+        bindings.result()
     link = [nvcc, *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs]
     r = subprocess.run(link, capture_output=True, text=True)
     if r.returncode != 0:

@@ -262,8 +262,9 @@ def layer_norm_train_supported(x: torch.Tensor, weight: torch.Tensor, out_dtype:
             and weight.dtype in (torch.float32, x.dtype) and out_dtype in (None, torch.float32, x.dtype))
 
 
-def _refuse_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
-    """Raises for the first thing that is wrong with the arguments of a training pass; returns if nothing is."""
+def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
+    """Argument checks of the training passes; returns (rows, C, rows_per_sample).  `x_dtype` is the dtype of the
+    branch input (x itself, except in the backward pass over a stored sum)."""
     C = x.shape[-1] if x.dim() else 0
     for t, n in ((x, "input"), (weight, "weight"), (bias, "bias"), (layer_scale, "layer_scale"),
                  (sample_scale, "sample_scale")):
@@ -288,37 +289,13 @@ def _refuse_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_
             _check_tensor(t, n)
             if t.shape != x.shape or t.dtype != out_dtype or t.device != x.device:
                 raise RuntimeError(f"{n} must have the shape of the input, dtype {out_dtype}, and its device")
+    rows = x.numel() // C
+    per = rows
     if sample_scale is not None:
         n = sample_scale.numel()
         if sample_scale.dtype != torch.float32 or x.dim() < 2 or (x.shape[0] % n if n else x.shape[0]) != 0:
             raise RuntimeError("sample_scale must be float32 with one factor per sample (its size divides the first "
                                "dimension of the input)")
-
-
-def _plain_cuda(t, device, dtype):
-    return t.device == device and t.dtype == dtype and t.is_contiguous()
-
-
-def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype):
-    """Argument checks of the training passes; returns (rows, C, rows_per_sample).  `x_dtype` is the dtype of the
-    branch input (x itself, except in the backward pass over a stored sum).  What an ordinary call looks like is
-    accepted at once; anything else goes through the checks one by one."""
-    device, shape, p_dtype = x.device, x.shape, weight.dtype
-    C = shape[-1] if shape else 0
-    if not (x.is_cuda and x.is_contiguous() and C > 0 and x.dtype in _DTYPES
-            and (sample_scale is None or (len(shape) > 1 and _plain_cuda(sample_scale, device, torch.float32)
-                                          and sample_scale.numel() > 0 and shape[0] % sample_scale.numel() == 0))
-            and x_dtype in _DTYPES and (out_dtype == torch.float32 or out_dtype == x_dtype)
-            and (p_dtype == torch.float32 or p_dtype == x_dtype)
-            and _plain_cuda(weight, device, p_dtype) and weight.numel() == C
-            and _plain_cuda(bias, device, p_dtype) and bias.numel() == C
-            and (layer_scale is None or (_plain_cuda(layer_scale, device, p_dtype) and layer_scale.numel() == C))
-            and all(t is None or (_plain_cuda(t, device, out_dtype) and t.shape == shape) for t, _ in others)):
-        _refuse_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_dtype)
-    rows = x.numel() // C
-    per = rows
-    if sample_scale is not None:
-        n = sample_scale.numel()
         per = max(rows // n, 1) if n else 1
     return rows, C, per
 
@@ -327,7 +304,25 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_binding = None
+
+
+def _load_binding():
+    global _binding
+    _binding = _lib.bindings()
+    return _binding
+
+
 def _ln_forward(mode, x, residual, weight, bias, eps, layer_scale, sample_scale, activation, out_dtype, what):
+    """(y, mean, rstd), with h in front for the pre-norm seam.  The binding takes ordinary calls; what it declines -- wrong
+    arguments, empty tensors, a device that is not the current one -- comes through here."""
+    act = 1 if activation == "gelu" else 0
+    got = (_binding or _load_binding()).ln_forward(mode, x, residual, weight, bias, eps, layer_scale, sample_scale, act,
+                                                   _DTYPES.get(out_dtype, -1))
+    if got.__class__ is tuple:
+        return got
+    if got is not None:
+        _lib.check(got, what)
     rows, C, per = _check_ln(x, x.dtype, weight, bias, ((residual, "residual"),), layer_scale, sample_scale, out_dtype)
     y = torch.empty_like(x) if out_dtype == x.dtype else x.new_empty(x.shape, dtype=out_dtype)
     h = torch.empty_like(y) if mode == _LN_PRE else None
@@ -336,21 +331,27 @@ def _ln_forward(mode, x, residual, weight, bias, eps, layer_scale, sample_scale,
     rc = _on_device(
         x, _lib.lib().dcnv4b200_layernorm_train_fwd, x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(),
         _ptr(layer_scale), _ptr(sample_scale), y.data_ptr(), _ptr(h), mean.data_ptr(), rstd.data_ptr(), mode,
-        _DTYPES[x.dtype], _DTYPES[out_dtype], _DTYPES[weight.dtype], rows, C, per, eps, 1 if activation == "gelu" else 0,
-        _stream(x))
-    if rc:
-        _lib.check(rc, what)
-    return y, h, mean, rstd
+        _DTYPES[x.dtype], _DTYPES[out_dtype], _DTYPES[weight.dtype], rows, C, per, eps, act, _stream(x))
+    _lib.check(rc, what)
+    return (y, mean, rstd) if h is None else (h, y, mean, rstd)
 
 
 def _ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale, sample_scale, activation, x_dtype,
                  what):
+    """(grad_x, grad_branch, grad_weight, grad_bias, grad_layer_scale); see `_ln_forward`."""
+    act = 1 if activation == "gelu" else 0
+    got = (_binding or _load_binding()).ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale,
+                                                    sample_scale, act, _DTYPES.get(x_dtype, -1))
+    if got.__class__ is tuple:
+        return got
+    if got is not None:
+        _lib.check(got, what)
     out_dtype = grad_y.dtype
     pre = mode == _LN_PRE
     grads = ((grad_y, "grad_y"), (grad_h, "grad_h"), (x, "h")) if pre else ((grad_y, "grad_y"),)
     rows, C, per = _check_ln(x, x_dtype, weight, bias, grads, layer_scale, sample_scale, out_dtype)
     for t in (mean, rstd):
-        if not (_plain_cuda(t, x.device, torch.float32) and t.numel() == rows):
+        if not (t.device == x.device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == rows):
             raise RuntimeError("mean and rstd must be the float32 row statistics the forward pass returned")
     lib = _lib.lib()
     code = _DTYPES[x_dtype]
@@ -365,9 +366,8 @@ def _ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale,
         x, lib.dcnv4b200_layernorm_train_bwd, grad_y.data_ptr(), _ptr(grad_h), x.data_ptr(), mean.data_ptr(),
         rstd.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale), grad_x.data_ptr(),
         _ptr(branch), grad_w.data_ptr(), grad_b.data_ptr(), _ptr(grad_s), ws.data_ptr(), ws_bytes, mode, code,
-        _DTYPES[out_dtype], _DTYPES[weight.dtype], rows, C, per, 1 if activation == "gelu" else 0, _stream(x))
-    if rc:
-        _lib.check(rc, what)
+        _DTYPES[out_dtype], _DTYPES[weight.dtype], rows, C, per, act, _stream(x))
+    _lib.check(rc, what)
     return grad_x, grad_x if branch is None else branch, grad_w, grad_b, grad_s
 
 
@@ -379,9 +379,8 @@ def layer_norm_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.
     1 to 8192 channels."""
     if activation not in ("none", "gelu"):
         raise ValueError("activation must be 'none' or 'gelu'")
-    y, _, mean, rstd = _ln_forward(_LN_PLAIN, x, None, weight, bias, eps, None, None, activation,
-                                   x.dtype if out_dtype is None else out_dtype, "layer_norm_train_forward")
-    return y, mean, rstd
+    return _ln_forward(_LN_PLAIN, x, None, weight, bias, eps, None, None, activation,
+                       x.dtype if out_dtype is None else out_dtype, "layer_norm_train_forward")
 
 
 def layer_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -402,9 +401,8 @@ def layer_norm_residual_forward(x: torch.Tensor, residual: torch.Tensor, weight:
     the row statistics as (out, mean, rstd).  `layer_scale` (C) like weight; `sample_scale` (N) float32, one factor
     per sample of the first dimension (stochastic depth: 0 or 1 / keep probability).  out and residual have the dtype
     of x or are float32."""
-    out, _, mean, rstd = _ln_forward(_LN_POST, x, residual, weight, bias, eps, layer_scale, sample_scale, "none",
-                                     residual.dtype, "layer_norm_residual_forward")
-    return out, mean, rstd
+    return _ln_forward(_LN_POST, x, residual, weight, bias, eps, layer_scale, sample_scale, "none", residual.dtype,
+                       "layer_norm_residual_forward")
 
 
 def layer_norm_residual_backward(grad_out: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -422,9 +420,8 @@ def add_layer_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: torc
     """The seam of two pre-norm branches in one pass: h = residual + sample_scale * x and y = LN(h), returned as
     (h, y, mean, rstd).  Statistics and y are taken of the fp32 sum, before h is rounded.  Types and `sample_scale`
     as `layer_norm_residual_forward`."""
-    y, h, mean, rstd = _ln_forward(_LN_PRE, x, residual, weight, bias, eps, None, sample_scale, "none",
-                                   residual.dtype, "add_layer_norm_forward")
-    return h, y, mean, rstd
+    return _ln_forward(_LN_PRE, x, residual, weight, bias, eps, None, sample_scale, "none", residual.dtype,
+                       "add_layer_norm_forward")
 
 
 def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor], h: torch.Tensor, mean: torch.Tensor,
