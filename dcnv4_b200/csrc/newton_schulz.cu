@@ -24,10 +24,14 @@
 // first, and a single small matrix pays a flag in memory between products instead of a kernel launch.  Every task that is
 // waited for has been taken by a running CTA, so the order of progress needs no co-residency.  Warps:
 //   warp 0     takes tasks, waits for what they need, TMA loads of the two operand tiles (64 x 64 boxes, 128-byte swizzle)
-//   warp 1     tcgen05.mma (M 128, N BN, K 16) into one of two accumulators in tensor memory
+//   warp 1     tcgen05.mma (M 128 or 256, N BN, K 16) into one of two accumulators in tensor memory
 //   last warp  counts the finished tiles
 //   others     epilogue: 32 x 32 units from tensor memory; the previous X (hi, lo) or A arrives by TMA
 //              in the staging buffer that the result leaves from
+// Large stacks give the tiles to pairs of CTAs (cta_group::2): a CTA loads its 128 rows of A and half of B's columns, so
+// that the operands cost 2/3 of the L2 traffic and of the shared memory's bandwidth, which is what a 128 x 256 tile is
+// short of (its 48 KB per 64 of K are written once and read once in the 512 cycles of the products).  The leader takes
+// the tasks, hands them to both queues and issues the products; each CTA has its own epilogue and counts its half.
 // Every mbarrier wait is bounded; one that runs out sets the device status word and the CTA winds down.
 //
 // Matrices with p <= 128 and q <= 256 take another kernel: one CTA holds a whole matrix (X and A, B as fp16 operands in shared
@@ -60,13 +64,15 @@ constexpr float kLoScale = 2048.f;
 
 enum : int { kGram = 0, kPoly = 1, kUpdate = 2 };
 
-template <int BN> constexpr int slot_bytes() { return (2 + BN / 64) * kBox; }
-template <int BN> constexpr int ns_stages() {
+// PAIR: two CTAs of a cluster share a 256 x BN tile, each with its 128 rows and half of the columns' operand.
+template <bool PAIR> constexpr int tile_m() { return PAIR ? 256 : 128; }
+template <int BN, bool PAIR> constexpr int slot_bytes() { return (2 + BN / (PAIR ? 128 : 64)) * kBox; }
+template <int BN, bool PAIR> constexpr int ns_stages() {
   constexpr int room = 227 * 1024 - 1024 - kBarBytes - epi_warps<BN>() * kStagingWarp;
-  return room / slot_bytes<BN>() > 6 ? 6 : room / slot_bytes<BN>();
+  return room / slot_bytes<BN, PAIR>() > 6 ? 6 : room / slot_bytes<BN, PAIR>();
 }
-template <int BN> constexpr size_t ns_smem() {
-  return (size_t)ns_stages<BN>() * slot_bytes<BN>() + epi_warps<BN>() * kStagingWarp + kBarBytes + 1024;
+template <int BN, bool PAIR> constexpr size_t ns_smem() {
+  return (size_t)ns_stages<BN, PAIR>() * slot_bytes<BN, PAIR>() + epi_warps<BN>() * kStagingWarp + kBarBytes + 1024;
 }
 
 // Tensor maps of a call: 64 x 64 boxes of the operands, 32 x 32 boxes of what an epilogue reads and writes.
@@ -135,9 +141,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {   //
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 // Tile columns of row block i of a symmetric product: those that reach the diagonal or lie left of it.
-template <int BN>
+template <int BN, int TM>
 __host__ __device__ inline int sym_cols(int i, int p) {
-  const int c = (i * kBM + kBM - 1) / BN + 1, most = (p + BN - 1) / BN;
+  const int c = (i * TM + TM - 1) / BN + 1, most = (p + BN - 1) / BN;
   return c < most ? c : most;
 }
 
@@ -148,7 +154,7 @@ struct Task { int step, kind, bi, mt, nt; };
 //   A of all | A A of groups 1, 2 | B X of 1 | A A of 3 | B X of 2 | B X of 3
 // with groups 1 and 2 the halves of the first wave.  (One product after the other for all matrices: CTAs waited 26 % of
 // the time at 22 x 640x2560.  Taking ready tiles of any matrix instead, from counters, cost more than it saved.)
-template <int BN>
+template <int BN, int TM>
 __device__ __forceinline__ Task task_of(unsigned t, const NsParams& p) {
   Task r;
   const unsigned sym = p.sym_tiles, upd = p.upd_tiles;
@@ -179,7 +185,7 @@ __device__ __forceinline__ Task task_of(unsigned t, const NsParams& p) {
     r.nt = tile - r.mt * p.upd_n;
   } else {
     int mt = 0;
-    for (int c = sym_cols<BN>(0, p.p); tile >= c; c = sym_cols<BN>(mt, p.p)) { tile -= c; ++mt; }
+    for (int c = sym_cols<BN, TM>(0, p.p); tile >= c; c = sym_cols<BN, TM>(mt, p.p)) { tile -= c; ++mt; }
     r.mt = mt;
     r.nt = tile;
   }
@@ -201,15 +207,61 @@ __device__ __forceinline__ uint32_t pack_b(float x, float y) {
 }
 __device__ __forceinline__ float2 unpack_h(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-template <int BN>
+// ---- two CTAs of a cluster ----
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+// Address, in the cluster's window, of a CTA's copy of something in shared memory; rank 0 is the leader.
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity) {   // bounded, as mbar_wait_bounded
+  for (int i = 0; i < (1 << 22); ++i) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Into this CTA's shared memory, the bytes counted by a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {     // arrives at this barrier in both CTAs
+  const uint16_t both_ctas = 3;
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"(both_ctas) : "memory");
+}
+
+template <int BN, bool PAIR>
 __global__ void __launch_bounds__(ns_threads<BN>(), 1)
 ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kStages = ns_stages<BN>();
-  constexpr uint32_t kSlot = slot_bytes<BN>();
+  constexpr int kStages = ns_stages<BN, PAIR>();
+  constexpr uint32_t kSlot = slot_bytes<BN, PAIR>();
   constexpr int kEpiWarps = epi_warps<BN>();
-  unsigned char* ring = smem;                      // per slot: A (2 boxes), B (BN / 64 boxes)
+  constexpr int TM = tile_m<PAIR>();
+  constexpr int kBoxesB = BN / (PAIR ? 128 : 64);
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  unsigned char* ring = smem;                      // per slot: A (2 boxes), B (kBoxesB boxes)
   unsigned char* staging = smem + kStages * kSlot;
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingWarp);
   uint64_t* full = bars;
@@ -233,23 +285,39 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
     };
     for (int s = 0; s < kStages; ++s) { init(&full[s], 1); init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { init(&acc_full[a], 1); init(&acc_empty[a], kEpiWarps); }
-    for (int q = 0; q < kQueue; ++q) { init(&task_full[q], 1); init(&task_empty[q], 1 + kEpiWarps); init(&tile_done[q], kEpiWarps); init(&tile_free[q], 1); }
+    for (int a = 0; a < 2; ++a) { init(&acc_full[a], 1); init(&acc_empty[a], (PAIR ? 2 : 1) * kEpiWarps); }
+    for (int q = 0; q < kQueue; ++q) { init(&task_full[q], 1); init(&task_empty[q], (PAIR ? 2 : 1) * (1 + kEpiWarps)); init(&tile_done[q], kEpiWarps); init(&tile_free[q], 1); }
     for (int w = 0; w < kEpiWarps; ++w) init(&res_bars[w], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
+  if (warp == 1) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_slot, kTmemCols);
+      tmem_relinquish();
+    }
+  }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();          // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();
 
   // Waits and their outcome are a warp's, not a lane's: all lanes leave a loop together.
   auto give_up = [&] { if (lane == 0) { atomicExch(p.status, kStatusStageTimeout); *abort_flag = 1; } };
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, PAIR ? wait_cluster(bar, parity) : mbar_wait_bounded(bar, parity)) != 0;
+  };
+  // Arrival of one lane at the leader's copy of a barrier.
+  auto arrive_leader = [&](uint64_t* bar) {
+    if (PAIR && rank != 0) arrive_cluster(at_rank(bar, 0));
+    else mbar_arrive(bar);
+  };
   auto aborted = [&] { return __any_sync(0xffffffffu, *abort_flag) != 0; };
   // operand orientation of a task: the tile's rows are the reduction's (MN-major)?
   auto a_mn = [&](int kind) { return kind == kGram && p.tall; };
@@ -261,57 +329,78 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
     uint32_t phase = 0, qphase = 0;
     pdl_wait();
     unsigned next = 0;                 // lane 0: the next ticket, asked for when the current task's last loads go out
-    if (lane == 0) next = atomicAdd(p.ticket, 1u);
+    if (rank == 0 && lane == 0) next = atomicAdd(p.ticket, 1u);
     while (!aborted()) {
-      const unsigned t = __shfl_sync(0xffffffffu, next, 0);
       Task q{-1, 3, 0, 0, 0};          // step * 4 + kind == -1: the end
-      if (t < p.total) {
-        q = task_of<BN>(t, p);
-        const unsigned want = needs(q, p);
-        bool ready = want == 0;
-        for (int spins = 0; !ready && spins < (1 << 25); ++spins) ready = load_acquire(p.done + q.bi) >= want;
-        if (!__all_sync(0xffffffffu, ready)) { give_up(); break; }
-        fence_async();                 // for this warp's loads and, by way of the queue, the epilogue's
-      }
-      if (!wait(&task_empty[slot], qphase ^ 1)) { give_up(); break; }
-      if (lane == 0) {
-        queue[slot] = make_int4(q.step * 4 + q.kind, q.bi, q.mt, q.nt);
-        mbar_arrive(&task_full[slot]);
+      if (rank == 0) {
+        const unsigned t = __shfl_sync(0xffffffffu, next, 0);
+        if (t < p.total) {
+          q = task_of<BN, TM>(t, p);
+          const unsigned want = needs(q, p) * (PAIR ? 2 : 1);     // each CTA of a pair counts a tile
+          bool ready = want == 0;
+          for (int spins = 0; !ready && spins < (1 << 25); ++spins) ready = load_acquire(p.done + q.bi) >= want;
+          if (!__all_sync(0xffffffffu, ready)) { give_up(); break; }
+          fence_async();               // for this warp's loads and, by way of the queue, the epilogue's
+        }
+        if (!wait(&task_empty[slot], qphase ^ 1)) { give_up(); break; }
+        if (lane == 0) {
+          const int4 code = make_int4(q.step * 4 + q.kind, q.bi, q.mt, q.nt);
+          queue[slot] = code;
+          if (PAIR) {
+            asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(at_rank(&queue[slot], 1)), "r"(code.x), "r"(code.y), "r"(code.z), "r"(code.w) : "memory");
+            arrive_cluster(at_rank(&task_full[slot], 1));
+          }
+          mbar_arrive(&task_full[slot]);
+        }
+      } else {
+        if (!wait(&task_full[slot], qphase)) { give_up(); break; }
+        const int4 code = queue[slot];
+        __syncwarp();
+        if (lane == 0) arrive_leader(&task_empty[slot]);
+        if (code.x >= 0) q = Task{code.x >> 2, code.x & 3, code.y, code.z, code.w};
+        fence_async();
       }
       if (++slot == kQueue) { slot = 0; qphase ^= 1; }
-      if (t >= p.total) break;
+      if (q.step < 0) break;
       const bool ta = a_mn(q.kind), tb = b_mn(q.kind);
       const CUtensorMap* mx = &maps.x[q.step & 1];
       const CUtensorMap* ma = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? mx : &maps.b);
       const CUtensorMap* mb = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? &maps.b : mx);
       const int kb_n = k_blocks(q.kind);
+      const int row = q.mt * TM + (int)rank * kBM, col = q.nt * BN + (int)rank * (BN / 2);
       __syncwarp();
       for (int kb = 0; kb < kb_n; ++kb) {
-        if (kb == kb_n - 1 && lane == 0) next = atomicAdd(p.ticket, 1u);
+        if (rank == 0 && kb == kb_n - 1 && lane == 0) next = atomicAdd(p.ticket, 1u);
         if (!wait(&empty[stage], phase ^ 1)) { give_up(); break; }
         if (elect_one()) {
-          mbar_expect_tx(&full[stage], kSlot);
           unsigned char* da = ring + stage * kSlot;
           unsigned char* db = da + 2 * kBox;
+          if (rank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * kSlot);
+          const uint32_t pair_bar = PAIR ? at_rank(&full[stage], 0) : 0;
+          auto load = [&](void* dst, const CUtensorMap* map, bool mn_major, int mn) {
+            const int c0 = mn_major ? mn : kb * kBK, c1 = mn_major ? kb * kBK : mn;
+            if (PAIR) tma_load_3d_pair(dst, map, c0, c1, q.bi, pair_bar);
+            else tma_load_3d(dst, map, c0, c1, q.bi, &full[stage]);
+          };
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int mn = q.mt * kBM + i * 64;
-            tma_load_3d(da + i * kBox, ma, ta ? mn : kb * kBK, ta ? kb * kBK : mn, q.bi, &full[stage]);
-          }
+          for (int i = 0; i < 2; ++i) load(da + i * kBox, ma, ta, row + i * 64);
 #pragma unroll
-          for (int i = 0; i < BN / 64; ++i) {
-            const int mn = q.nt * BN + i * 64;
-            tma_load_3d(db + i * kBox, mb, tb ? mn : kb * kBK, tb ? kb * kBK : mn, q.bi, &full[stage]);
-          }
+          for (int i = 0; i < kBoxesB; ++i) load(db + i * kBox, mb, tb, col + i * 64);
         }
         __syncwarp();
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
+    if (PAIR && !aborted())            // the leader's last arrivals at this CTA's barriers have come in
+      for (int s = 0; s < kStages; ++s) {
+        if (!wait(&empty[stage], phase ^ 1)) { give_up(); break; }
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
   } else if (warp == 1) {
     int stage = 0, acc = 0, slot = 0;
     uint32_t phase = 0, acc_phase = 0, qphase = 0;
-    while (!aborted()) {
+    while (rank == 0 && !aborted()) {
       if (!wait(&task_full[slot], qphase)) { give_up(); break; }
       const int code = queue[slot].x, kind = code & 3;
       __syncwarp();
@@ -319,7 +408,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       if (++slot == kQueue) { slot = 0; qphase ^= 1; }
       if (code < 0) break;
       const bool ta = a_mn(kind), tb = b_mn(kind);
-      const uint32_t idesc = instr_desc<__half>(BN) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
+      const uint32_t idesc = instr_desc<__half>(BN, TM) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
       const uint64_t step_a = ta ? 128 : 2, step_b = tb ? 128 : 2;  // 16 of K: 16 rows of an MN-major box, 32 bytes of a K-major row
       const int kb_n = k_blocks(kind);
       if (!wait(&acc_empty[acc], acc_phase ^ 1)) { give_up(); break; }
@@ -333,9 +422,17 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
           const uint64_t a0 = ta ? smem_desc_mn(da) : smem_desc_sw128(da);
           const uint64_t b0 = tb ? smem_desc_mn(da + 2 * kBox) : smem_desc_sw128(da + 2 * kBox);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) tc_mma_f16(d_tmem, a0 + k * step_a, b0 + k * step_b, idesc, (kb | k) != 0);
-          tc_commit(&empty[stage]);
-          if (kb == kb_n - 1) tc_commit(&acc_full[acc]);
+          for (int k = 0; k < kBK / 16; ++k) {
+            if (PAIR) mma_f16_pair(d_tmem, a0 + k * step_a, b0 + k * step_b, idesc, (kb | k) != 0);
+            else tc_mma_f16(d_tmem, a0 + k * step_a, b0 + k * step_b, idesc, (kb | k) != 0);
+          }
+          if (PAIR) {
+            commit_pair(&empty[stage]);
+            if (kb == kb_n - 1) commit_pair(&acc_full[acc]);
+          } else {
+            tc_commit(&empty[stage]);
+            if (kb == kb_n - 1) tc_commit(&acc_full[acc]);
+          }
         }
         __syncwarp();
         if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -395,7 +492,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       if (!wait(&task_full[slot], qphase)) { give_up(); break; }
       const int4 code = queue[slot];
       __syncwarp();
-      if (lane == 0) mbar_arrive(&task_empty[slot]);
+      if (lane == 0) arrive_leader(&task_empty[slot]);
       if (++slot == kQueue) { slot = 0; qphase ^= 1; }
       if (code.x < 0) break;
       const Task q{code.x >> 2, code.x & 3, code.y, code.z, code.w};
@@ -411,7 +508,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       const CUtensorMap* o0 = kind == kGram ? &maps.as : kind == kPoly ? &maps.bs : (last ? &maps.out : &maps.xs[(q.step & 1) ^ 1]);
       const CUtensorMap* o1 = &maps.ls[(q.step & 1) ^ 1];
       const int rows = kind == kUpdate ? p.m : p.p, cols = kind == kUpdate ? p.n : p.p;
-      const int row0 = q.mt * kBM + quad * 32, colw = q.nt * BN + group * kCols;
+      const int row0 = q.mt * TM + (int)rank * kBM + quad * 32, colw = q.nt * BN + group * kCols;
       const bool rows_in = row0 < rows;                  // else this warp's quarter lies below the matrix
       // make the staging buffer free and ask for the unit of the previous X or A that unit `u` needs
       auto fetch = [&](int u) {
@@ -423,7 +520,10 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       };
       int units = rows_in ? (cols - colw + 31) / 32 : 0;   // units with any column of the matrix
       units = units < 0 ? 0 : (units > kUnits ? kUnits : units);
-      if (units > 0 && elect_one()) fetch(0);
+      if (units > 0 && elect_one()) {
+        if (PAIR && has_res) fence_async();              // the leader's does not cover this CTA's loads
+        fetch(0);
+      }
       __syncwarp();
       if (!wait(&acc_full[acc], acc_phase)) { give_up(); break; }
       tc_fence_after();
@@ -443,7 +543,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
         }
         tmem_ld_wait();
         // a unit below the diagonal whose mirror image no tile computes is stored there as well
-        const bool mirror = kind != kUpdate && row0 > col0 && row0 / BN >= sym_cols<BN>(col0 / kBM, p.p);
+        const bool mirror = kind != kUpdate && row0 > col0 && row0 / BN >= sym_cols<BN, TM>(col0 / TM, p.p);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           // 64-byte swizzle: 16-byte piece index xor bits 1-2 of the row
@@ -516,7 +616,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       tc_fence_before();
       __syncwarp();
       if (elect_one()) {
-        mbar_arrive(&acc_empty[acc]);
+        arrive_leader(&acc_empty[acc]);
         for (int u = units; u < kUnits; ++u) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         asm volatile("cp.async.bulk.wait_group %0;" ::"n"(kUnits) : "memory");   // all but this tile's
       }
@@ -539,10 +639,12 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
   // 20 ms to land before the memory is handed back.
   if (*abort_flag)
     for (int i = 0; i < 20000; ++i) __nanosleep(1000);
+  if (PAIR) cluster_sync();          // nobody reaches into a CTA that has left
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, kTmemCols);
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+    else tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
@@ -897,36 +999,54 @@ Layout layout_of(long long batch, int m, int n) {
   return w;
 }
 
-#ifndef DCNB200_NS_BN
-#define DCNB200_NS_BN 0
-#endif
+// Tiles of TM x BN that a step takes for one matrix; sets the counts of its products.
+template <int BN, int TM>
+int tiles(NsParams& p) {
+  p.sym_tiles = 0;
+  for (int i = 0; i < (p.p + TM - 1) / TM; ++i) p.sym_tiles += sym_cols<BN, TM>(i, p.p);
+  p.upd_n = (p.n + BN - 1) / BN;
+  p.upd_tiles = (p.m + TM - 1) / TM * p.upd_n;
+  return 2 * p.sym_tiles + p.upd_tiles;
+}
 
-template <int BN>
+template <int BN, bool PAIR>
 cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
+  constexpr int TM = tile_m<PAIR>();
   int dev = 0;
   cudaGetDevice(&dev);
   dev = dev < 0 || dev >= 64 ? 0 : dev;
   std::call_once(once[dev], [&] {
-    attr_err[dev] = cudaFuncSetAttribute(ns_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ns_smem<BN>());
+    attr_err[dev] = cudaFuncSetAttribute(ns_kernel<BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ns_smem<BN, PAIR>());
   });
   if (attr_err[dev] != cudaSuccess) return attr_err[dev];
-  p.sym_tiles = 0;
-  for (int i = 0; i < (p.p + kBM - 1) / kBM; ++i) p.sym_tiles += sym_cols<BN>(i, p.p);
-  p.upd_n = (p.n + BN - 1) / BN;
-  p.upd_tiles = (p.m + kBM - 1) / kBM * p.upd_n;
-  const long long total = (long long)p.batch * p.steps * (2LL * p.sym_tiles + p.upd_tiles);
+  const int per_matrix = tiles<BN, TM>(p);
+  const long long total = (long long)p.batch * p.steps * per_matrix;
   if (total >= (1LL << 31)) return cudaErrorInvalidValue;
   p.total = (unsigned)total;
-  // the matrices whose A fits one wave of CTAs, in two halves; the rest are the third group
-  const int wave = sms / p.sym_tiles < p.batch ? sms / p.sym_tiles : p.batch;
+  const int workers = PAIR ? sms / 2 : sms;
+  // the matrices whose A fits one wave, in two halves; the rest are the third group
+  const int wave = workers / p.sym_tiles < p.batch ? workers / p.sym_tiles : p.batch;
   p.group1 = (wave + 1) / 2;
   p.group2 = wave - p.group1;
-  // more CTAs than a product has tiles would only wait
+  // more workers than a product has tiles would only wait
   const long long most = (long long)p.batch * (p.sym_tiles > p.upd_tiles ? p.sym_tiles : p.upd_tiles);
-  const unsigned grid = (unsigned)(most < sms ? most : sms);
-  return launch_overlapped(ns_kernel<BN>, dim3(grid), dim3(ns_threads<BN>()), ns_smem<BN>(), s, maps, p);
+  const unsigned grid = (unsigned)(most < workers ? most : workers) * (PAIR ? 2 : 1);
+  if (!PAIR) return launch_overlapped(ns_kernel<BN, PAIR>, dim3(grid), dim3(ns_threads<BN>()), ns_smem<BN, PAIR>(), s, maps, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(ns_threads<BN>());
+  cfg.dynamicSmemBytes = ns_smem<BN, PAIR>();
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, ns_kernel<BN, PAIR>, maps, p);
 }
 
 template <typename T>
@@ -1024,11 +1144,14 @@ cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* work
   ok = ok && (direct ? map3(&maps.out, true, out, batch, m, n, n, 32, 32)
                      : map3(&maps.out, true, ws + w.x[steps & 1], batch, m, n, w.ldn, 32, 32));
   if (!ok) return cudaErrorNotSupported;
-  // Tile width: the widest whose update still gives every SM a tile.
+  // Tile width: the widest whose update still gives every SM a tile.  The widest also goes to pairs of CTAs, whose
+  // 256 x 256 tiles fetch a third less of the operands, unless padding rows to 256 takes that back: with the same number
+  // of tiles (5 x 5120x1280) pairs take 0.91 of the time (836 -> 763 us), with 1.24 times as many (22 x 640x2560) 1.03.
   const long long rows = (m + kBM - 1) / kBM;
-  const int width = DCNB200_NS_BN ? DCNB200_NS_BN
-                    : batch * rows * ((n + 255) / 256) >= sms ? 256 : batch * rows * ((n + 127) / 128) >= sms ? 128 : 64;
-  e = width == 256 ? launch_ns<256>(maps, p, sms, s) : width == 128 ? launch_ns<128>(maps, p, sms, s) : launch_ns<64>(maps, p, sms, s);
+  if (batch * rows * ((n + 255) / 256) >= sms)
+    e = 16 * tiles<256, 256>(p) <= 9 * tiles<256, 128>(p) ? launch_ns<256, true>(maps, p, sms, s) : launch_ns<256, false>(maps, p, sms, s);
+  else
+    e = batch * rows * ((n + 127) / 128) >= sms ? launch_ns<128, false>(maps, p, sms, s) : launch_ns<64, false>(maps, p, sms, s);
   if (e == cudaSuccess && !direct) {
     const long long total = batch * (long long)m * n;
     long long blocks = (total + kNormThreads - 1) / kNormThreads;

@@ -103,6 +103,29 @@ def test_odd_sizes(m, n):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("batch,m,n", [(40, 300, 260), (80, 130, 257), (150, 255, 333), (150, 333, 255), (40, 512, 264), (75, 257, 513),
+                                       (12, 1000, 770), (9, 770, 1100)])
+def test_stacks_that_fill_the_gpu(batch, m, n):
+    """Wide tiles, by one CTA and by pairs of them, with ragged rows and columns; both streams at once and captured."""
+    from dcnv4_b200 import ops
+    x = momentum(batch, m, n, torch.bfloat16)
+    want = ops.newton_schulz(x)
+    check(want, ref(x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [ops.newton_schulz(x) for _ in range(2)]
+    mine = [ops.newton_schulz(x) for _ in range(2)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for t in other + mine)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.newton_schulz(x)
+    graph.replay()
+    assert torch.equal(y, want)
+    assert ops.device_status() == 0
+
+
 def test_spectra():
     """Flat, decaying and nearly rank-deficient spectra: the pair (hi, lo) keeps the small directions."""
     from dcnv4_b200 import ops
