@@ -895,17 +895,15 @@ template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
 ns_scale_kernel(const T* __restrict__ x, const double* __restrict__ partial, __half* __restrict__ hi,
                 __half* __restrict__ lo, int rows, int cols, int ld, int n_chunks, float eps, int vec) {
-  __shared__ float inv_s;
   pdl_trigger();
   pdl_wait();
   const int bi = blockIdx.y;
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int i = 0; i < n_chunks; ++i) t += partial[(long long)bi * kMaxChunks + i];
-    inv_s = (float)(1.0 / (sqrt(t) + (double)eps));
-  }
-  __syncthreads();
-  const float inv = inv_s;
+  // every warp adds the partial sums for itself: one thread's chain of loads would hold up the block
+  double t = 0.0;
+  for (int i = threadIdx.x & 31; i < n_chunks; i += 32) t += partial[(long long)bi * kMaxChunks + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const float inv = (float)(1.0 / (sqrt(t) + (double)eps));
   const T* src = x + (long long)bi * rows * cols;
   __half* dh = hi + (long long)bi * rows * ld;
   __half* dl = lo + (long long)bi * rows * ld;
