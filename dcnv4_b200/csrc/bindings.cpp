@@ -50,6 +50,12 @@ inline bool plain(const at::Tensor& t, at::Device dev, at::ScalarType type) {
 }
 inline void* data(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
+// The interpreter goes on while results are allocated and kernels launched (a kernel's first launch loads it).
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // What both passes check; fills rows, channels and rows per sample.
 bool accept(const at::Tensor& x, at::ScalarType x_type, at::ScalarType out_type, const at::Tensor& w, const at::Tensor& b,
             const at::Tensor* gamma, const at::Tensor* s, int64_t& rows, int64_t& C, int64_t& per) {
@@ -99,14 +105,20 @@ PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t rows, C, per;
   if (!accept(*x, x->scalar_type(), out, *w, *b, gamma, s, rows, C, per)) Py_RETURN_NONE;
   if (res && (!plain(*res, x->device(), out) || res->sizes() != x->sizes())) Py_RETURN_NONE;
-  const auto opts = x->options().requires_grad(false);
-  at::Tensor y = at::empty(x->sizes(), opts.dtype(out)), h, mean = at::empty({rows}, opts.dtype(at::kFloat));
-  at::Tensor rstd = at::empty({rows}, opts.dtype(at::kFloat));
-  if (mode == kPre) h = at::empty(x->sizes(), opts.dtype(out));
-  const int rc = g_fwd(x->data_ptr(), data(res), w->data_ptr(), b->data_ptr(), data(gamma), static_cast<const float*>(data(s)),
-                       y.data_ptr(), mode == kPre ? h.data_ptr() : nullptr, mean.data_ptr<float>(), rstd.data_ptr<float>(),
-                       mode, code_of(x->scalar_type()), out_code, code_of(w->scalar_type()), rows, (int)C, per, (float)eps,
-                       act, c10::cuda::getCurrentCUDAStream(x->device().index()).stream());
+  at::Tensor y, h, mean, rstd;
+  int rc;
+  {
+    Unlocked unlocked;
+    const auto opts = x->options().requires_grad(false);
+    y = at::empty(x->sizes(), opts.dtype(out));
+    mean = at::empty({rows}, opts.dtype(at::kFloat));
+    rstd = at::empty({rows}, opts.dtype(at::kFloat));
+    if (mode == kPre) h = at::empty(x->sizes(), opts.dtype(out));
+    rc = g_fwd(x->data_ptr(), data(res), w->data_ptr(), b->data_ptr(), data(gamma), static_cast<const float*>(data(s)),
+               y.data_ptr(), mode == kPre ? h.data_ptr() : nullptr, mean.data_ptr<float>(), rstd.data_ptr<float>(), mode,
+               code_of(x->scalar_type()), out_code, code_of(w->scalar_type()), rows, (int)C, per, (float)eps, act,
+               c10::cuda::getCurrentCUDAStream(x->device().index()).stream());
+  }
   if (rc) return PyLong_FromLong(rc);
   const int extra = mode == kPre;
   PyObject* tuple = PyTuple_New(3 + extra);
@@ -141,20 +153,26 @@ PyObject* py_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       (gh && (!plain(*gh, dev, out) || gh->sizes() != x->sizes())) || !plain(*mean, dev, at::kFloat) ||
       mean->numel() != rows || !plain(*rstd, dev, at::kFloat) || rstd->numel() != rows)
     Py_RETURN_NONE;
-  const auto opts = x->options().requires_grad(false);
-  const auto param = opts.dtype(w->scalar_type());
-  at::Tensor gx = at::empty(x->sizes(), opts), branch, gs;
-  if (pre && (s || branch_type != out)) branch = at::empty(x->sizes(), opts.dtype(branch_type));
-  at::Tensor gw = at::empty(w->sizes(), param), gb = at::empty(b->sizes(), param);
-  if (gamma) gs = at::empty(gamma->sizes(), param);
-  const size_t bytes = g_workspace(code, rows, (int)C);
-  at::Tensor ws = at::empty({(int64_t)bytes}, opts.dtype(at::kByte));
-  const int rc = g_bwd(gy->data_ptr(), pre ? data(gh) : nullptr, x->data_ptr(), mean->data_ptr<float>(), rstd->data_ptr<float>(),
-                       w->data_ptr(), b->data_ptr(), data(gamma), static_cast<const float*>(data(s)), gx.data_ptr(),
-                       branch.defined() ? branch.data_ptr() : nullptr, gw.data_ptr(), gb.data_ptr(),
-                       gs.defined() ? gs.data_ptr() : nullptr, ws.data_ptr(), bytes, mode, code, code_of(out),
-                       code_of(w->scalar_type()), rows, (int)C, per, act,
-                       c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  at::Tensor gx, branch, gw, gb, gs;
+  int rc;
+  {
+    Unlocked unlocked;
+    const auto opts = x->options().requires_grad(false);
+    const auto param = opts.dtype(w->scalar_type());
+    gx = at::empty(x->sizes(), opts);
+    if (pre && (s || branch_type != out)) branch = at::empty(x->sizes(), opts.dtype(branch_type));
+    gw = at::empty(w->sizes(), param);
+    gb = at::empty(b->sizes(), param);
+    if (gamma) gs = at::empty(gamma->sizes(), param);
+    const size_t bytes = g_workspace(code, rows, (int)C);
+    at::Tensor ws = at::empty({(int64_t)bytes}, opts.dtype(at::kByte));
+    rc = g_bwd(gy->data_ptr(), pre ? data(gh) : nullptr, x->data_ptr(), mean->data_ptr<float>(), rstd->data_ptr<float>(),
+               w->data_ptr(), b->data_ptr(), data(gamma), static_cast<const float*>(data(s)), gx.data_ptr(),
+               branch.defined() ? branch.data_ptr() : nullptr, gw.data_ptr(), gb.data_ptr(),
+               gs.defined() ? gs.data_ptr() : nullptr, ws.data_ptr(), bytes, mode, code, code_of(out),
+               code_of(w->scalar_type()), rows, (int)C, per, act,
+               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  }
   if (rc) return PyLong_FromLong(rc);
   PyObject* tuple = PyTuple_New(5);
   if (!tuple) return nullptr;

@@ -194,7 +194,8 @@ int dcnv4b200_layernorm_act_fwd(const void* x, const void* gamma, const void* be
  *   mean, rstd   (rows) fp32: the row statistics, kept for the backward pass
  * `out_dtype` is `dtype` or fp32 (16-bit branches beside an fp32 residual stream, as autocast has them),
  * `param_dtype` is fp32 or `dtype`.  `activation` may be DCNV4B200_ACT_GELU (erf form) with PLAIN only.
- * 1 <= C <= 8192, any alignment of rows: tensors and C that fill 16-byte vectors take the wide loads.
+ * 1 <= C <= 8192, rows < 2^31, any alignment of rows: tensors and C that fill 16-byte vectors take the wide loads.
+ * What a call writes overlaps nothing that it reads.
  */
 int dcnv4b200_layernorm_train_fwd(const void* x, const void* residual, const void* weight, const void* bias,
                                   const void* layer_scale, const float* sample_scale, void* y, void* h, float* mean,
@@ -212,7 +213,8 @@ size_t dcnv4b200_layernorm_train_bwd_workspace_bytes(int dtype, long long rows, 
  *   grad_branch  PRE: gradient of the forward's x, in `dtype`, or NULL where it equals grad_x (sample_scale NULL and
  *                dtype == out_dtype); NULL otherwise
  *   grad_weight, grad_bias, grad_layer_scale (C) in `param_dtype`; the last one with layer_scale only
- *   workspace    16-byte aligned, at least dcnv4b200_layernorm_train_bwd_workspace_bytes() bytes
+ *   workspace    16-byte aligned, at least dcnv4b200_layernorm_train_bwd_workspace_bytes() bytes, private to calls that
+ *                may overlap on the GPU
  * The gradient of POST's residual is grad_y itself.  Everything is fully overwritten; no atomics, results repeat
  * bit for bit.  With rows == 0 the parameter gradients are zero.
  */

@@ -355,6 +355,36 @@ def test_another_stream_and_a_captured_graph():
         assert all(torch.equal(static[k], want[k]) for k in want)
 
 
+def test_captured_backward_pass():
+    """Forward and backward of the three functions as one captured graph, replayed after its inputs changed."""
+    from dcnv4_b200 import AddLayerNormFunction, LayerNormFunction, LayerNormResidualFunction
+    g = torch.Generator(device=DEV).manual_seed(3)
+    leaves = [torch.randn(shape, device=DEV, generator=g, requires_grad=True)
+              for shape in ((4, 50, 192), (4, 50, 192), (192,), (192,))]
+
+    def grads():
+        x, r, w, b = leaves
+        h, y = AddLayerNormFunction.apply(x, r, w, b, 1e-6)
+        z = LayerNormFunction.apply(y, w, b, 1e-6, "gelu")
+        loss = LayerNormResidualFunction.apply(z, h, w, b, 1e-6, w).square().mean()
+        return torch.autograd.grad(loss, leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = grads()
+    with torch.no_grad():
+        for t in leaves:
+            t.mul_(1.5)
+    graph.replay()
+    for a, b in zip(static, grads()):
+        assert torch.equal(a, b)
+
+
 def test_directional_differences():
     """The gradients against central differences of the kernel's own forward pass, in fp32.  Allowed: the forward's
     rounding over the step, and the truncation that the 64-bit formula shows for the same step."""
