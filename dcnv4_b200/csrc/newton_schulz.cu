@@ -31,7 +31,10 @@
 // Large stacks give the tiles to pairs of CTAs (cta_group::2): a CTA loads its 128 rows of A and half of B's columns, so
 // that the operands cost 2/3 of the L2 traffic and of the shared memory's bandwidth, which is what a 128 x 256 tile is
 // short of (its 48 KB per 64 of K are written once and read once in the 512 cycles of the products).  The leader takes
-// the tasks, hands them to both queues and issues the products; each CTA has its own epilogue and counts its half.
+// the tasks, hands them to both queues and issues the products; each CTA has its own epilogue and counts its half.  A last
+// row block of at most 128 rows is a 128 x BN product (M 128, 64 rows in each CTA), so that no rows are padded to 256.
+// What bounds both forms is operand bytes in flight: with three slots of the ring instead of five, pairs took 1.15 times
+// as long; the rest of shared memory is the epilogue's staging, which must cover the same latency.
 // Every mbarrier wait is bounded; one that runs out sets the device status word and the CTA winds down.
 //
 // Matrices with p <= 128 and q <= 256 take another kernel: one CTA holds a whole matrix (X and A, B as fp16 operands in shared
@@ -322,6 +325,8 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
   // operand orientation of a task: the tile's rows are the reduction's (MN-major)?
   auto a_mn = [&](int kind) { return kind == kGram && p.tall; };
   auto b_mn = [&](int kind) { return kind == kGram ? p.tall != 0 : kind == kUpdate && !p.tall; };
+  // a pair's last row block with no more than 128 rows: 64 of them in each CTA
+  auto is_half = [&](int kind, int mt) { return PAIR && (kind == kUpdate ? p.m : p.p) - mt * TM <= TM / 2; };
   auto k_blocks = [&](int kind) { return ((kind == kGram ? p.q : p.p) + kBK - 1) / kBK; };
 
   if (warp == 0) {
@@ -368,7 +373,8 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       const CUtensorMap* ma = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? mx : &maps.b);
       const CUtensorMap* mb = q.kind == kGram ? mx : q.kind == kPoly ? &maps.a : (p.tall ? &maps.b : mx);
       const int kb_n = k_blocks(q.kind);
-      const int row = q.mt * TM + (int)rank * kBM, col = q.nt * BN + (int)rank * (BN / 2);
+      const bool half = is_half(q.kind, q.mt);
+      const int row = q.mt * TM + (int)rank * (half ? kBM / 2 : kBM), col = q.nt * BN + (int)rank * (BN / 2);
       __syncwarp();
       for (int kb = 0; kb < kb_n; ++kb) {
         if (rank == 0 && kb == kb_n - 1 && lane == 0) next = atomicAdd(p.ticket, 1u);
@@ -376,15 +382,15 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
         if (elect_one()) {
           unsigned char* da = ring + stage * kSlot;
           unsigned char* db = da + 2 * kBox;
-          if (rank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * kSlot);
+          if (rank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * (half ? kSlot - kBox : kSlot));
           const uint32_t pair_bar = PAIR ? at_rank(&full[stage], 0) : 0;
           auto load = [&](void* dst, const CUtensorMap* map, bool mn_major, int mn) {
             const int c0 = mn_major ? mn : kb * kBK, c1 = mn_major ? kb * kBK : mn;
             if (PAIR) tma_load_3d_pair(dst, map, c0, c1, q.bi, pair_bar);
             else tma_load_3d(dst, map, c0, c1, q.bi, &full[stage]);
           };
-#pragma unroll
-          for (int i = 0; i < 2; ++i) load(da + i * kBox, ma, ta, row + i * 64);
+          load(da, ma, ta, row);
+          if (!half) load(da + kBox, ma, ta, row + 64);
 #pragma unroll
           for (int i = 0; i < kBoxesB; ++i) load(db + i * kBox, mb, tb, col + i * 64);
         }
@@ -402,13 +408,14 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
     uint32_t phase = 0, acc_phase = 0, qphase = 0;
     while (rank == 0 && !aborted()) {
       if (!wait(&task_full[slot], qphase)) { give_up(); break; }
-      const int code = queue[slot].x, kind = code & 3;
+      const int4 task = queue[slot];
+      const int code = task.x, kind = code & 3;
       __syncwarp();
       if (lane == 0) mbar_arrive(&task_empty[slot]);
       if (++slot == kQueue) { slot = 0; qphase ^= 1; }
       if (code < 0) break;
       const bool ta = a_mn(kind), tb = b_mn(kind);
-      const uint32_t idesc = instr_desc<__half>(BN, TM) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
+      const uint32_t idesc = instr_desc<__half>(BN, is_half(kind, task.z) ? TM / 2 : TM) | ((uint32_t)ta << 15) | ((uint32_t)tb << 16);
       const uint64_t step_a = ta ? 128 : 2, step_b = tb ? 128 : 2;  // 16 of K: 16 rows of an MN-major box, 32 bytes of a K-major row
       const int kb_n = k_blocks(kind);
       if (!wait(&acc_empty[acc], acc_phase ^ 1)) { give_up(); break; }
@@ -508,7 +515,11 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       const CUtensorMap* o0 = kind == kGram ? &maps.as : kind == kPoly ? &maps.bs : (last ? &maps.out : &maps.xs[(q.step & 1) ^ 1]);
       const CUtensorMap* o1 = &maps.ls[(q.step & 1) ^ 1];
       const int rows = kind == kUpdate ? p.m : p.p, cols = kind == kUpdate ? p.n : p.p;
-      const int row0 = q.mt * TM + (int)rank * kBM + quad * 32, colw = q.nt * BN + group * kCols;
+      // A half block's 64 rows of a CTA lie in the upper lanes for the tile's left columns, in the lower for its right.
+      const bool half = is_half(kind, q.mt);
+      const int row0 = q.mt * TM + (half ? (int)rank * 64 + (quad & 1) * 32 : (int)rank * kBM + quad * 32);
+      const int first = group * (half ? kCols / 2 : kCols);
+      const int colw = q.nt * BN + first + (half ? (quad >> 1) * (BN / 2) : 0);
       const bool rows_in = row0 < rows;                  // else this warp's quarter lies below the matrix
       // make the staging buffer free and ask for the unit of the previous X or A that unit `u` needs
       auto fetch = [&](int u) {
@@ -519,7 +530,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
         if (res) tma_load_3d(set + kUnit, r1, colw + u * 32, row0, q.bi, res_bar);
       };
       int units = rows_in ? (cols - colw + 31) / 32 : 0;   // units with any column of the matrix
-      units = units < 0 ? 0 : (units > kUnits ? kUnits : units);
+      units = units < 0 ? 0 : min(units, half ? kUnits / 2 : kUnits);
       if (units > 0 && elect_one()) {
         if (PAIR && has_res) fence_async();              // the leader's does not cover this CTA's loads
         fetch(0);
@@ -527,7 +538,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       __syncwarp();
       if (!wait(&acc_full[acc], acc_phase)) { give_up(); break; }
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + group * kCols);
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + first);
 #pragma unroll 1
       for (int u = 0; u < units; ++u) {
         const int col0 = colw + u * 32;
@@ -997,16 +1008,6 @@ Layout layout_of(long long batch, int m, int n) {
   return w;
 }
 
-// Tiles of TM x BN that a step takes for one matrix; sets the counts of its products.
-template <int BN, int TM>
-int tiles(NsParams& p) {
-  p.sym_tiles = 0;
-  for (int i = 0; i < (p.p + TM - 1) / TM; ++i) p.sym_tiles += sym_cols<BN, TM>(i, p.p);
-  p.upd_n = (p.n + BN - 1) / BN;
-  p.upd_tiles = (p.m + TM - 1) / TM * p.upd_n;
-  return 2 * p.sym_tiles + p.upd_tiles;
-}
-
 template <int BN, bool PAIR>
 cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
   static std::once_flag once[64];
@@ -1019,8 +1020,11 @@ cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
     attr_err[dev] = cudaFuncSetAttribute(ns_kernel<BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ns_smem<BN, PAIR>());
   });
   if (attr_err[dev] != cudaSuccess) return attr_err[dev];
-  const int per_matrix = tiles<BN, TM>(p);
-  const long long total = (long long)p.batch * p.steps * per_matrix;
+  p.sym_tiles = 0;
+  for (int i = 0; i < (p.p + TM - 1) / TM; ++i) p.sym_tiles += sym_cols<BN, TM>(i, p.p);
+  p.upd_n = (p.n + BN - 1) / BN;
+  p.upd_tiles = (p.m + TM - 1) / TM * p.upd_n;
+  const long long total = (long long)p.batch * p.steps * (2LL * p.sym_tiles + p.upd_tiles);
   if (total >= (1LL << 31)) return cudaErrorInvalidValue;
   p.total = (unsigned)total;
   const int workers = PAIR ? sms / 2 : sms;
@@ -1142,12 +1146,13 @@ cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* work
   ok = ok && (direct ? map3(&maps.out, true, out, batch, m, n, n, 32, 32)
                      : map3(&maps.out, true, ws + w.x[steps & 1], batch, m, n, w.ldn, 32, 32));
   if (!ok) return cudaErrorNotSupported;
-  // Tile width: the widest whose update still gives every SM a tile.  The widest also goes to pairs of CTAs, whose
-  // 256 x 256 tiles fetch a third less of the operands, unless padding rows to 256 takes that back: with the same number
-  // of tiles (5 x 5120x1280) pairs take 0.91 of the time (836 -> 763 us), with 1.24 times as many (22 x 640x2560) 1.03.
+  // Tile width: the widest whose update still gives every SM a tile.  The widest also goes to pairs of CTAs where products
+  // are long enough to gain from their smaller traffic (pairs over single CTAs: 1 x 4000x6000 0.81, 3 x 896x7000 0.76,
+  // 5 x 5120x1280 0.91); in short ones the hand-over between two CTAs costs as much (30 x 768x768 1.05, 22 x 640x2560 1.01,
+  // 18 x 512x2048 1.00, 40 x 320x1280 1.12).
   const long long rows = (m + kBM - 1) / kBM;
   if (batch * rows * ((n + 255) / 256) >= sms)
-    e = 16 * tiles<256, 256>(p) <= 9 * tiles<256, 128>(p) ? launch_ns<256, true>(maps, p, sms, s) : launch_ns<256, false>(maps, p, sms, s);
+    e = p.p > 768 ? launch_ns<256, true>(maps, p, sms, s) : launch_ns<256, false>(maps, p, sms, s);
   else
     e = batch * rows * ((n + 127) / 128) >= sms ? launch_ns<128, false>(maps, p, sms, s) : launch_ns<64, false>(maps, p, sms, s);
   if (e == cudaSuccess && !direct) {

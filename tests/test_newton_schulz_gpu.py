@@ -104,7 +104,7 @@ def test_odd_sizes(m, n):
 
 
 @pytest.mark.parametrize("batch,m,n", [(40, 300, 260), (80, 130, 257), (150, 255, 333), (150, 333, 255), (40, 512, 264), (75, 257, 513),
-                                       (12, 1000, 770), (9, 770, 1100)])
+                                       (12, 1000, 770), (9, 770, 1100), (6, 900, 1030), (8, 1031, 897), (9, 1030, 1025)])
 def test_stacks_that_fill_the_gpu(batch, m, n):
     """Wide tiles, by one CTA and by pairs of them, with ragged rows and columns; both streams at once and captured."""
     from dcnv4_b200 import ops
