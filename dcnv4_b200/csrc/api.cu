@@ -438,6 +438,9 @@ int dcnv4b200_layernorm_act_fwd(const void* x, const void* gamma, const void* be
 // Limits of the Newton-Schulz entry point: a side of a matrix, matrices per call (a grid dimension), steps.
 constexpr int kNsMaxSide = 65536, kNsMaxBatch = 65535, kNsMaxSteps = 100;
 
+// Rows of a LayerNorm training pass: the kernels add strides of their grid to row numbers in 32 bits.
+constexpr long long kLnMaxRows = 1LL << 30;
+
 // Checks the two LayerNorm training passes share; fills the arguments they have in common.
 static int fill_ln_train(LnTrainArgs& a, const void* weight, const void* bias, const void* layer_scale,
                          const float* sample_scale, int mode, int dtype, int out_dtype, int param_dtype,
@@ -450,7 +453,7 @@ static int fill_ln_train(LnTrainArgs& a, const void* weight, const void* bias, c
     return DCNV4B200_ERR_DTYPE;
   if (rows < 0 || C <= 0) return DCNV4B200_ERR_SHAPE;
   if (C > ln_train_max_channels()) return DCNV4B200_ERR_UNSUPPORTED;
-  if (rows >= (1LL << 31)) return DCNV4B200_ERR_TOO_LARGE;
+  if (rows > kLnMaxRows) return DCNV4B200_ERR_TOO_LARGE;
   if (sample_scale && (rows_per_sample <= 0 || rows % rows_per_sample != 0)) return DCNV4B200_ERR_SHAPE;
   const uintptr_t pa = (param_dtype == DCNV4B200_F32 ? 4 : 2) - 1;
   if (((uintptr_t)weight | (uintptr_t)bias | (uintptr_t)layer_scale) & pa || (uintptr_t)sample_scale & 3)
@@ -490,7 +493,7 @@ int dcnv4b200_layernorm_train_fwd(const void* x, const void* residual, const voi
 }
 
 size_t dcnv4b200_layernorm_train_bwd_workspace_bytes(int dtype, long long rows, int C) {
-  if (!dtype_ok(dtype) || rows <= 0 || rows >= (1LL << 31) || C <= 0 || C > ln_train_max_channels()) return 0;
+  if (!dtype_ok(dtype) || rows <= 0 || rows > kLnMaxRows || C <= 0 || C > ln_train_max_channels()) return 0;
   return ln_train_workspace_bytes(dtype, (int)rows, C);
 }
 

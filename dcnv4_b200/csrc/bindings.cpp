@@ -31,7 +31,7 @@ BwdFn g_bwd = nullptr;
 WorkspaceFn g_workspace = nullptr;
 
 constexpr int kPlain = 0, kPost = 1, kPre = 2;
-constexpr int64_t kMaxChannels = 8192, kMaxRows = (int64_t)1 << 31;
+constexpr int64_t kMaxChannels = 8192, kMaxRows = (int64_t)1 << 30;
 
 // Type code of the C ABI, or -1.
 inline int code_of(at::ScalarType t) {
@@ -67,7 +67,7 @@ bool accept(const at::Tensor& x, at::ScalarType x_type, at::ScalarType out_type,
   C = x.size(-1);
   rows = x.numel() / C;
   per = rows;
-  if (C > kMaxChannels || rows >= kMaxRows || (out_type != x_type && out_type != at::kFloat) ||
+  if (C > kMaxChannels || rows > kMaxRows || (out_type != x_type && out_type != at::kFloat) ||
       (p != x_type && p != at::kFloat) || !plain(w, dev, p) || w.numel() != C || !plain(b, dev, p) || b.numel() != C)
     return false;
   if (gamma && (!plain(*gamma, dev, p) || gamma->numel() != C)) return false;

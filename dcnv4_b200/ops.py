@@ -251,13 +251,14 @@ def layer_norm_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
 # LayerNorm training passes ---------------------------------------------------------------------------------
 
 LAYER_NORM_MAX_CHANNELS = 8192
+LAYER_NORM_MAX_ROWS = 2 ** 30
 _LN_PLAIN, _LN_POST, _LN_PRE = 0, 1, 2
 
 
 def layer_norm_train_supported(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> bool:
     """True when the LayerNorm training passes cover this input (dtypes, size, layout)."""
     return (x.is_cuda and x.is_contiguous() and x.dtype in _DTYPES and x.dim() > 0
-            and 0 < x.shape[-1] <= LAYER_NORM_MAX_CHANNELS and x.numel() // x.shape[-1] < 2 ** 31
+            and 0 < x.shape[-1] <= LAYER_NORM_MAX_CHANNELS and x.numel() // x.shape[-1] <= LAYER_NORM_MAX_ROWS
             and weight is not None and weight.is_cuda and weight.is_contiguous()
             and weight.dtype in (torch.float32, x.dtype) and out_dtype in (None, torch.float32, x.dtype))
 
@@ -375,8 +376,8 @@ def layer_norm_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.
                              activation: str = "none", out_dtype: Optional[torch.dtype] = None):
     """LayerNorm over the last dimension of a contiguous CUDA tensor for training: (y, mean, rstd), with y optionally
     through the exact GELU in the same pass and the fp32 row statistics that `layer_norm_backward` reads.  `out_dtype`
-    is the dtype of x (default) or float32; weight and bias are float32 or have the dtype of x.  Any number of rows,
-    1 to 8192 channels."""
+    is the dtype of x (default) or float32; weight and bias are float32 or have the dtype of x.  Up to 2^30 rows, 1 to
+    8192 channels."""
     if activation not in ("none", "gelu"):
         raise ValueError("activation must be 'none' or 'gelu'")
     return _ln_forward(_LN_PLAIN, x, None, weight, bias, eps, None, None, activation,

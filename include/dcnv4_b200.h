@@ -194,7 +194,7 @@ int dcnv4b200_layernorm_act_fwd(const void* x, const void* gamma, const void* be
  *   mean, rstd   (rows) fp32: the row statistics, kept for the backward pass
  * `out_dtype` is `dtype` or fp32 (16-bit branches beside an fp32 residual stream, as autocast has them),
  * `param_dtype` is fp32 or `dtype`.  `activation` may be DCNV4B200_ACT_GELU (erf form) with PLAIN only.
- * 1 <= C <= 8192, rows < 2^31, any alignment of rows: tensors and C that fill 16-byte vectors take the wide loads.
+ * 1 <= C <= 8192, rows <= 2^30, any alignment of rows: tensors and C that fill 16-byte vectors take the wide loads.
  * What a call writes overlaps nothing that it reads.
  */
 int dcnv4b200_layernorm_train_fwd(const void* x, const void* residual, const void* weight, const void* bias,

@@ -250,6 +250,33 @@ def test_unaligned_tensors(tx, ty):
         check_pre(d)
 
 
+@pytest.mark.parametrize("C", [8192, 8191])
+def test_offsets_beyond_32_bits(C):
+    """More than 2^32 elements: the last rows against the same rows on their own."""
+    from dcnv4_b200 import ops
+    rows, tail = 2 ** 32 // C + 1500, 700
+    if torch.cuda.mem_get_info()[0] < 50 << 30:
+        pytest.skip("needs 50 GB")
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.zeros(rows, C, device=DEV, dtype=BF16)
+    x[-tail:] = torch.randn(tail, C, device=DEV, generator=g)
+    w, b = (torch.randn(C, device=DEV, generator=g) for _ in range(2))
+    y, mean, rstd = ops.layer_norm_train_forward(x, w, b, EPS)
+    gx, gw, gb = ops.layer_norm_backward(x, x, mean, rstd, w, b)
+    own = x[-tail:].clone()
+    want, m, r = ops.layer_norm_train_forward(own, w, b, EPS)
+    assert torch.equal(y[-tail:], want) and torch.equal(mean[-tail:], m) and torch.equal(rstd[-tail:], r)
+    wx, ww, wb = ops.layer_norm_backward(own, own, m, r, w, b)
+    assert torch.equal(gx[-tail:], wx)
+    assert torch.equal(y[0], b.to(BF16)) and not gx[:1000].any()
+    # parameter gradients: other rows are zero, so both are sums of the same values in other orders
+    scale = own.double().abs().sum(0)
+    order = 2 * tail * 2.0 ** -24                        # each of two orders of `tail` fp32 additions
+    assert bool(((gb - wb).double().abs() <= order * scale).all())
+    xh = (own.double() - m[:, None]) * r[:, None]
+    assert bool(((gw - ww).double().abs() <= 1.01 * order * (xh * own.double()).abs().sum(0)).all())
+
+
 def test_degenerate_rows():
     """Constant rows have no spread: xh is 0 and rstd 1/sqrt(eps); the gradient follows the formula."""
     d = make(6, 40, F32, F32, F32)

@@ -42,6 +42,14 @@ def test_layernorm_forward_refuses(lib):
     assert _fwd(lib, rows=0) == 0
 
 
+def test_layernorm_row_limit(lib):
+    """Row numbers plus a stride of the grid stay within 32 bits."""
+    most = 1 << 30
+    assert _fwd(lib, rows=most + 1) == -9 and _bwd(lib, rows=most + 1) == -9
+    need = lib.dcnv4b200_layernorm_train_bwd_workspace_bytes
+    assert need(0, most, 1) > 0 and need(0, most + 1, 1) == 0
+
+
 def test_layernorm_backward_refuses(lib):
     assert _bwd(lib, gx=None) == -1 and _bwd(lib, gw=None) == -1 and _bwd(lib, gy=None) == -1
     assert _bwd(lib, mode=1, gamma=0x100) == -1           # layer scale without room for its gradient
