@@ -47,6 +47,7 @@ _SIGNATURES = {
     "dcnv4b200_layernorm_train_fwd": (_i, [_p] * 10 + [_i] * 4 + [C.c_longlong, _i, C.c_longlong, _f, _i, _p]),
     "dcnv4b200_layernorm_train_bwd_workspace_bytes": (_z, [_i, C.c_longlong, _i]),
     "dcnv4b200_layernorm_train_bwd": (_i, [_p] * 15 + [_z] + [_i] * 4 + [C.c_longlong, _i, C.c_longlong, _i, _p]),
+    "dcnv4b200_add_layernorm_bwd": (_i, [_p] * 13 + [_z, _i, _i, C.c_longlong, _i, C.c_longlong, _p]),
     "dcnv4b200_newton_schulz_workspace_bytes": (_z, [C.c_longlong, _i, _i]),
     "dcnv4b200_newton_schulz": (_i, [_p, _p, _p, _z, _i, C.c_longlong, _i, _i, _i, _f, _f, _f, _f, _p]),
     "dcnv4b200_device_status": (_i, [C.POINTER(_i)]),
@@ -101,7 +102,7 @@ def bindings():
             spec.loader.exec_module(module)
             module.init(*(C.cast(fn, C.c_void_p).value for fn in (
                 handle.dcnv4b200_layernorm_train_fwd, handle.dcnv4b200_layernorm_train_bwd,
-                handle.dcnv4b200_layernorm_train_bwd_workspace_bytes)))
+                handle.dcnv4b200_layernorm_train_bwd_workspace_bytes, handle.dcnv4b200_add_layernorm_bwd)))
             _bindings = module
     return _bindings
 

@@ -497,12 +497,12 @@ size_t dcnv4b200_layernorm_train_bwd_workspace_bytes(int dtype, long long rows, 
   return ln_train_workspace_bytes(dtype, (int)rows, C);
 }
 
-int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const void* x, const float* mean,
-                                  const float* rstd, const void* weight, const void* bias, const void* layer_scale,
-                                  const float* sample_scale, void* grad_x, void* grad_branch, void* grad_weight,
-                                  void* grad_bias, void* grad_layer_scale, void* workspace, size_t workspace_bytes,
-                                  int mode, int dtype, int out_dtype, int param_dtype, long long rows, int C,
-                                  long long rows_per_sample, int activation, void* stream) {
+// The backward pass; `residual` where the pre-norm seam forms its sum again from branch x and residual, else null.
+static int ln_train_bwd(const void* grad_y, const void* grad_h, const void* x, const void* residual, const float* mean,
+                        const float* rstd, const void* weight, const void* bias, const void* layer_scale,
+                        const float* sample_scale, void* grad_x, void* grad_branch, void* grad_weight, void* grad_bias,
+                        void* grad_layer_scale, void* workspace, size_t workspace_bytes, int mode, int dtype, int out_dtype,
+                        int param_dtype, long long rows, int C, long long rows_per_sample, int activation, void* stream) {
   LnTrainArgs a;
   if (int rc = fill_ln_train(a, weight, bias, layer_scale, sample_scale, mode, dtype, out_dtype, param_dtype, rows, C,
                              rows_per_sample, activation))
@@ -523,18 +523,42 @@ int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const 
   const bool pre = mode == DCNV4B200_LN_PRE;
   if (pre && !grad_branch && (sample_scale || dtype != out_dtype)) return DCNV4B200_ERR_NULL;
   if (!element_aligned(grad_y, out_dtype) || !element_aligned(grad_h, out_dtype) ||
-      !element_aligned(x, pre ? out_dtype : dtype) || !element_aligned(grad_x, pre ? out_dtype : dtype) ||
-      !element_aligned(grad_branch, dtype) || !aligned16(workspace) || !element_aligned(mean, DCNV4B200_F32) ||
-      !element_aligned(rstd, DCNV4B200_F32))
+      !element_aligned(x, pre ? out_dtype : dtype) || !element_aligned(residual, out_dtype) ||
+      !element_aligned(grad_x, pre ? out_dtype : dtype) || !element_aligned(grad_branch, dtype) || !aligned16(workspace) ||
+      !element_aligned(mean, DCNV4B200_F32) || !element_aligned(rstd, DCNV4B200_F32))
     return DCNV4B200_ERR_ALIGN;
   if (!workspace || workspace_bytes < ln_train_workspace_bytes(dtype, (int)rows, C)) return DCNV4B200_ERR_WORKSPACE;
-  if (pre) a.h = const_cast<void*>(x);
+  if (pre && !residual) a.h = const_cast<void*>(x);
   else a.x = x;
+  a.res = residual;
   a.gy = grad_y; a.gh = pre ? grad_h : nullptr; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.dx = grad_x; a.dx2 = pre ? grad_branch : nullptr; a.partial = static_cast<float*>(workspace);
   a.dw = grad_weight; a.db = grad_bias; a.dgamma = grad_layer_scale;
   if (int rc = status_ptr(&a.status)) return rc;
   return (int)launch_ln_train_bwd(mode, activation, dtype, out_dtype, a, s);
+}
+
+int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const void* x, const float* mean,
+                                  const float* rstd, const void* weight, const void* bias, const void* layer_scale,
+                                  const float* sample_scale, void* grad_x, void* grad_branch, void* grad_weight,
+                                  void* grad_bias, void* grad_layer_scale, void* workspace, size_t workspace_bytes,
+                                  int mode, int dtype, int out_dtype, int param_dtype, long long rows, int C,
+                                  long long rows_per_sample, int activation, void* stream) {
+  return ln_train_bwd(grad_y, grad_h, x, nullptr, mean, rstd, weight, bias, layer_scale, sample_scale, grad_x, grad_branch,
+                      grad_weight, grad_bias, grad_layer_scale, workspace, workspace_bytes, mode, dtype, out_dtype,
+                      param_dtype, rows, C, rows_per_sample, activation, stream);
+}
+
+int dcnv4b200_add_layernorm_bwd(const void* grad_y, const void* grad_h, const void* x, const void* residual,
+                                const float* mean, const float* rstd, const void* weight, const float* sample_scale,
+                                void* grad_residual, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                size_t workspace_bytes, int dtype, int param_dtype, long long rows, int C,
+                                long long rows_per_sample, void* stream) {
+  if (dtype != DCNV4B200_F16 && dtype != DCNV4B200_BF16) return DCNV4B200_ERR_DTYPE;
+  if (rows > 0 && !residual) return DCNV4B200_ERR_NULL;
+  return ln_train_bwd(grad_y, grad_h, x, residual, mean, rstd, weight, weight, nullptr, sample_scale, grad_residual, grad_x,
+                      grad_weight, grad_bias, nullptr, workspace, workspace_bytes, DCNV4B200_LN_PRE, dtype, dtype,
+                      param_dtype, rows, C, rows_per_sample, DCNV4B200_ACT_NONE, stream);
 }
 
 size_t dcnv4b200_newton_schulz_workspace_bytes(long long batch, int m, int n) {

@@ -24,11 +24,14 @@ using FwdFn = int (*)(const void*, const void*, const void*, const void*, const 
 using BwdFn = int (*)(const void*, const void*, const void*, const float*, const float*, const void*, const void*,
                       const void*, const float*, void*, void*, void*, void*, void*, void*, size_t, int, int, int, int,
                       long long, int, long long, int, void*);
+using SeamBwdFn = int (*)(const void*, const void*, const void*, const void*, const float*, const float*, const void*,
+                          const float*, void*, void*, void*, void*, void*, size_t, int, int, long long, int, long long, void*);
 using WorkspaceFn = size_t (*)(int, long long, int);
 
 FwdFn g_fwd = nullptr;
 BwdFn g_bwd = nullptr;
 WorkspaceFn g_workspace = nullptr;
+SeamBwdFn g_seam_bwd = nullptr;
 
 constexpr int kPlain = 0, kPost = 1, kPre = 2;
 constexpr int64_t kMaxChannels = 8192, kMaxRows = (int64_t)1 << 30;
@@ -79,12 +82,13 @@ bool accept(const at::Tensor& x, at::ScalarType x_type, at::ScalarType out_type,
   return true;
 }
 
-// init(forward, backward, workspace bytes): addresses of the library's functions.
+// init(forward, backward, workspace bytes, backward of the seam from branch and residual): addresses of the library's functions.
 PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 3) { PyErr_SetString(PyExc_TypeError, "init takes three addresses"); return nullptr; }
+  if (n != 4) { PyErr_SetString(PyExc_TypeError, "init takes four addresses"); return nullptr; }
   g_fwd = reinterpret_cast<FwdFn>(PyLong_AsVoidPtr(a[0]));
   g_bwd = reinterpret_cast<BwdFn>(PyLong_AsVoidPtr(a[1]));
   g_workspace = reinterpret_cast<WorkspaceFn>(PyLong_AsVoidPtr(a[2]));
+  g_seam_bwd = reinterpret_cast<SeamBwdFn>(PyLong_AsVoidPtr(a[3]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -131,24 +135,27 @@ PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// ln_backward(mode, grad_y, grad_h, x or h, mean, rstd, weight, bias, layer_scale, sample_scale, activation, type code of
-// the branch input) -> (grad_x, grad_branch, grad_weight, grad_bias, grad_layer_scale), an error code, or None.  grad_branch
-// is grad_x itself where the two are equal; grad_layer_scale is None without a layer scale.
+// ln_backward(mode, grad_y, grad_h, x or h, residual, mean, rstd, weight, bias, layer_scale, sample_scale, activation, type
+// code of the branch input) -> (grad_x, grad_branch, grad_weight, grad_bias, grad_layer_scale), an error code, or None.
+// With a residual (pre-norm seam in 16 bits) x is the branch.  grad_branch is grad_x itself where the two are equal;
+// grad_layer_scale is None without a layer scale.
 PyObject* py_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 12 || !g_bwd) Py_RETURN_NONE;
+  if (n != 13 || !g_bwd) Py_RETURN_NONE;
   bool ok = true;
-  const int mode = (int)PyLong_AsLong(a[0]), act = (int)PyLong_AsLong(a[10]), code = (int)PyLong_AsLong(a[11]);
+  const int mode = (int)PyLong_AsLong(a[0]), act = (int)PyLong_AsLong(a[11]), code = (int)PyLong_AsLong(a[12]);
   if (PyErr_Occurred()) return nullptr;
-  const at::Tensor *gy = tensor(a[1], ok), *gh = tensor(a[2], ok), *x = tensor(a[3], ok), *mean = tensor(a[4], ok);
-  const at::Tensor *rstd = tensor(a[5], ok), *w = tensor(a[6], ok), *b = tensor(a[7], ok), *gamma = tensor(a[8], ok);
-  const at::Tensor* s = tensor(a[9], ok);
+  const at::Tensor *gy = tensor(a[1], ok), *gh = tensor(a[2], ok), *x = tensor(a[3], ok), *res = tensor(a[4], ok);
+  const at::Tensor *mean = tensor(a[5], ok), *rstd = tensor(a[6], ok), *w = tensor(a[7], ok), *b = tensor(a[8], ok);
+  const at::Tensor *gamma = tensor(a[9], ok), *s = tensor(a[10], ok);
   if (!ok || !gy || !x || !mean || !rstd || !w || !b || code < 0 || code > 2) Py_RETURN_NONE;
   const bool pre = mode == kPre;
   const at::ScalarType branch_type = type_of(code), out = gy->scalar_type();
   int64_t rows, C, per;
   if (!accept(*x, branch_type, out, *w, *b, gamma, s, rows, C, per)) Py_RETURN_NONE;
   const at::Device dev = x->device();
+  if (res && (!pre || branch_type != out || out == at::kFloat || !plain(*res, dev, out) || res->sizes() != x->sizes()))
+    Py_RETURN_NONE;
   if (x->scalar_type() != (pre ? out : branch_type) || !plain(*gy, dev, out) || gy->sizes() != x->sizes() ||
       (gh && (!plain(*gh, dev, out) || gh->sizes() != x->sizes())) || !plain(*mean, dev, at::kFloat) ||
       mean->numel() != rows || !plain(*rstd, dev, at::kFloat) || rstd->numel() != rows)
@@ -166,12 +173,17 @@ PyObject* py_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (gamma) gs = at::empty(gamma->sizes(), param);
     const size_t bytes = g_workspace(code, rows, (int)C);
     at::Tensor ws = at::empty({(int64_t)bytes}, opts.dtype(at::kByte));
-    rc = g_bwd(gy->data_ptr(), pre ? data(gh) : nullptr, x->data_ptr(), mean->data_ptr<float>(), rstd->data_ptr<float>(),
-               w->data_ptr(), b->data_ptr(), data(gamma), static_cast<const float*>(data(s)), gx.data_ptr(),
-               branch.defined() ? branch.data_ptr() : nullptr, gw.data_ptr(), gb.data_ptr(),
-               gs.defined() ? gs.data_ptr() : nullptr, ws.data_ptr(), bytes, mode, code, code_of(out),
-               code_of(w->scalar_type()), rows, (int)C, per, act,
-               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    void* branch_ptr = branch.defined() ? branch.data_ptr() : nullptr;
+    if (res)
+      rc = g_seam_bwd(gy->data_ptr(), data(gh), x->data_ptr(), res->data_ptr(), mean->data_ptr<float>(), rstd->data_ptr<float>(),
+                      w->data_ptr(), static_cast<const float*>(data(s)), gx.data_ptr(), branch_ptr, gw.data_ptr(),
+                      gb.data_ptr(), ws.data_ptr(), bytes, code, code_of(w->scalar_type()), rows, (int)C, per, stream);
+    else
+      rc = g_bwd(gy->data_ptr(), pre ? data(gh) : nullptr, x->data_ptr(), mean->data_ptr<float>(), rstd->data_ptr<float>(),
+                 w->data_ptr(), b->data_ptr(), data(gamma), static_cast<const float*>(data(s)), gx.data_ptr(), branch_ptr,
+                 gw.data_ptr(), gb.data_ptr(), gs.defined() ? gs.data_ptr() : nullptr, ws.data_ptr(), bytes, mode, code,
+                 code_of(out), code_of(w->scalar_type()), rows, (int)C, per, act, stream);
   }
   if (rc) return PyLong_FromLong(rc);
   PyObject* tuple = PyTuple_New(5);

@@ -51,7 +51,7 @@ static ln::Plan plan_of(bool backward, int mode, int xd, int yd, const LnTrainAr
   auto on = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const bool base = on(a.x, 16) && on(a.res, 16) && on(a.h, 16) && on(a.gy, 16) && on(a.gh, 16);
   const bool vec = on(a.y, 16) && on(a.h, 16) && on(a.dx, 16) && on(a.dx2, 16);
-  return ln::plan_for(backward, mode, size_of(xd), size_of(yd), a.gh != nullptr, base, vec, a.rows, a.C);
+  return ln::plan_for(backward, mode, size_of(xd), size_of(yd), a.gh != nullptr, a.res != nullptr, base, vec, a.rows, a.C);
 }
 
 // Partial sums of the backward pass: one (2, C) fp32 block per CTA, for whichever kernel the alignment will choose.

@@ -11,6 +11,13 @@
 //   plain, pre: dw = A, db = B;   post: dw = gamma A, db = gamma B, dgamma = w A + b B
 // so one row kernel and one small reduction over the CTAs' partial (A, B) serve all three.
 //
+// The statistics of `pre` are those of the fp32 sum, of which a 16-bit h has lost bits: xh of the stored h with them would
+// carry h's rounding into every gradient, and a row whose spread is small beside that rounding would get an xh of
+// anything up to |h| 2^-9 / sqrt(eps).  So where h has 16 bits the backward pass reads residual and branch and forms the
+// sum again, by the forward's own fma, hence bit for bit (one more 16-bit tensor read; an fp32 h is the sum itself).  A
+// caller who has kept the 16-bit h alone gets the gradient at h as stored: the mean is h's own, and 1/sigma is the given
+// one or what h's own spread allows, whichever is less.
+//
 // All of them are bound by memory: a few operations per element, each tensor read and written once.  Rows are contiguous,
 // so a tile of rows is one span per tensor, and a ring of such tiles is kept in flight with bulk copies (cp.async.bulk,
 // mbarriers, bounded waits) while the CTA's 8 or 16 warps compute: the bytes in flight do not depend on how many
@@ -34,8 +41,8 @@
 namespace dcnb200 {
 
 struct LnTrainArgs {
-  const void* x;         // branch input (plain, post: the normalised tensor)
-  const void* res;       // residual (post, pre)
+  const void* x;         // branch input (plain, post: the normalised tensor); backward of pre: with res, to form the sum again
+  const void* res;       // residual (post, pre; backward: pre with a 16-bit sum, or null)
   const void* w;         // LayerNorm weight, bias, layer scale (may be null): all in the parameter type
   const void* b;
   const void* gamma;
@@ -240,11 +247,11 @@ __device__ __forceinline__ void span_tail(unsigned char* dst, const T* src, uint
   for (uint32_t i = (bytes & ~15u) / sizeof(T); i < bytes / sizeof(T); ++i) reinterpret_cast<T*>(dst)[i] = src[i];
 }
 
-// Fills the ring.  One lane of the first warp asks for a tile of up to three tensors; it refills a slot when it starts the
+// Fills the ring.  One lane of the first warp asks for a tile of up to four tensors; it refills a slot when it starts the
 // tile after the one the slot held, so it waits for the slowest warp of that tile and no warp does nothing else.
-template <typename T0, typename T1, typename T2>
+template <typename T0, typename T1, typename T2, typename T3 = T2>
 struct RingFill {
-  const T0* p0; const T1* p1; const T2* p2;
+  const T0* p0; const T1* p1; const T2* p2; const T3* p3;
   unsigned char* ring;
   RingHeader* h;
   int tiles;
@@ -252,25 +259,29 @@ struct RingFill {
   __device__ __forceinline__ uint32_t slot0(const LnTrainArgs& a) const { return span_bytes(a.tile_rows, a.C, sizeof(T0)); }
   __device__ __forceinline__ uint32_t slot1(const LnTrainArgs& a) const { return p1 ? span_bytes(a.tile_rows, a.C, sizeof(T1)) : 0; }
   __device__ __forceinline__ uint32_t slot2(const LnTrainArgs& a) const { return p2 ? span_bytes(a.tile_rows, a.C, sizeof(T2)) : 0; }
+  __device__ __forceinline__ uint32_t slot3(const LnTrainArgs& a) const { return p3 ? span_bytes(a.tile_rows, a.C, sizeof(T3)) : 0; }
 
   // tile `t` into slot `stage`, which is free
   __device__ void issue(const LnTrainArgs& a, int t, int stage) const {
-    const uint32_t z0 = slot0(a), z1 = slot1(a);
+    const uint32_t z0 = slot0(a), z1 = slot1(a), z2 = slot2(a);
     const long long row0 = (long long)t * a.tile_rows;
     const int n = (int)(a.rows - row0 < a.tile_rows ? a.rows - row0 : a.tile_rows);
     const uint32_t b0 = span_bytes(n, a.C, sizeof(T0)), b1 = p1 ? span_bytes(n, a.C, sizeof(T1)) : 0;
-    const uint32_t b2 = p2 ? span_bytes(n, a.C, sizeof(T2)) : 0;
-    unsigned char* d = ring + (size_t)stage * (z0 + z1 + slot2(a));
+    const uint32_t b2 = p2 ? span_bytes(n, a.C, sizeof(T2)) : 0, b3 = p3 ? span_bytes(n, a.C, sizeof(T3)) : 0;
+    unsigned char* d = ring + (size_t)stage * (z0 + z1 + z2 + slot3(a));
     const T0* s0 = p0 + row0 * a.C;
     const T1* s1 = p1 ? p1 + row0 * a.C : nullptr;
     const T2* s2 = p2 ? p2 + row0 * a.C : nullptr;
+    const T3* s3 = p3 ? p3 + row0 * a.C : nullptr;
     span_tail(d, s0, b0);
     if (p1) span_tail(d + z0, s1, b1);
     if (p2) span_tail(d + z0 + z1, s2, b2);
-    mbar_expect_tx(&h->full[stage], (b0 & ~15u) + (b1 & ~15u) + (b2 & ~15u));
+    if (p3) span_tail(d + z0 + z1 + z2, s3, b3);
+    mbar_expect_tx(&h->full[stage], (b0 & ~15u) + (b1 & ~15u) + (b2 & ~15u) + (b3 & ~15u));
     if (b0 & ~15u) bulk_g2s(d, s0, b0 & ~15u, &h->full[stage]);
     if (b1 & ~15u) bulk_g2s(d + z0, s1, b1 & ~15u, &h->full[stage]);
     if (b2 & ~15u) bulk_g2s(d + z0 + z1, s2, b2 & ~15u, &h->full[stage]);
+    if (b3 & ~15u) bulk_g2s(d + z0 + z1 + z2, s3, b3 & ~15u, &h->full[stage]);
   }
   __device__ void start(const LnTrainArgs& a) const {
     for (int s = 0; s < a.stages; ++s) {
@@ -486,6 +497,36 @@ __device__ __forceinline__ float ring_sum(float t, int lpr, RingHeader* h, int& 
   return t;
 }
 
+// Sum of a lane's elements.  Two chains of additions, here and below: a warp's own latency is what short rows wait for.
+template <int N>
+__device__ __forceinline__ float lane_sum(const float2 (&x)[N]) {
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum[i & 1] = add2(sum[i & 1], x[i]);
+  sum[0] = add2(sum[0], sum[1]);
+  return sum[0].x + sum[0].y;
+}
+// Takes the mean off a lane's elements; returns the sum of the squares of those that belong to the row.
+template <int VEC, int NV, bool SHIFT>
+__device__ __forceinline__ float lane_centre(float2 (&x)[NV * VEC / 2], float mean, int sub, int lpr, int C, int shift) {
+  float2 sq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) {
+    x[i] = add2(x[i], both(-mean));
+    if (VEC > 1 && (SHIFT ? 2 * i / VEC != 0 && 2 * i / VEC + 2 < NV : 2 * i / VEC + 1 < NV)) {
+      sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
+    } else if (VEC > 1 && !SHIFT) {
+      if (column<VEC>(2 * i, sub, lpr) < C) sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
+    } else {      // the elements of a pair may differ in whether they belong to the row
+      const int c0 = column<VEC>(2 * i, sub, lpr) - shift, c1 = column<VEC>(2 * i + 1, sub, lpr) - shift;
+      if (c0 >= 0 && c0 < C) sq[i & 1].x = fmaf(x[i].x, x[i].x, sq[i & 1].x);
+      if (c1 >= 0 && c1 < C) sq[i & 1].y = fmaf(x[i].y, x[i].y, sq[i & 1].y);
+    }
+  }
+  sq[0] = add2(sq[0], sq[1]);
+  return sq[0].x + sq[0].y;
+}
+
 template <typename TX, typename TY, int VEC, int NV, bool SHIFT, int MODE, bool GELU>
 __global__ void __launch_bounds__(32 * ring_warps<VEC * NV>(), fwd_ctas(VEC * NV))
 ln_ring_fwd_kernel(const LnTrainArgs a) {
@@ -497,7 +538,7 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
   const int lpr = a.lpr, C = a.C, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
   const RingFill<TX, TY, TY> fill{static_cast<const TX*>(a.x), MODE == kPlain ? nullptr : static_cast<const TY*>(a.res), nullptr,
-                                  ring, h, tiles};
+                                  nullptr, ring, h, tiles};
   // the first thread sets up and fills the ring while the others fetch the parameters
   if (threadIdx.x == 0) ring_init(h, a.stages, W);
   pdl_trigger();
@@ -564,28 +605,8 @@ ln_ring_fwd_kernel(const LnTrainArgs a) {
           for (int i = 0; i < NE / 2; ++i) x[i] = fma2(both(s), x[i], r[i]);
           if (live) row_store<TY, VEC, NV, SHIFT>(static_cast<TY*>(a.h) + (long long)row * C, x, sub, lpr, C, shift);
         }
-        // two chains of additions each: a warp's own latency is what these short rows wait for
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int i = 0; i < NE / 2; ++i) sum[i & 1] = add2(sum[i & 1], x[i]);
-        sum[0] = add2(sum[0], sum[1]);
-        const float mean = ring_sum(sum[0].x + sum[0].y, lpr, h, flip) * inv_c;
-        float2 sq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int i = 0; i < NE / 2; ++i) {
-          x[i] = add2(x[i], both(-mean));
-          if (VEC > 1 && (SHIFT ? 2 * i / VEC != 0 && 2 * i / VEC + 2 < NV : 2 * i / VEC + 1 < NV)) {
-            sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
-          } else if (VEC > 1 && !SHIFT) {
-            if (column<VEC>(2 * i, sub, lpr) < C) sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
-          } else {      // the elements of a pair may differ in whether they belong to the row
-            const int c0 = column<VEC>(2 * i, sub, lpr) - shift, c1 = column<VEC>(2 * i + 1, sub, lpr) - shift;
-            if (c0 >= 0 && c0 < C) sq[i & 1].x = fmaf(x[i].x, x[i].x, sq[i & 1].x);
-            if (c1 >= 0 && c1 < C) sq[i & 1].y = fmaf(x[i].y, x[i].y, sq[i & 1].y);
-          }
-        }
-        sq[0] = add2(sq[0], sq[1]);
-        const float rstd = rsqrtf(ring_sum(sq[0].x + sq[0].y, lpr, h, flip) * inv_c + a.eps);
+        const float mean = ring_sum(lane_sum(x), lpr, h, flip) * inv_c;
+        const float rstd = rsqrtf(ring_sum(lane_centre<VEC, NV, SHIFT>(x, mean, sub, lpr, C, shift), lpr, h, flip) * inv_c + a.eps);
         if (!live) continue;
         if constexpr (kStaged) {
           param_row<VEC, NV>(w, ws, sub, lpr, C);
@@ -624,13 +645,16 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
   const int lpr = a.lpr, C = a.C, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
   const bool with_gh = MODE == kPre && a.gh != nullptr;
+  constexpr bool kNarrow = MODE == kPre && sizeof(TL) == 2;   // h has lost bits of the sum that was normalised
+  const bool summed = kNarrow && a.res != nullptr;            // x is the branch, and the sum is formed again
   const int sub = (int)threadIdx.x % lpr, team = (int)threadIdx.x / lpr;
   const int shift = SHIFT ? (int)((unsigned)team * (unsigned)C % VEC) : 0;
   float2 sa[NE / 2], sb[NE / 2];
 #pragma unroll
   for (int i = 0; i < NE / 2; ++i) sa[i] = sb[i] = make_float2(0.f, 0.f);
-  const RingFill<TL, TG, TG> fill{static_cast<const TL*>(MODE == kPre ? a.h : a.x), static_cast<const TG*>(a.gy),
-                                  with_gh ? static_cast<const TG*>(a.gh) : nullptr, ring, h, tiles};
+  const RingFill<TL, TG, TG, TL> fill{static_cast<const TL*>(MODE == kPre && !summed ? a.h : a.x), static_cast<const TG*>(a.gy),
+                                      with_gh ? static_cast<const TG*>(a.gh) : nullptr,
+                                      kNarrow ? static_cast<const TL*>(a.res) : nullptr, ring, h, tiles};
   if (threadIdx.x == 0) ring_init(h, a.stages, W);
   pdl_trigger();
   pdl_wait();
@@ -640,7 +664,7 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
     const int first = lpr > 32 ? team : warp * (32 / lpr);
     const int passes = (a.tile_rows + per_pass - 1) / per_pass;
     const float inv_c = 1.f / (float)C;
-    const uint32_t slot0 = fill.slot0(a), slot1 = fill.slot1(a), slot = slot0 + slot1 + fill.slot2(a);
+    const uint32_t slot0 = fill.slot0(a), slot1 = fill.slot1(a), slot2 = fill.slot2(a), slot = slot0 + slot1 + slot2 + fill.slot3(a);
     int flip = 0;
     constexpr bool kStaged = params_in_smem<VEC, NV>();
     float2 w[NE / 2], b[GELU ? NE / 2 : 1];
@@ -682,7 +706,8 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
       const int row0 = t * a.tile_rows;
       const int n = a.rows - row0 < a.tile_rows ? a.rows - row0 : a.tile_rows;
       for (int pass = 0; pass < passes; ++pass) {
-        const float mean = mean_n, rstd = rstd_n, s = s_n;
+        float mean = mean_n, rstd = rstd_n;
+        const float s = s_n;
         if (pass + 1 < passes) stats(t, pass + 1, mean_n, rstd_n, s_n);
         else stats(t + gridDim.x, 0, mean_n, rstd_n, s_n);
         const int lr = pass * per_pass + team;
@@ -691,6 +716,17 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
         const int row = row0 + lr;
         float2 x[NE / 2], g[NE / 2];
         row_load<TL, VEC, NV, SHIFT>(x, reinterpret_cast<const TL*>(base) + (size_t)lr * C, sub, lpr, C, live, shift);
+        if constexpr (kNarrow) {
+          if (summed) {
+            row_load<TL, VEC, NV, SHIFT>(g, reinterpret_cast<const TL*>(base + slot0 + slot1 + slot2) + (size_t)lr * C, sub, lpr, C, live, shift);
+#pragma unroll
+            for (int i = 0; i < NE / 2; ++i) x[i] = fma2(both(s), x[i], g[i]);
+          } else {
+            mean = ring_sum(lane_sum(x), lpr, h, flip) * inv_c;
+            rstd = fminf(rstd, rsqrtf(ring_sum(lane_centre<VEC, NV, SHIFT>(x, mean, sub, lpr, C, shift), lpr, h, flip) * inv_c));
+            mean = 0.f;
+          }
+        }
         row_load<TG, VEC, NV, SHIFT>(g, reinterpret_cast<const TG*>(base + slot0) + (size_t)lr * C, sub, lpr, C, live, shift);
         // elements beyond C have g = w = 0 and add nothing to any sum
         float2 t1[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, t2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -893,6 +929,8 @@ ln_train_bwd_kernel(const LnTrainArgs a) {
   const int lpr = a.lpr, C = a.C;
   const bool wide = lpr > 32;
   const int lane = threadIdx.x & 31;
+  constexpr bool kNarrow = MODE == kPre && sizeof(TL) == 2;   // as in the ring kernel
+  const bool summed = kNarrow && a.res != nullptr;
   const int sub = wide ? threadIdx.x : lane % lpr;
   const int team0 = wide ? blockIdx.x : (blockIdx.x * blockDim.x + threadIdx.x) / lpr;
   const int n_teams = wide ? gridDim.x : gridDim.x * blockDim.x / lpr;
@@ -918,25 +956,50 @@ ln_train_bwd_kernel(const LnTrainArgs a) {
     const int row = wide ? r0 : r0 + lane / lpr;
     const bool live = row < a.rows;
     const long long base = (long long)row * C;
-    Words<TL, VEC> rx[NV];
+    Words<TL, VEC> rx[NV], rr[kNarrow ? NV : 1];
     Words<TG, VEC> rg[NV], rh[MODE == kPre ? NV : 1];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (sub + v * lpr) * VEC;
       const bool ok = live && c < C;
-      load<TL, VEC>(rx[v], static_cast<const TL*>(MODE == kPre ? a.h : a.x) + base + c, ok);
+      load<TL, VEC>(rx[v], static_cast<const TL*>(MODE == kPre && !summed ? a.h : a.x) + base + c, ok);
+      if (kNarrow) load<TL, VEC>(rr[v], static_cast<const TL*>(a.res) + base + c, ok && summed);
       load<TG, VEC>(rg[v], static_cast<const TG*>(a.gy) + base + c, ok);
       if (MODE == kPre) load<TG, VEC>(rh[v], static_cast<const TG*>(a.gh) + base + c, ok && a.gh != nullptr);
     }
-    const float mean = live ? __ldg(a.mean + row) : 0.f, rstd = live ? __ldg(a.rstd + row) : 0.f;
+    float mean = live ? __ldg(a.mean + row) : 0.f, rstd = live ? __ldg(a.rstd + row) : 0.f;
     float s = 1.f;
     if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
     float xh[NV][VEC], gw[NV][VEC];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float g[VEC];
       to_floats<TL, VEC>(rx[v], xh[v]);
+      if (kNarrow && summed) {
+        float rv[VEC];
+        to_floats<TL, VEC>(rr[v], rv);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) xh[v][e] = fmaf(s, xh[v][e], rv[e]);
+      }
+    }
+    if (kNarrow && !summed) {
+      float sum = 0.f, sq = 0.f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += xh[v][e];
+      mean = team_sum(sum, 0.f, lpr, red, flip).x * inv_c;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if ((sub + v * lpr) * VEC < C) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) { const float d = xh[v][e] - mean; sq = fmaf(d, d, sq); }
+        }
+      rstd = fminf(rstd, rsqrtf(team_sum(sq, 0.f, lpr, red, flip).x * inv_c));
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float g[VEC];
       to_floats<TG, VEC>(rg[v], g);
       const bool ok = live && (sub + v * lpr) * VEC < C;
 #pragma unroll
@@ -1116,7 +1179,7 @@ struct Plan {
   bool direct;
   int grid;
 };
-inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool base16, bool vec_ok, int rows, int C) {
+inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool summed, bool base16, bool vec_ok, int rows, int C) {
   Plan p;
   const int V = x_es == 4 || y_es == 4 ? 4 : 8;
   p.vec = vec_ok && base16 ? V : 1;
@@ -1129,7 +1192,7 @@ inline Plan plan_for(bool backward, int mode, int x_es, int y_es, bool gh, bool 
   }
   if (!p.shift) p.g = geometry(p.vec > 1 ? C / V : C, p.vec, V == 8 ? 3 : 6);
   const int lx = backward && mode == kPre ? y_es : x_es;      // element size of the normalised tensor
-  const size_t row_bytes = (size_t)C * (backward ? lx + y_es * (1 + (mode == kPre && gh)) : x_es + (mode == kPlain ? 0 : y_es));
+  const size_t row_bytes = (size_t)C * (backward ? lx * (1 + (mode == kPre && summed)) + y_es * (1 + (mode == kPre && gh)) : x_es + (mode == kPlain ? 0 : y_es));
   const int es_min = backward ? (lx < y_es ? lx : y_es) : (mode == kPlain || x_es < y_es ? x_es : y_es);
   const int slots = p.shift || p.g.lpr > 32 ? p.g.warps * 32 / p.g.lpr : p.g.warps;
   const size_t acc = backward ? (size_t)slots * 2 * C * sizeof(float) : 0;

@@ -95,23 +95,32 @@ class LayerNormResidualFunction(Function):
 
 class AddLayerNormFunction(Function):
     """(h, y) with h = residual + sample_scale * x and y = LN(h): apply(x, residual, weight, bias, eps,
-    sample_scale=None).  `sample_scale` gets no gradient."""
+    sample_scale=None).  `sample_scale` gets no gradient.  Kept for the backward pass: h where it is float32, and x and
+    residual where h has 16 bits, since statistics and y are taken of the sum before it is rounded."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, sample_scale=None):
         ctx.set_materialize_grads(False)
         h, y, mean, rstd = ops.add_layer_norm_forward(x.contiguous(), residual.contiguous(), weight, bias, eps,
                                                       sample_scale)
-        ctx.eps, ctx.x_dtype = eps, x.dtype
-        ctx.save_for_backward(h, weight, bias, mean, rstd, sample_scale)   # h alone: x and residual may be freed
+        ctx.eps, ctx.x_dtype, ctx.from_sum = eps, x.dtype, h.dtype == torch.float32
+        kept = (h, None) if ctx.from_sum else (x, residual)
+        ctx.save_for_backward(*kept, weight, bias, mean, rstd, sample_scale)
         return h, y
 
     @staticmethod
     def backward(ctx, grad_h, grad_y):
-        h, weight, bias, mean, rstd, sample_scale = ctx.saved_tensors
+        first, residual, weight, bias, mean, rstd, sample_scale = ctx.saved_tensors
         if grad_h is None and grad_y is None:
             return (None,) * 6
-        if torch.is_grad_enabled():     # through h, an output of this node and so part of the graph
+        if torch.is_grad_enabled():
+            if not ctx.from_sum:
+                def both(x_, r_, w_, b_):
+                    s_ = x_.float() if sample_scale is None else x_.float() * _per_sample(sample_scale, x_)
+                    h_ = r_.float() + s_
+                    return h_.to(r_.dtype), _layer_norm(h_, w_, b_, ctx.eps, torch.float32).to(r_.dtype)
+                return (*_differentiable(both, (first, residual, weight, bias), (grad_h, grad_y)), None, None)
+            h = first                   # an output of this node and so part of the graph
             gr = grad_h
             gw = gb = None
             if grad_y is not None:
@@ -121,7 +130,13 @@ class AddLayerNormFunction(Function):
                 gr = through if gr is None else gr + through
             gx = (gr if sample_scale is None else gr * _per_sample(sample_scale, gr).to(gr.dtype)).to(ctx.x_dtype)
             return gx, gr, gw, gb, None, None
-        grad_y = torch.zeros_like(h) if grad_y is None else grad_y.contiguous()
+        first = first.contiguous()
+        grad_y = torch.zeros(first.shape, dtype=grad_h.dtype, device=first.device) if grad_y is None else grad_y.contiguous()
         grad_h = None if grad_h is None else grad_h.contiguous()
-        gr, gx, gw, gb = ops.add_layer_norm_backward(grad_y, grad_h, h, mean, rstd, weight, sample_scale, ctx.x_dtype)
+        if ctx.from_sum:
+            gr, gx, gw, gb = ops.add_layer_norm_backward(grad_y, grad_h, first, mean, rstd, weight, sample_scale,
+                                                         ctx.x_dtype)
+        else:
+            gr, gx, gw, gb = ops.add_layer_norm_backward(grad_y, grad_h, None, mean, rstd, weight, sample_scale, None,
+                                                         first, residual.contiguous())
         return gx, gr, gw, gb, None, None

@@ -338,18 +338,20 @@ def _ln_forward(mode, x, residual, weight, bias, eps, layer_scale, sample_scale,
 
 
 def _ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale, sample_scale, activation, x_dtype,
-                 what):
-    """(grad_x, grad_branch, grad_weight, grad_bias, grad_layer_scale); see `_ln_forward`."""
+                 what, residual=None):
+    """(grad_x, grad_branch, grad_weight, grad_bias, grad_layer_scale); see `_ln_forward`.  With `residual` (the seam
+    in 16 bits) x is the branch, else it is the normalised tensor."""
     act = 1 if activation == "gelu" else 0
-    got = (_binding or _load_binding()).ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale,
-                                                    sample_scale, act, _DTYPES.get(x_dtype, -1))
+    got = (_binding or _load_binding()).ln_backward(mode, grad_y, grad_h, x, residual, mean, rstd, weight, bias,
+                                                    layer_scale, sample_scale, act, _DTYPES.get(x_dtype, -1))
     if got.__class__ is tuple:
         return got
     if got is not None:
         _lib.check(got, what)
     out_dtype = grad_y.dtype
     pre = mode == _LN_PRE
-    grads = ((grad_y, "grad_y"), (grad_h, "grad_h"), (x, "h")) if pre else ((grad_y, "grad_y"),)
+    grads = ((grad_y, "grad_y"), (grad_h, "grad_h"), (residual, "residual"),
+             (x, "h" if residual is None else "x")) if pre else ((grad_y, "grad_y"),)
     rows, C, per = _check_ln(x, x_dtype, weight, bias, grads, layer_scale, sample_scale, out_dtype)
     for t in (mean, rstd):
         if not (t.device == x.device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == rows):
@@ -363,6 +365,14 @@ def _ln_backward(mode, grad_y, grad_h, x, mean, rstd, weight, bias, layer_scale,
     grad_s = None if layer_scale is None else torch.empty_like(layer_scale)
     ws_bytes = lib.dcnv4b200_layernorm_train_bwd_workspace_bytes(code, rows, C)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    if residual is not None:
+        rc = _on_device(
+            x, lib.dcnv4b200_add_layernorm_bwd, grad_y.data_ptr(), _ptr(grad_h), x.data_ptr(), residual.data_ptr(),
+            mean.data_ptr(), rstd.data_ptr(), weight.data_ptr(), _ptr(sample_scale), grad_x.data_ptr(), _ptr(branch),
+            grad_w.data_ptr(), grad_b.data_ptr(), ws.data_ptr(), ws_bytes, code, _DTYPES[weight.dtype], rows, C, per,
+            _stream(x))
+        _lib.check(rc, what)
+        return grad_x, grad_x if branch is None else branch, grad_w, grad_b, None
     rc = _on_device(
         x, lib.dcnv4b200_layernorm_train_bwd, grad_y.data_ptr(), _ptr(grad_h), x.data_ptr(), mean.data_ptr(),
         rstd.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(layer_scale), _ptr(sample_scale), grad_x.data_ptr(),
@@ -425,12 +435,25 @@ def add_layer_norm_forward(x: torch.Tensor, residual: torch.Tensor, weight: torc
                        "add_layer_norm_forward")
 
 
-def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor], h: torch.Tensor, mean: torch.Tensor,
-                            rstd: torch.Tensor, weight: torch.Tensor, sample_scale: Optional[torch.Tensor] = None,
-                            x_dtype: Optional[torch.dtype] = None):
+def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor], h: Optional[torch.Tensor],
+                            mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor,
+                            sample_scale: Optional[torch.Tensor] = None, x_dtype: Optional[torch.dtype] = None,
+                            x: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None):
     """(grad_residual, grad_x, grad_weight, grad_bias) of `add_layer_norm_forward`; `grad_h` may be None, `x_dtype` is
-    the dtype of the forward's x (default: that of h).  Without `sample_scale` and with equal dtypes the first two are
-    one tensor.  Deterministic."""
+    the dtype of the forward's x (default: that of h).  A float32 h is all the pass needs.  A 16-bit h has lost bits of
+    the sum whose statistics mean and rstd are: give the forward's x and residual too (h may then be None), and the pass
+    forms that sum again, bit for bit.  From a 16-bit h alone come the gradients at h as stored, normalised by its own
+    mean and by rstd or what h's own spread allows, whichever is less.  Without `sample_scale` and with equal dtypes the
+    first two results are one tensor.  Deterministic."""
+    if (x is None) != (residual is None):
+        raise RuntimeError("x and residual go together")
+    if residual is not None and residual.dtype != torch.float32:
+        if x_dtype not in (None, x.dtype):
+            raise RuntimeError("x_dtype must be the dtype of x")
+        return _ln_backward(_LN_PRE, grad_y, grad_h, x, mean, rstd, weight, weight, None, sample_scale, "none", x.dtype,
+                            "add_layer_norm_backward", residual)[:4]
+    if h is None:
+        raise RuntimeError("h is needed where it is float32")
     return _ln_backward(_LN_PRE, grad_y, grad_h, h, mean, rstd, weight, weight, None, sample_scale, "none",
                         h.dtype if x_dtype is None else x_dtype, "add_layer_norm_backward")[:4]
 

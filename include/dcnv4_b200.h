@@ -208,7 +208,10 @@ size_t dcnv4b200_layernorm_train_bwd_workspace_bytes(int dtype, long long rows, 
 /*
  * Backward of dcnv4b200_layernorm_train_fwd, same modes, types and limits:
  *   grad_y       (rows, C) in `out_dtype`; grad_h (rows, C) in `out_dtype` or NULL (PRE: gradient of h)
- *   x            the forward's x (PLAIN, POST) in `dtype`, or its h in `out_dtype` (PRE)
+ *   x            the forward's x (PLAIN, POST) in `dtype`, or its h in `out_dtype` (PRE).  A 16-bit h has lost bits of the
+ *                sum that the forward normalised: the gradients are then those at h as stored (its own mean; 1/sigma
+ *                the given one, or what h's own spread allows if that is less); dcnv4b200_add_layernorm_bwd gives those
+ *                at the sum itself
  *   grad_x       PLAIN, POST: gradient of x, in `dtype`; PRE: gradient of the residual, in `out_dtype`
  *   grad_branch  PRE: gradient of the forward's x, in `dtype`, or NULL where it equals grad_x (sample_scale NULL and
  *                dtype == out_dtype); NULL otherwise
@@ -224,6 +227,18 @@ int dcnv4b200_layernorm_train_bwd(const void* grad_y, const void* grad_h, const 
                                   void* grad_bias, void* grad_layer_scale, void* workspace, size_t workspace_bytes,
                                   int mode, int dtype, int out_dtype, int param_dtype, long long rows, int C,
                                   long long rows_per_sample, int activation, void* stream);
+
+/*
+ * Backward of the PRE form where everything but the parameters has 16 bits (`dtype` fp16 or bf16), from the forward's x
+ * and residual: the sum is formed again in fp32, bit for bit the one that mean and rstd belong to.  grad_residual and
+ * grad_x (rows, C); grad_x may be NULL without sample_scale, where the two are equal.  Everything else as
+ * dcnv4b200_layernorm_train_bwd, the workspace among it.
+ */
+int dcnv4b200_add_layernorm_bwd(const void* grad_y, const void* grad_h, const void* x, const void* residual,
+                                const float* mean, const float* rstd, const void* weight, const float* sample_scale,
+                                void* grad_residual, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                size_t workspace_bytes, int dtype, int param_dtype, long long rows, int C,
+                                long long rows_per_sample, void* stream);
 
 /*
  * Newton-Schulz orthogonalisation of a stack of matrices, the step of the Muon optimiser:
