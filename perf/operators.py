@@ -196,8 +196,9 @@ def _own(s):
         return {"out": out, "grad_x": gx, "grad_weight": gw, "grad_bias": gb, "grad_layer_scale": gs}
     h, y, mean, rstd = ops.add_layer_norm_forward(s["x"], s["residual"], s["weight"], s["bias"], EPS,
                                                   s["sample_scale"])
+    # a 16-bit h has lost bits of the sum that was normalised: the pass forms it again from branch and residual
     gr, gx, gw, gb = ops.add_layer_norm_backward(s["grad"], s["grad_h"], h, mean, rstd, s["weight"],
-                                                 s["sample_scale"], s["x"].dtype)
+                                                 s["sample_scale"], s["x"].dtype, s["x"], s["residual"])
     return {"h": h, "y": y, "grad_residual": gr, "grad_x": gx, "grad_weight": gw, "grad_bias": gb}
 
 
