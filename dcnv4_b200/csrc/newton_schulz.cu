@@ -718,10 +718,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallP
   const int n_gram = (p.p + 15) / 16 * 16, n_upd = (p.q + 15) / 16 * 16;
   if (threadIdx.x == 0) { mbar_init(&bar, 1); asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
   if (warp == 0) { tmem_alloc(&tmem_slot, (uint32_t)p.tmem_cols); tmem_relinquish(); }
-  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // only now: a dependent's block that took tensor memory while this one still waits for its own would hold it until this
+  // kernel's end
+  pdl_trigger();
   const uint32_t tx = tmem_slot + ((uint32_t)(quad * 32) << 16), ta = tx + (uint32_t)p.acc_col;
   const uint32_t acc = tmem_slot + (uint32_t)p.acc_col;
   pdl_wait();
