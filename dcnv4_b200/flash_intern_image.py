@@ -44,6 +44,10 @@ class LayerNorm(nn.LayerNorm):
 
     use_library_kernel = True   # class-wide switch (benchmarks turn it off to time the stock path)
 
+    def needs_grad(self, x):
+        """Whether autograd records the operation: any of its three inputs may be the one that is trained."""
+        return ops.needs_grad(x, self.weight, self.bias)
+
     def train_out_dtype(self, x):
         """Result dtype of the training kernels for this input, or None where the stock path has to run."""
         if not (self.use_library_kernel and self.elementwise_affine and self.bias is not None and x.is_cuda
@@ -58,16 +62,14 @@ class LayerNorm(nn.LayerNorm):
 
     def forward_act(self, x, activation="none"):
         """act(self(x)) by the training kernels, or None where they do not apply."""
-        needs_grad = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad)
-        out = self.train_out_dtype(x) if needs_grad else None
+        out = self.train_out_dtype(x) if self.needs_grad(x) else None
         return None if out is None else LayerNormFunction.apply(x, self.weight, self.bias, self.eps, activation, out)
 
     def forward(self, x):
         y = self.forward_act(x)
         if y is not None:
             return y
-        needs_grad = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad)
-        if (self.use_library_kernel and not needs_grad and self.elementwise_affine and self.bias is not None
+        if (self.use_library_kernel and not self.needs_grad(x) and self.elementwise_affine and self.bias is not None
                 and len(self.normalized_shape) == 1 and not torch.is_autocast_enabled()
                 and ops.layer_norm_supported(x, self.weight)):
             return ops.layer_norm_forward(x, self.weight, self.bias, self.eps)
@@ -150,7 +152,7 @@ class StemLayer(nn.Module):
         ln = self.norm1[1] if len(self.norm1) == 3 and isinstance(self.norm1[1], LayerNorm) else None
         if ln is None or not isinstance(self.act, nn.GELU) or self.act.approximate != "none":
             return None
-        if torch.is_grad_enabled() and (x.requires_grad or ln.weight.requires_grad):
+        if ln.needs_grad(x):
             y = ln.forward_act(x.permute(0, 2, 3, 1), "gelu")
             return None if y is None else y.permute(0, 3, 1, 2)
         if torch.is_autocast_enabled() or not LayerNorm.use_library_kernel:

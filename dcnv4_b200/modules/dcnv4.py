@@ -92,19 +92,18 @@ class DCNv4(nn.Module):
 
     def _blend_fusable(self, x, x_proj) -> bool:
         w = self.center_feature_scale_proj_weight
-        needs_grad = torch.is_grad_enabled() and (x.requires_grad or x_proj.requires_grad or w.requires_grad)
-        return (not needs_grad and not torch.is_autocast_enabled() and x.dtype == x_proj.dtype
+        return (not ops.needs_grad(x, x_proj, w, self.center_feature_scale_proj_bias) and not torch.is_autocast_enabled() and x.dtype == x_proj.dtype
                 and self.center_feature_scale_proj_bias.dtype == w.dtype
                 and ops.center_scale_blend_supported(x, w, self.group_channels))
 
     def _offsets_fusable(self, input) -> bool:
         """Inference on 16-bit CUDA tensors in the configuration the fused kernel is written for (3x3,
         stride 1, pad 1, dilation 1, all nine points, 16 channels per group), at a size where it pays."""
-        params = [self.offset_mask.weight] + ([] if self.without_pointwise else [self.value_proj.weight])
-        needs_grad = torch.is_grad_enabled() and (input.requires_grad or any(p.requires_grad for p in params))
+        layers = [self.offset_mask] + ([] if self.without_pointwise else [self.value_proj])
+        params = [p for m in layers for p in (m.weight, m.bias)]
         return (input.is_cuda and input.is_contiguous() and input.numel() > 0
                 and input.dtype in (torch.float16, torch.bfloat16) and self.offset_mask.weight.dtype == input.dtype
-                and not needs_grad and not torch.is_autocast_enabled()
+                and not ops.needs_grad(input, *params) and not torch.is_autocast_enabled()
                 and not self.remove_center and self.kernel_size == 3 and self.stride == 1 and self.pad == 1
                 and self.dilation == 1 and self.group_channels == 16
                 and ops.fused_offset_pays(input.numel() // input.shape[-1], self.channels, input.device))
