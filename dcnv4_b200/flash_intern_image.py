@@ -17,6 +17,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import nn
+from torch.nn.modules.module import _has_any_global_hook
 from torch.utils import checkpoint
 
 from . import ops
@@ -152,6 +153,9 @@ class StemLayer(nn.Module):
         ln = self.norm1[1] if len(self.norm1) == 3 and isinstance(self.norm1[1], LayerNorm) else None
         if ln is None or not isinstance(self.act, nn.GELU) or self.act.approximate != "none":
             return None
+        if not (_as_written(self.norm1, nn.Sequential) and _as_written(ln, LayerNorm) and _as_written(self.act, nn.GELU)
+                and _as_written(self.norm1[0], _ToChannelsLast) and _as_written(self.norm1[2], _ToChannelsFirst)):
+            return None
         if ln.needs_grad(x):
             y = ln.forward_act(x.permute(0, 2, 3, 1), "gelu")
             return None if y is None else y.permute(0, 3, 1, 2)
@@ -203,17 +207,30 @@ def _single_layer_norm(module) -> Optional[nn.LayerNorm]:
     return None
 
 
-def _has_hooks(*modules) -> bool:
-    """Hooks see a module's call, so a module that has some is called."""
-    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+def _as_written(module, *classes) -> bool:
+    """Whether a kernel may stand in for the module's call: exactly one of these classes (a subclass may compute something
+    else), with its own `forward`, and without hooks, which see the call -- its own or those of all modules."""
+    return (type(module) in classes and "forward" not in module.__dict__ and not _has_any_global_hook()
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                     or module._backward_pre_hooks))
+
+
+def _fusable_norm(norm_layer, drop_path) -> Optional["LayerNorm"]:
+    """The LayerNorm of a branch's norm layer where the library may run it in one step with the drop path beside it, which
+    then is this file's DropPath or nothing; anything else put in their places is called."""
+    norm = _single_layer_norm(norm_layer)
+    if (torch.is_grad_enabled() and isinstance(norm, LayerNorm) and norm.weight.requires_grad
+            and _as_written(norm, LayerNorm) and _as_written(norm_layer, LayerNorm, nn.Sequential)
+            and _as_written(drop_path, DropPath, nn.Identity)):
+        return norm
+    return None
 
 
 def _post_norm(norm_layer, x, residual, layer_scale, drop_path):
     """residual + drop_path(layer_scale * norm(x)) for the tail of a post-norm branch: one kernel forward and one
     backward in training, the stock operations otherwise."""
-    norm = _single_layer_norm(norm_layer)
-    if (torch.is_grad_enabled() and isinstance(norm, LayerNorm) and norm.weight.requires_grad
-            and not _has_hooks(norm_layer, norm, drop_path)):
+    norm = _fusable_norm(norm_layer, drop_path)
+    if norm is not None:
         out = norm.train_out_dtype(x)
         if (out is not None and residual.dtype == out and residual.shape == x.shape and kernels_apply(residual, layer_scale)
                 and (layer_scale is None or layer_scale.dtype == norm.weight.dtype)):
@@ -225,9 +242,8 @@ def _post_norm(norm_layer, x, residual, layer_scale, drop_path):
 
 def _pre_norm(norm_layer, branch, residual, drop_path):
     """(h, norm(h)) with h = residual + drop_path(branch) for the seam between two pre-norm branches, fused in training."""
-    norm = _single_layer_norm(norm_layer)
-    if (torch.is_grad_enabled() and isinstance(norm, LayerNorm) and norm.weight.requires_grad
-            and not _has_hooks(norm_layer, norm, drop_path)):
+    norm = _fusable_norm(norm_layer, drop_path)
+    if norm is not None:
         out = norm.train_out_dtype(branch)
         if out is not None and residual.dtype == out and residual.shape == branch.shape and kernels_apply(residual):
             scale = drop_path.sample_scale(branch) if isinstance(drop_path, DropPath) else None
