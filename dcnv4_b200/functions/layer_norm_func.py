@@ -2,8 +2,9 @@
 
 The reference composes these from torch.nn.LayerNorm, the layer-scale product, timm's DropPath and residual additions
 (classification/models/flash_intern_image.py:34-56, 414-432).  Each function below is one kernel forward and one
-(plus a small reduction) backward; gradients come out in the dtype of their inputs.  Under `create_graph=True` the
-backward pass is composed of PyTorch operations instead, so second derivatives work as with the stock modules.
+(plus a small reduction) backward; gradients come out in the dtype of their inputs.  Under `create_graph=True`, and for
+gradients that are no plain tensors (batched ones), the backward pass is composed of PyTorch operations instead, so second
+derivatives and vectorised Jacobians work as with the stock modules.
 """
 from __future__ import annotations
 
@@ -14,11 +15,12 @@ from .. import ops
 
 
 def kernels_apply(*tensors) -> bool:
-    """Whether an autograd function over a foreign kernel may take these tensors: not inside a torch.func transform or
-    forward-mode AD, which only the stock operations support."""
-    wrapped = getattr(torch._C, "_functorch", None)
-    is_wrapped = getattr(wrapped, "is_functorch_wrapped_tensor", None)
-    if is_wrapped is not None and any(t is not None and is_wrapped(t) for t in tensors):
+    """Whether an autograd function over a foreign kernel may take these tensors: plain tensors with memory behind them, not
+    subclasses (fake, distributed, masked ones), and nobody who watches or rewrites operations -- a compiler, a tracer, a
+    dispatch mode, a torch.func transform, forward-mode AD, batched gradients -- all of whom only the stock ones support."""
+    if torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() > 0:
+        return False
+    if any(t is not None and not (type(t) in (torch.Tensor, torch.nn.Parameter) and torch._C._has_storage(t)) for t in tensors):
         return False
     return getattr(torch.autograd.forward_ad, "_current_level", -1) < 0
 
@@ -57,7 +59,7 @@ class LayerNormFunction(Function):
     @staticmethod
     def backward(ctx, grad_y):
         x, weight, bias, mean, rstd = ctx.saved_tensors
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or not kernels_apply(grad_y):
             def plain(x_, w_, b_):
                 y = _layer_norm(x_, w_, b_, ctx.eps, grad_y.dtype)
                 return torch.nn.functional.gelu(y) if ctx.activation == "gelu" else y
@@ -81,7 +83,7 @@ class LayerNormResidualFunction(Function):
     @staticmethod
     def backward(ctx, grad_out):
         x, weight, bias, mean, rstd, layer_scale, sample_scale = ctx.saved_tensors
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or not kernels_apply(grad_out):
             def plain(x_, w_, b_, s_):
                 z = _layer_norm(x_, w_, b_, ctx.eps, grad_out.dtype)
                 z = z if s_ is None else z * s_.to(z.dtype)
@@ -113,7 +115,7 @@ class AddLayerNormFunction(Function):
         first, residual, weight, bias, mean, rstd, sample_scale = ctx.saved_tensors
         if grad_h is None and grad_y is None:
             return (None,) * 6
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or not kernels_apply(grad_h, grad_y):
             if not ctx.from_sum:
                 def both(x_, r_, w_, b_):
                     s_ = x_.float() if sample_scale is None else x_.float() * _per_sample(sample_scale, x_)

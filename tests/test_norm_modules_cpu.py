@@ -179,3 +179,40 @@ def test_the_stem_calls_hooked_and_replaced_modules(monkeypatch):
         assert bool(seen) == change.endswith("hook"), change
         if change == "act class":
             torch.testing.assert_close(out, stem.norm2(stem.conv2(torch.zeros(1, 8, 8, 8))).contiguous())
+
+
+# ---- tensors and modes that only the stock operations support ------------------------------------------------
+
+def test_fake_tensors_train_through_the_stock_operation():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        ln = fii.LayerNorm(8, device="cuda")
+        x = torch.empty(4, 8, device="cuda", requires_grad=True)
+        y = ln(x)
+        assert y.shape == (4, 8) and "LayerNorm" in y.grad_fn.name()
+        h, z = fii._pre_norm(ln, x, x, torch.nn.Identity())
+        assert z.shape == h.shape == (4, 8)
+        assert fii._post_norm(ln, x, x, None, torch.nn.Identity()).shape == (4, 8)
+
+
+def test_kernels_decline_what_they_cannot_see_through():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from dcnv4_b200.functions.layer_norm_func import kernels_apply
+
+    class Tagged(torch.Tensor):
+        pass
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = torch.zeros(2, 8)
+    assert kernels_apply(x, None, torch.nn.Parameter(x))
+    assert not kernels_apply(x, x.as_subclass(Tagged))
+    with Watch():
+        assert not kernels_apply(x)
+    seen = []
+    torch.func.vmap(lambda t: seen.append(kernels_apply(t)) or t)(x)
+    torch.jit.trace(lambda t: seen.append(kernels_apply(t)) or t, (x,), check_trace=False)
+    assert not any(seen) and len(seen) >= 2
+    assert kernels_apply(x)

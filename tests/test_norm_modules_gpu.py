@@ -50,3 +50,68 @@ def test_the_stem_trains_its_bias_alone():
     assert out.requires_grad
     out.square().sum().backward()
     assert bias.grad is not None and bias.grad.abs().sum() > 0
+
+
+# ---- what only the stock operations support ------------------------------------------------------------------
+
+def test_compiled_and_traced_modules():
+    """One graph of stock operations, no break at the library's calls."""
+    from dcnv4_b200.flash_intern_image import _post_norm, _pre_norm
+    lib, ref = pair(24)
+    t = torch.randn(6, 24, device=DEV)
+
+    def block(m):
+        def f(x):
+            h, y = _pre_norm(m, x, x, torch.nn.Identity())
+            return _post_norm(m, y, h, None, torch.nn.Identity()) + m(y)
+        return f
+
+    want = torch.autograd.grad(block(ref)(t.requires_grad_()).square().sum(), (t, ref.weight, ref.bias))
+    got = torch.autograd.grad(torch.compile(block(lib), fullgraph=True, backend="eager")(t).square().sum(), (t, lib.weight, lib.bias))
+    for a, b in zip(got, want):        # fp32 sums of 24 and 6 terms, three norms deep
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    graph = make_fx(lambda x: lib(x), tracing_mode="real")(t.detach())
+    assert any("layer_norm" in str(n.target) for n in graph.graph.nodes)
+    other = torch.randn(6, 24, device=DEV)
+    torch.testing.assert_close(graph(other), ref(other), rtol=1e-5, atol=1e-5)
+    traced = torch.jit.trace(lib, (t.detach(),), check_trace=False)
+    assert "layer_norm" in str(traced.inlined_graph)
+
+
+def test_tensor_subclasses_keep_their_class():
+    class Tagged(torch.Tensor):
+        pass
+
+    lib, ref = pair(24)
+    x = torch.randn(5, 24, device=DEV)
+    y = lib(x.as_subclass(Tagged).requires_grad_())
+    assert type(y) is Tagged
+    torch.testing.assert_close(y.as_subclass(torch.Tensor), ref(x), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("which", ["plain", "gelu", "post", "pre", "pre f16"])
+def test_batched_gradients(which):
+    """Several gradients through one backward pass at once (vectorised Jacobians), against one after the other."""
+    from dcnv4_b200 import AddLayerNormFunction, LayerNormFunction, LayerNormResidualFunction
+    g = torch.Generator(device=DEV).manual_seed(4)
+    t = torch.float16 if which == "pre f16" else torch.float32
+    x, r = (torch.randn(4, 3, 20, device=DEV, generator=g).to(t).requires_grad_() for _ in range(2))
+    w, b, gamma = (torch.randn(20, device=DEV, generator=g).requires_grad_() for _ in range(3))
+    s = torch.tensor([1.0, 0.0, 2.0, 1.0], device=DEV)
+    leaves = (x, r, w, b)
+    if which in ("plain", "gelu"):
+        leaves = (x, w, b)
+        outs = (LayerNormFunction.apply(x, w, b, 1e-6, "none" if which == "plain" else "gelu"),)
+    elif which == "post":
+        leaves = (x, r, w, b, gamma)
+        outs = (LayerNormResidualFunction.apply(x, r, w, b, 1e-6, gamma, s),)
+    else:
+        outs = AddLayerNormFunction.apply(x, r, w, b, 1e-6, s)
+    grads = [torch.randn(5, *o.shape, device=DEV, generator=g).to(o.dtype) for o in outs]
+    got = torch.autograd.grad(outs, leaves, grads, is_grads_batched=True, retain_graph=True)
+    for i in range(5):
+        one = torch.autograd.grad(outs, leaves, [v[i] for v in grads], retain_graph=True)
+        for a, e in zip(got, one):
+            # fp32 sums of 20 and 12 terms either way; in fp16 one rounding of each result, 2^-11, on both sides
+            torch.testing.assert_close(a[i], e, rtol=1e-4 if e.dtype == torch.float32 else 2.0 ** -10 + 1e-4, atol=1e-4)
