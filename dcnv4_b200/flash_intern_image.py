@@ -59,7 +59,7 @@ class LayerNorm(nn.LayerNorm):
         if not autocast and self.weight.dtype != x.dtype:
             return None                                   # the stock module refuses mixed types: leave that to it
         out = torch.float32 if autocast else x.dtype
-        return out if ops.layer_norm_train_supported(x if x.is_contiguous() else x.contiguous(), self.weight, out) else None
+        return out if ops.layer_norm_train_covers(x, self.weight, out) else None
 
     def forward_act(self, x, activation="none"):
         """act(self(x)) by the training kernels, or None where they do not apply."""

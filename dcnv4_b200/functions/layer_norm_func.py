@@ -45,13 +45,20 @@ def _differentiable(fn, inputs, grads):
         return [next(got) if t is not None and t.requires_grad else None for t in inputs]
 
 
+# The `apply` of each function makes its inputs contiguous in front of it, in the graph: one copy where one is needed, which
+# both passes read.
+
+
 class LayerNormFunction(Function):
     """y = act(LN(x)): apply(x, weight, bias, eps, activation="none", out_dtype=None)."""
 
+    @classmethod
+    def apply(cls, x, *args):
+        return super().apply(x.contiguous(), *args)
+
     @staticmethod
     def forward(ctx, x, weight, bias, eps, activation="none", out_dtype=None):
-        xc = x.contiguous()
-        y, mean, rstd = ops.layer_norm_train_forward(xc, weight, bias, eps, activation, out_dtype)
+        y, mean, rstd = ops.layer_norm_train_forward(x, weight, bias, eps, activation, out_dtype)
         ctx.eps, ctx.activation = eps, activation
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         return y
@@ -64,7 +71,7 @@ class LayerNormFunction(Function):
                 y = _layer_norm(x_, w_, b_, ctx.eps, grad_y.dtype)
                 return torch.nn.functional.gelu(y) if ctx.activation == "gelu" else y
             return (*_differentiable(plain, (x, weight, bias), (grad_y,)), None, None, None)
-        gx, gw, gb = ops.layer_norm_backward(grad_y.contiguous(), x.contiguous(), mean, rstd, weight, bias, ctx.activation)
+        gx, gw, gb = ops.layer_norm_backward(grad_y.contiguous(), x, mean, rstd, weight, bias, ctx.activation)
         return gx, gw, gb, None, None, None
 
 
@@ -72,10 +79,13 @@ class LayerNormResidualFunction(Function):
     """out = residual + sample_scale * layer_scale * LN(x): apply(x, residual, weight, bias, eps, layer_scale=None,
     sample_scale=None).  `sample_scale` is a constant (a stochastic-depth mask) and gets no gradient."""
 
+    @classmethod
+    def apply(cls, x, residual, *args):
+        return super().apply(x.contiguous(), residual.contiguous(), *args)
+
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, layer_scale=None, sample_scale=None):
-        out, mean, rstd = ops.layer_norm_residual_forward(x.contiguous(), residual.contiguous(), weight, bias, eps,
-                                                          layer_scale, sample_scale)
+        out, mean, rstd = ops.layer_norm_residual_forward(x, residual, weight, bias, eps, layer_scale, sample_scale)
         ctx.eps = eps
         ctx.save_for_backward(x, weight, bias, mean, rstd, layer_scale, sample_scale)
         return out
@@ -90,8 +100,8 @@ class LayerNormResidualFunction(Function):
                 return z if sample_scale is None else z * _per_sample(sample_scale, z).to(z.dtype)
             gx, gw, gb, gs = _differentiable(plain, (x, weight, bias, layer_scale), (grad_out,))
             return gx, grad_out, gw, gb, None, gs, None
-        gx, gw, gb, gs = ops.layer_norm_residual_backward(grad_out.contiguous(), x.contiguous(), mean, rstd, weight, bias,
-                                                          layer_scale, sample_scale)
+        gx, gw, gb, gs = ops.layer_norm_residual_backward(grad_out.contiguous(), x, mean, rstd, weight, bias, layer_scale,
+                                                          sample_scale)
         return gx, grad_out, gw, gb, None, gs, None
 
 
@@ -100,11 +110,14 @@ class AddLayerNormFunction(Function):
     sample_scale=None).  `sample_scale` gets no gradient.  Kept for the backward pass: h where it is float32, and x and
     residual where h has 16 bits, since statistics and y are taken of the sum before it is rounded."""
 
+    @classmethod
+    def apply(cls, x, residual, *args):
+        return super().apply(x.contiguous(), residual.contiguous(), *args)
+
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, sample_scale=None):
         ctx.set_materialize_grads(False)
-        h, y, mean, rstd = ops.add_layer_norm_forward(x.contiguous(), residual.contiguous(), weight, bias, eps,
-                                                      sample_scale)
+        h, y, mean, rstd = ops.add_layer_norm_forward(x, residual, weight, bias, eps, sample_scale)
         ctx.eps, ctx.x_dtype, ctx.from_sum = eps, x.dtype, h.dtype == torch.float32
         kept = (h, None) if ctx.from_sum else (x, residual)
         ctx.save_for_backward(*kept, weight, bias, mean, rstd, sample_scale)
@@ -132,7 +145,6 @@ class AddLayerNormFunction(Function):
                 gr = through if gr is None else gr + through
             gx = (gr if sample_scale is None else gr * _per_sample(sample_scale, gr).to(gr.dtype)).to(ctx.x_dtype)
             return gx, gr, gw, gb, None, None
-        first = first.contiguous()
         grad_y = torch.zeros(first.shape, dtype=grad_h.dtype, device=first.device) if grad_y is None else grad_y.contiguous()
         grad_h = None if grad_h is None else grad_h.contiguous()
         if ctx.from_sum:
@@ -140,5 +152,5 @@ class AddLayerNormFunction(Function):
                                                          ctx.x_dtype)
         else:
             gr, gx, gw, gb = ops.add_layer_norm_backward(grad_y, grad_h, None, mean, rstd, weight, sample_scale, None,
-                                                         first, residual.contiguous())
+                                                         first, residual)
         return gx, gr, gw, gb, None, None

@@ -263,7 +263,12 @@ _LN_PLAIN, _LN_POST, _LN_PRE = 0, 1, 2
 
 def layer_norm_train_supported(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> bool:
     """True when the LayerNorm training passes cover this input (dtypes, size, layout)."""
-    return (x.is_cuda and x.is_contiguous() and x.dtype in _DTYPES and x.dim() > 0
+    return x.is_contiguous() and layer_norm_train_covers(x, weight, out_dtype)
+
+
+def layer_norm_train_covers(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> bool:
+    """`layer_norm_train_supported` of `x.contiguous()`, asked without making the copy."""
+    return (x.is_cuda and x.dtype in _DTYPES and x.dim() > 0
             and 0 < x.shape[-1] <= LAYER_NORM_MAX_CHANNELS and x.numel() // x.shape[-1] <= LAYER_NORM_MAX_ROWS
             and weight is not None and weight.is_cuda and weight.is_contiguous()
             and weight.dtype in (torch.float32, x.dtype) and out_dtype in (None, torch.float32, x.dtype))

@@ -115,3 +115,48 @@ def test_batched_gradients(which):
         for a, e in zip(got, one):
             # fp32 sums of 20 and 12 terms either way; in fp16 one rounding of each result, 2^-11, on both sides
             torch.testing.assert_close(a[i], e, rtol=1e-4 if e.dtype == torch.float32 else 2.0 ** -10 + 1e-4, atol=1e-4)
+
+
+# ---- memory layout -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("which", ["module", "post", "pre", "pre f16"])
+def test_a_strided_input_is_copied_once(which):
+    """One copy in the forward pass, none to ask whether the kernels apply, none in the backward pass."""
+    from dcnv4_b200.flash_intern_image import _post_norm, _pre_norm
+    lib, ref = pair(64)
+    t = torch.float32
+    if which == "pre f16":
+        t = torch.float16
+        lib, ref = lib.half(), ref.half()
+    base = torch.randn(2, 64, 50, device=DEV, dtype=t)
+    grads, copies = [], []
+    for m in (lib, ref):
+        leaf = base.clone().requires_grad_()
+        x = leaf.transpose(1, 2)
+        res = torch.randn(2, 50, 64, device=DEV, dtype=t, generator=torch.Generator(device=DEV).manual_seed(1))
+        with torch.autograd.profiler.profile() as prof:
+            if which == "module":
+                out = (m(x),)
+            elif which == "post":
+                out = (_post_norm(m, x, res, None, torch.nn.Identity()),)
+            else:
+                out = _pre_norm(m, x, res, torch.nn.Identity())
+            (g,) = torch.autograd.grad(out, leaf, [o.detach() for o in out])      # contiguous gradients
+        copies.append(sum(e.name == "aten::clone" for e in prof.function_events))
+        grads.append(g)
+    assert copies[0] == 1
+    # fp32: sums of 64 terms in two orders; fp16: roundings of out, of its gradient and of the stored sum, 2^-11 each,
+    # against values up to a few
+    tol = 1e-4 if t == torch.float32 else 8 * 2.0 ** -11
+    torch.testing.assert_close(grads[0], grads[1], rtol=tol, atol=tol * float(grads[1].abs().max()))
+
+
+def test_second_derivative_through_a_strided_input():
+    lib, ref = pair(24)
+    outs = []
+    base = torch.randn(24, 7, device=DEV)
+    for m in (lib, ref):
+        leaf = base.clone().requires_grad_()
+        (g,) = torch.autograd.grad((m(leaf.t()) ** 3).sum(), leaf, create_graph=True)
+        outs.append(torch.autograd.grad((g ** 2).sum(), leaf)[0])
+    torch.testing.assert_close(outs[0], outs[1], rtol=1e-3, atol=1e-3 * float(outs[1].abs().max()))
