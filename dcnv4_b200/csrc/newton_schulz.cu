@@ -17,6 +17,12 @@
 // bf16 iteration: 2e-1).  In the last two steps nothing is left to amplify: a is folded into B's diagonal and X is hi.
 // The result is returned in bf16, whose own rounding is of the size of that error.
 //
+// fp16 also has a lower end: where eps outweighs |G|, X_0 is as small as their quotient and grows by a factor of a a step.
+// Such a matrix is held as 2^k X, with k from an upper bound of |X| that every step carries on, s <- s (|a| + |b| s^2 +
+// |c| s^4): then 2^k X is below 1 and not below 1/2 times what the bound overestimates.  The products are those of 2^k X;
+// a step's coefficients are b 2^-2k and c 2^-4k, its result is scaled by 2^(k' - k), the last one's by 2^-k.  Powers of two
+// are exact, and with |G| >= eps k is 0 throughout.
+//
 // One persistent kernel runs all products of all steps.  A task is one 128 x BN tile of one product of one matrix; tasks
 // are numbered so that a task only needs earlier ones (step by step, product by product), CTAs take them in that order from
 // a counter, and each matrix counts its finished tiles: a task starts when its matrix has all tiles of the products
@@ -94,7 +100,8 @@ struct NsParams {
   int sym_tiles, upd_tiles;      // tiles of a symmetric product, of an update
   int upd_n;                     // tile columns of an update
   unsigned total;                // tasks
-  float a, b, c;
+  float a;
+  const float4* coef;            // [batch][steps] StepCoef
   unsigned* done;                // [batch] finished tiles
   unsigned* ticket;              // next task
   int* status;
@@ -149,6 +156,47 @@ __host__ __device__ inline int sym_cols(int i, int p) {
   const int c = (i * TM + TM - 1) / BN + 1, most = (p + BN - 1) / BN;
   return c < most ? c : most;
 }
+
+// ---- range of a matrix ----
+constexpr int kMaxScale = 120;       // 2^-120 is a normal number
+// k of 2^k X for |X| <= s; 0 for a zero matrix and for NaN.
+__device__ __forceinline__ int scale_of(float s) {
+  if (!(s > 0.f && s < 0.5f)) return 0;
+  const int k = -(ilogbf(s) + 1);
+  return k < kMaxScale ? k : kMaxScale;
+}
+// What a step works with: B = b A + c A A of the scaled matrix, its result times `post`.
+struct StepCoef { float b, c, post; };
+// Coefficients of a step; s bounds |X| before and after it, k is the scale before and after it.
+__device__ __forceinline__ StepCoef step_coef(float a, float b, float c, float& s, int& k, bool last) {
+  const float s2 = s * s;
+  s *= fabsf(a) + s2 * (fabsf(b) + s2 * fabsf(c));
+  const int next = last ? 0 : scale_of(s);
+  StepCoef r{b, c, 1.f};
+  if (k != 0 || next != 0) { r.b = ldexpf(b, -2 * k); r.c = ldexpf(c, -4 * k); r.post = ldexpf(1.f, next - k); }
+  k = next;
+  return r;
+}
+// 2^k X_0 from x and the sum of its squares.  The factor need not be a normal fp32 number (|x| beyond 1e38, or below 1e-38
+// with a small eps): such a matrix is scaled in 64 bits.
+struct Scaling {
+  float s, factor;
+  int k;
+  double exact;
+  bool wide;
+  __device__ Scaling(double sum, float eps) {
+    const double norm = sqrt(sum), by = norm + (double)eps;
+    exact = 1.0 / by;
+    s = (float)(norm * exact);
+    k = scale_of(s);
+    if (k != 0) exact = ldexp(exact, k);
+    factor = (float)exact;
+    wide = !(factor >= 1.1754944e-38f && factor <= 1.7e38f);
+  }
+  template <bool WIDE> __device__ __forceinline__ float operator()(float x) const {
+    return WIDE ? (float)((double)x * exact) : x * factor;
+  }
+};
 
 struct Task { int step, kind, bi, mt, nt; };
 // Task order.  CTAs take tasks in order, so a task whose matrix is not ready holds up its CTA: the distance between a
@@ -520,6 +568,7 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
       const int row0 = q.mt * TM + (half ? (int)rank * 64 + (quad & 1) * 32 : (int)rank * kBM + quad * 32);
       const int first = group * (half ? kCols / 2 : kCols);
       const int colw = q.nt * BN + first + (half ? (quad >> 1) * (BN / 2) : 0);
+      const float4 cf = kind == kGram ? make_float4(0.f, 0.f, 1.f, 0.f) : p.coef[(long long)q.bi * p.steps + q.step];   // b, c, post
       const bool rows_in = row0 < rows;                  // else this warp's quarter lies below the matrix
       // make the staging buffer free and ask for the unit of the previous X or A that unit `u` needs
       auto fetch = [&](int u) {
@@ -568,8 +617,8 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 f = unpack_h(rr[e]);
-              x[2 * e] = fmaf(p.c, x[2 * e], p.b * f.x);
-              x[2 * e + 1] = fmaf(p.c, x[2 * e + 1], p.b * f.y);
+              x[2 * e] = fmaf(cf.y, x[2 * e], cf.x * f.x);
+              x[2 * e + 1] = fmaf(cf.y, x[2 * e + 1], cf.x * f.y);
             }
             if (row0 + lane >= col0 + j && row0 + lane < col0 + j + 8) {
 #pragma unroll
@@ -587,6 +636,10 @@ ns_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams 
               x[2 * e] = fmaf(p.a, fmaf(g.x, 1.f / kLoScale, f.x), x[2 * e]);
               x[2 * e + 1] = fmaf(p.a, fmaf(g.y, 1.f / kLoScale, f.y), x[2 * e + 1]);
             }
+          }
+          if (kind == kUpdate) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= cf.z;
           }
           uint32_t o[4];
           if (bf16) {
@@ -753,22 +806,31 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallP
   __syncthreads();
   sum = 0.0;
   for (int i = 0; i < kSmallThreads / 32; ++i) sum += part[i];
-  const float inv = (float)(1.0 / (sqrt(sum) + (double)p.eps));
+  const Scaling scaling(sum, p.eps);
+  float bound = scaling.s;
+  int k = scaling.k;
   for (int c0 = xc0; c0 < xc1; c0 += 32) {
     uint32_t v[32];
     float f[32];
     tmem_ld_32x32(tx + (uint32_t)c0, v);
     tmem_ld_wait();
+    if (scaling.wide) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) { f[j] = __uint_as_float(v[j]) * inv; v[j] = __float_as_uint(f[j]); }
+      for (int j = 0; j < 32; ++j) f[j] = scaling.operator()<true>(__uint_as_float(v[j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = scaling.operator()<false>(__uint_as_float(v[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(f[j]);
     tmem_st_32x32(tx + (uint32_t)c0, v);
     put_row(sx, row, c0, f);
   }
   tmem_st_wait();
 
   uint32_t phase = 0;
-  // every thread's operand writes are visible, the product runs, every thread sees the accumulator
-  auto product = [&](const unsigned char* ma, const unsigned char* mb, bool b_mn, int n, int k) {
+  // every thread's operand writes are visible, the product runs ...
+  auto begin = [&](const unsigned char* ma, const unsigned char* mb, bool b_mn, int n, int k) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
@@ -785,13 +847,19 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallP
       tc_commit(&bar);
     }
     __syncwarp();
+  };
+  // ... and every thread sees the accumulator
+  auto finish = [&] {
     if (!mbar_wait_bounded(&bar, phase)) atomicExch(p.status, kStatusStageTimeout);
     phase ^= 1;
     tc_fence_after();
   };
+  auto product = [&](const unsigned char* ma, const unsigned char* mb, bool b_mn, int n, int k) { begin(ma, mb, b_mn, n, k); finish(); };
   for (int step = 0; step < p.steps; ++step) {
     const bool pair = step < p.keep, last = step == p.steps - 1;
-    product(sx, sx, false, n_gram, n_upd);                       // A = X X^T
+    begin(sx, sx, false, n_gram, n_upd);                         // A = X X^T
+    const StepCoef cf = step_coef(p.a, p.b, p.c, bound, k, last);
+    finish();
     for (int c0 = ac0; c0 < ac1; c0 += 32) {
       uint32_t v[32];
       float f[32];
@@ -815,7 +883,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallP
         for (int e = 0; e < 8; ++e) {
           const float2 h = unpack_h(rr[e >> 1]);
           const bool in = row < p.p && c0 + j + e < p.p;
-          f[j + e] = in ? fmaf(p.c, __uint_as_float(v[j + e]), p.b * (e & 1 ? h.y : h.x)) : 0.f;
+          f[j + e] = in ? fmaf(cf.c, __uint_as_float(v[j + e]), cf.b * (e & 1 ? h.y : h.x)) : 0.f;
           if (!pair && in && row == c0 + j + e) f[j + e] += p.a;
         }
       }
@@ -832,6 +900,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallP
       for (int j = 0; j < 32; ++j) {
         f[j] = row < p.p && c0 + j < p.q ? __uint_as_float(v[j]) : 0.f;
         if (pair) f[j] = row < p.p && c0 + j < p.q ? fmaf(p.a, __uint_as_float(w[j]), f[j]) : 0.f;
+      }
+      if (cf.post != 1.f) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] *= cf.post;
       }
       if (last) {
         __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (long long)blockIdx.x * p.m * p.n;
@@ -861,6 +933,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const SmallP
 
 constexpr int kNormThreads = 256;
 constexpr int kMaxChunks = 64;   // partial sums of squares of one matrix
+constexpr int kMaxSteps = 100;   // the entry point's limit: the workspace has room for the coefficients of so many
 
 template <typename T> __device__ __forceinline__ float load1(const T* p) { return to_f32(*p); }
 
@@ -903,23 +976,10 @@ ns_square_kernel(const T* __restrict__ x, double* __restrict__ partial, long lon
   }
 }
 
-// X_0 = x / (norm + eps) as the fp16 pair, rows padded to `ld` elements (the padding is never read).
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads)
-ns_scale_kernel(const T* __restrict__ x, const double* __restrict__ partial, __half* __restrict__ hi,
-                __half* __restrict__ lo, int rows, int cols, int ld, int n_chunks, float eps, int vec) {
-  pdl_trigger();
-  pdl_wait();
-  const int bi = blockIdx.y;
-  // every warp adds the partial sums for itself: one thread's chain of loads would hold up the block
-  double t = 0.0;
-  for (int i = threadIdx.x & 31; i < n_chunks; i += 32) t += partial[(long long)bi * kMaxChunks + i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  const float inv = (float)(1.0 / (sqrt(t) + (double)eps));
-  const T* src = x + (long long)bi * rows * cols;
-  __half* dh = hi + (long long)bi * rows * ld;
-  __half* dl = lo + (long long)bi * rows * ld;
+// One matrix' share of a block: 2^k X_0 as the fp16 pair, rows padded to `ld` elements (the padding is never read).
+template <bool WIDE, typename T>
+__device__ __forceinline__ void scale_matrix(const T* __restrict__ src, __half* __restrict__ dh, __half* __restrict__ dl,
+                                             int rows, int cols, int ld, const Scaling& scaling, int vec) {
   const long long stride = (long long)gridDim.x * kNormThreads;
   if (vec) {   // whole matrix in vectors of 8: rows are contiguous (cols == ld)
     const long long n8 = (long long)rows * cols / 8;
@@ -936,7 +996,7 @@ ns_scale_kernel(const T* __restrict__ x, const double* __restrict__ partial, __h
       uint32_t h[4], l[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x0 = v[2 * e] * inv, x1 = v[2 * e + 1] * inv;
+        const float x0 = scaling.template operator()<WIDE>(v[2 * e]), x1 = scaling.template operator()<WIDE>(v[2 * e + 1]);
         h[e] = pack_h(x0, x1);
         const float2 f = unpack_h(h[e]);
         l[e] = pack_h((x0 - f.x) * kLoScale, (x1 - f.y) * kLoScale);
@@ -949,10 +1009,39 @@ ns_scale_kernel(const T* __restrict__ x, const double* __restrict__ partial, __h
     for (long long i = (long long)blockIdx.x * kNormThreads + threadIdx.x; i < total; i += stride) {
       const long long r = i / cols;
       const int c = (int)(i - r * cols);
-      const float v = load1(src + i) * inv;
+      const float v = scaling.template operator()<WIDE>(load1(src + i));
       const __half h = __float2half_rn(v);
       dh[r * ld + c] = h;
       dl[r * ld + c] = __float2half_rn((v - __half2float(h)) * kLoScale);
+    }
+  }
+}
+// 2^k X_0 of every matrix, and the coefficients of its steps.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+ns_scale_kernel(const T* __restrict__ x, const double* __restrict__ partial, __half* __restrict__ hi,
+                __half* __restrict__ lo, float4* __restrict__ coef, int rows, int cols, int ld, int n_chunks, int steps,
+                float a, float b, float c, float eps, int vec) {
+  pdl_trigger();
+  pdl_wait();
+  const int bi = blockIdx.y;
+  // every warp adds the partial sums for itself: one thread's chain of loads would hold up the block
+  double t = 0.0;
+  for (int i = threadIdx.x & 31; i < n_chunks; i += 32) t += partial[(long long)bi * kMaxChunks + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const Scaling scaling(t, eps);
+  const T* src = x + (long long)bi * rows * cols;
+  __half* dh = hi + (long long)bi * rows * ld;
+  __half* dl = lo + (long long)bi * rows * ld;
+  if (scaling.wide) scale_matrix<true>(src, dh, dl, rows, cols, ld, scaling, vec);
+  else scale_matrix<false>(src, dh, dl, rows, cols, ld, scaling, vec);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    float s = scaling.s;
+    int k = scaling.k;
+    for (int i = 0; i < steps; ++i) {
+      const StepCoef cf = step_coef(a, b, c, s, k, i == steps - 1);
+      coef[(long long)bi * steps + i] = make_float4(cf.b, cf.c, cf.post, 0.f);
     }
   }
 }
@@ -989,7 +1078,7 @@ inline long long pad8(long long v) { return (v + 7) / 8 * 8; }
 inline size_t pad1k(size_t v) { return (v + 1023) / 1024 * 1024; }
 
 struct Layout {
-  size_t x[2], l[2], a, b, norm, done, ticket, total;
+  size_t x[2], l[2], a, b, norm, coef, done, ticket, total;
   int ldn, ldp;
 };
 Layout layout_of(long long batch, int m, int n) {
@@ -1004,6 +1093,7 @@ Layout layout_of(long long batch, int m, int n) {
   w.a = at; at += ab;
   w.b = at; at += ab;
   w.norm = at; at += pad1k((size_t)batch * kMaxChunks * sizeof(double));
+  w.coef = at; at += pad1k((size_t)batch * kMaxSteps * sizeof(float4));
   w.ticket = at;                   // 8 bytes, the per-matrix counts behind them
   w.done = at + 8; at += pad1k(8 + (size_t)batch * sizeof(unsigned));
   w.total = at;
@@ -1054,8 +1144,8 @@ cudaError_t launch_ns(const NsMaps& maps, NsParams p, int sms, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t prepare(const void* x, const Layout& w, unsigned char* ws, long long batch, int m, int n, float eps,
-                    int sms, cudaStream_t s) {
+cudaError_t prepare(const void* x, const Layout& w, unsigned char* ws, long long batch, int m, int n, int steps, float a,
+                    float b, float c, float eps, int sms, cudaStream_t s) {
   const long long per = (long long)m * n;
   const bool vec = n % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   // slices of a matrix: enough to fill the GPU, each a whole number of vector rounds
@@ -1076,7 +1166,8 @@ cudaError_t prepare(const void* x, const Layout& w, unsigned char* ws, long long
   if (blocks > most) blocks = most;
   return launch_overlapped(ns_scale_kernel<T>, dim3((unsigned)blocks, (unsigned)batch), dim3(kNormThreads), 0, s, src,
                            (const double*)partial, reinterpret_cast<__half*>(ws + w.x[0]),
-                           reinterpret_cast<__half*>(ws + w.l[0]), m, n, w.ldn, (int)chunks, eps, (int)vec);
+                           reinterpret_cast<__half*>(ws + w.l[0]), reinterpret_cast<float4*>(ws + w.coef), m, n, w.ldn,
+                           (int)chunks, steps, a, b, c, eps, (int)vec);
 }
 
 bool small(int m, int n) { return (m < n ? m : n) <= kSmallP && (m < n ? n : m) <= kSmallQ; }
@@ -1119,9 +1210,9 @@ cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* work
   }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const Layout w = layout_of(batch, m, n);
-  cudaError_t e = dtype == 0   ? prepare<float>(x, w, ws, batch, m, n, eps, sms, s)
-                  : dtype == 1 ? prepare<__half>(x, w, ws, batch, m, n, eps, sms, s)
-                               : prepare<__nv_bfloat16>(x, w, ws, batch, m, n, eps, sms, s);
+  cudaError_t e = dtype == 0   ? prepare<float>(x, w, ws, batch, m, n, steps, a, b, c, eps, sms, s)
+                  : dtype == 1 ? prepare<__half>(x, w, ws, batch, m, n, steps, a, b, c, eps, sms, s)
+                               : prepare<__nv_bfloat16>(x, w, ws, batch, m, n, steps, a, b, c, eps, sms, s);
   if (e != cudaSuccess) return e;
   const bool direct = n % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   NsParams p = {};
@@ -1129,7 +1220,8 @@ cudaError_t launch_newton_schulz(int dtype, const void* x, void* out, void* work
   p.p = p.tall ? n : m; p.q = p.tall ? m : n;
   p.steps = steps; p.keep = steps - 2;
   p.batch = (int)batch;
-  p.a = a; p.b = b; p.c = c;
+  p.a = a;
+  p.coef = reinterpret_cast<const float4*>(ws + w.coef);
   p.done = reinterpret_cast<unsigned*>(ws + w.done);
   p.ticket = reinterpret_cast<unsigned*>(ws + w.ticket);
   p.status = status;

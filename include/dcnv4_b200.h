@@ -250,7 +250,8 @@ int dcnv4b200_add_layernorm_bwd(const void* grad_y, const void* grad_h, const vo
  *              overlap on the GPU; NULL where that is 0 (matrices of at most 128 x 256, either way round)
  * m, n <= 65536, batch <= 65535, 1 <= steps <= 100 (DCNV4B200_ERR_UNSUPPORTED / _ERR_SHAPE otherwise).  The iteration
  * runs on fp16 tensor-core products with fp32 accumulation, with X carried in 22 bits until the last two steps; the
- * coefficients must keep |X| within fp16's range, as those of the published iteration do.  A zero matrix gives zeros,
+ * coefficients must keep |X| within fp16's range, as those of the published iteration do.  From below that range is no
+ * limit: a matrix that eps outweighs is carried with a power of two of its own.  A zero matrix gives zeros,
  * a matrix with a NaN gives NaN, other matrices of the stack are not affected.  Results repeat bit for bit.
  */
 size_t dcnv4b200_newton_schulz_workspace_bytes(long long batch, int m, int n);
