@@ -71,3 +71,69 @@ def test_matrices_of_one_stack_have_ranges_of_their_own(batch, m, n):
     assert not y[2].any()
     cubic = (1.5, -0.5, 0.0)
     check(ops.newton_schulz(x * scale, 12, cubic)[keep], ref((x * scale)[keep], 12, cubic), REL * 12 / 5)
+
+
+# ---- every form with every option ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("batch,m,n", SIZES, ids=IDS)
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 10])
+def test_steps_and_coefficients(batch, m, n, steps):
+    """Results that end in either buffer, with and without steps that carry the pair, both iterations."""
+    from dcnv4_b200 import ops
+    x = momentum(batch, m, n)
+    rel = REL * max(1, steps / 5)
+    check(ops.newton_schulz(x, steps), ref(x, steps), rel)
+    cubic = (1.5, -0.5, 0.0)
+    check(ops.newton_schulz(x, steps, cubic), ref(x, steps, cubic), rel)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("batch,m,n", SIZES, ids=IDS)
+def test_magnitudes_and_special_values(batch, m, n):
+    from dcnv4_b200 import ops
+    base = momentum(batch, m, n)
+    for scale in (1e-3, 1e12, 1e25):
+        check(ops.newton_schulz(base * scale), ref(base * scale))
+    x = momentum(max(batch, 4), m, n)
+    x[1] = 0
+    x[2, 3, 5] = float("nan")
+    y = ops.newton_schulz(x)
+    assert not y[1].any() and y[2].isnan().all()
+    keep = [i for i in range(len(x)) if i not in (1, 2)]
+    check(y[keep], ref(x[keep]))
+    x[2, 3, 5] = float("inf")
+    y = ops.newton_schulz(x)
+    assert not y[2].isfinite().any() and not y[1].any()
+    check(y[keep], ref(x[keep]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("batch,m,n", SIZES + [(9, 1030, 1032)], ids=IDS + ["pairs of whole vectors"])
+def test_unaligned_tensors(batch, m, n, dtype):
+    """x one element into its storage, and an out that 16-byte stores cannot address, by the C entry point; the elements
+    around out keep their values."""
+    from dcnv4_b200 import _lib, ops
+    x = momentum(batch, m, n, dtype)
+    want = ops.newton_schulz(x)
+    flat = torch.empty(x.numel() + 1, device=DEV, dtype=dtype)
+    view = flat[1:].view(x.shape).copy_(x)
+    assert torch.equal(ops.newton_schulz(view), want)
+    L = _lib.lib()
+    need = L.dcnv4b200_newton_schulz_workspace_bytes(batch, m, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    guard = torch.full((x.numel() + 130,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = guard[65:65 + x.numel()]
+    a, b, c = ops.NEWTON_SCHULZ_COEFFICIENTS
+    assert L.dcnv4b200_newton_schulz(x.data_ptr(), out.data_ptr(), ws.data_ptr(), need, {torch.float32: 0, torch.bfloat16: 2}[dtype],
+                                     batch, m, n, 5, a, b, c, 1e-7, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out.view(x.shape), want)
+    assert (guard[:65] == 7).all() and (guard[65 + x.numel():] == 7).all()
+
+
+@pytest.mark.parametrize("m,n", [(1, 65536), (65536, 3), (40, 65535), (300, 65536), (129, 8)])
+def test_long_and_thin(m, n):
+    from dcnv4_b200 import ops
+    from tests.test_newton_schulz_gpu import allowed
+    x = momentum(1, m, n)
+    check(ops.newton_schulz(x), ref(x), allowed(x))
+    assert ops.device_status() == 0
