@@ -291,6 +291,8 @@ def _check_ln(x, x_dtype, weight, bias, others, layer_scale, sample_scale, out_d
         raise RuntimeError("the result must have the dtype of the input or be float32")
     if C == 0:
         raise RuntimeError("the last dimension must not be empty")
+    if C > LAYER_NORM_MAX_CHANNELS:          # before it becomes a C int
+        raise ValueError(f"at most {LAYER_NORM_MAX_CHANNELS} channels, got {C}")
     for t, n in ((weight, "weight"), (bias, "bias"), (layer_scale, "layer_scale")):
         if t is not None and (t.numel() != C or t.dtype != weight.dtype):
             raise RuntimeError(f"{n} must have the size of the last dimension and the dtype of weight")
@@ -469,6 +471,8 @@ def add_layer_norm_backward(grad_y: torch.Tensor, grad_h: Optional[torch.Tensor]
                         h.dtype if x_dtype is None else x_dtype, "add_layer_norm_backward")[:4]
 
 
+NEWTON_SCHULZ_MAX_SIDE = 65536
+NEWTON_SCHULZ_MAX_STEPS = 100
 NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # the quintic published with the Muon optimiser
 
 
@@ -477,13 +481,16 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     """Orthogonalise a matrix or a stack of matrices (..., m, n) by the quintic Newton-Schulz iteration:
     X = x / (|x|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T.  Contiguous CUDA tensor in
     float32 / float16 / bfloat16; the result is a new bfloat16 tensor (its rounding is of the size of the
-    iteration's own error).  No autograd.  Deterministic."""
+    iteration's own error).  Sides up to 65536, 1 to 100 steps.  No autograd.  Deterministic."""
     _check_tensor(x, "input")
     if x.dim() < 2:
         raise RuntimeError("input must be a matrix or a stack of matrices (..., m, n)")
     a, b, c = (float(v) for v in coefficients)
     code = _code(x)
     m, n = x.shape[-2:]
+    if max(m, n) > NEWTON_SCHULZ_MAX_SIDE or steps > NEWTON_SCHULZ_MAX_STEPS:          # before they become C ints
+        raise ValueError(f"matrices of up to {NEWTON_SCHULZ_MAX_SIDE} rows and columns and {NEWTON_SCHULZ_MAX_STEPS} steps, got "
+                         f"{m} x {n}, {steps} steps")
     out = x.new_empty(x.shape, dtype=torch.bfloat16)
     if out.numel() == 0:
         return out
