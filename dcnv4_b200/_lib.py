@@ -7,13 +7,24 @@ made without a CUDA tensor, an exception is raised.  Build the library with
 from __future__ import annotations
 
 import ctypes as C
+import importlib.metadata
 import importlib.util
 import os
+import sys
 import threading
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_C", "libdcnv4_b200.so")
-BINDINGS_PATH = os.path.join(HERE, "_C", "dcnv4_b200_bindings.so")
+
+
+
+def bindings_path() -> str:
+    """The binding links against PyTorch's C++ libraries, so its file is named after the PyTorch and Python it was built for."""
+    tag = f"{importlib.metadata.version('torch')}-{sys.implementation.cache_tag}"
+    return os.path.join(HERE, "_C", f"dcnv4_b200_bindings-{tag}.so")
+
+
 ABI_VERSION = 1
 
 F32, F16, BF16 = 0, 1, 2
@@ -89,21 +100,37 @@ def lib() -> C.CDLL:
 _bindings = None
 
 
+class NoBindings:
+    """Stands for a binding that is not there: declines every call, which then takes the Python route into the same
+    kernels."""
+
+    @staticmethod
+    def ln_forward(*args):
+        return None
+
+    ln_backward = ln_forward
+
+
 def bindings():
-    """The binding of the latency-critical entry points (csrc/bindings.cpp), handed the library's functions."""
+    """The binding of the latency-critical entry points (csrc/bindings.cpp), handed the library's functions.  It saves host
+    time and nothing else: without one for the running PyTorch, `NoBindings` and a warning."""
     global _bindings
     handle = lib()
     with _lock:
         if _bindings is None:
-            if not os.path.exists(BINDINGS_PATH):
-                raise LibraryError(f"{BINDINGS_PATH} not found: run `python -m dcnv4_b200.build`")
-            spec = importlib.util.spec_from_file_location("dcnv4_b200_bindings", BINDINGS_PATH)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
-            module.init(*(C.cast(fn, C.c_void_p).value for fn in (
-                handle.dcnv4b200_layernorm_train_fwd, handle.dcnv4b200_layernorm_train_bwd,
-                handle.dcnv4b200_layernorm_train_bwd_workspace_bytes, handle.dcnv4b200_add_layernorm_bwd)))
-            _bindings = module
+            path = bindings_path()
+            try:
+                spec = importlib.util.spec_from_file_location("dcnv4_b200_bindings", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.init(*(C.cast(fn, C.c_void_p).value for fn in (
+                    handle.dcnv4b200_layernorm_train_fwd, handle.dcnv4b200_layernorm_train_bwd,
+                    handle.dcnv4b200_layernorm_train_bwd_workspace_bytes, handle.dcnv4b200_add_layernorm_bwd)))
+                _bindings = module
+            except (ImportError, OSError, TypeError) as e:
+                warnings.warn(f"{path} cannot be used ({e}): LayerNorm calls of the training passes spend 13 to 19 us instead of "
+                              "6 to 9 on the host; run `python -m dcnv4_b200.build`", RuntimeWarning, stacklevel=2)
+                _bindings = NoBindings
     return _bindings
 
 

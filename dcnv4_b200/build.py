@@ -1,5 +1,5 @@
 """Build the CUDA library in-tree, dcnv4_b200/csrc/*.cu -> dcnv4_b200/_C/libdcnv4_b200.so, and the Python binding of its
-latency-critical entry points, dcnv4_b200/csrc/bindings.cpp -> dcnv4_b200/_C/dcnv4_b200_bindings.so.
+latency-critical entry points, dcnv4_b200/csrc/bindings.cpp -> dcnv4_b200/_C/dcnv4_b200_bindings-<PyTorch and Python>.so.
 
     python -m dcnv4_b200.build [--force] [--verbose]
 
@@ -17,11 +17,12 @@ import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
+from ._lib import bindings_path
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_C")
 LIB = os.path.join(OUT_DIR, "libdcnv4_b200.so")
-BINDINGS = os.path.join(OUT_DIR, "dcnv4_b200_bindings.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ("api.cu", "dcnv4_fwd.cu", "dcnv4_bwd.cu", "dcnv4_bwd_tiled.cu", "dcnv4_fwd_tiled.cu", "dcnv4_fwd_fused.cu", "fda_fwd.cu", "fda_bwd.cu", "aux.cu", "layernorm.cu",
@@ -46,12 +47,15 @@ def _build_bindings(nvcc: str) -> None:
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-I", sysconfig.get_paths()["include"], "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-I", cuda, os.path.join(CSRC, "bindings.cpp"), "-o", BINDINGS, "-L", os.path.join(torch_dir, "lib"),
+           "-I", cuda, os.path.join(CSRC, "bindings.cpp"), "-o", bindings_path(), "-L", os.path.join(torch_dir, "lib"),
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("g++ failed on bindings.cpp")
+    for f in os.listdir(OUT_DIR):          # those of other PyTorch versions are out of date with the sources by now
+        if f.startswith("dcnv4_b200_bindings") and os.path.join(OUT_DIR, f) != bindings_path():
+            os.remove(os.path.join(OUT_DIR, f))
 
 
 def _deps_mtime() -> float:
@@ -60,7 +64,7 @@ def _deps_mtime() -> float:
 
 
 def is_current() -> bool:
-    return all(os.path.exists(f) and os.path.getmtime(f) >= _deps_mtime() for f in (LIB, BINDINGS))
+    return all(os.path.exists(f) and os.path.getmtime(f) >= _deps_mtime() for f in (LIB, bindings_path()))
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -83,7 +87,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         bindings = ex.submit(_build_bindings, nvcc)
         objs = list(ex.map(compile_one, SOURCES))
-        bindings.result()
     link = [nvcc, *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs]
     r = subprocess.run(link, capture_output=True, text=True)
     if r.returncode != 0:
@@ -91,6 +94,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError("nvcc link failed")
     for obj in objs:          # every source is recompiled on any change: the objects are of no further use
         os.remove(obj)
+    bindings.result()         # the library stands without it, but its failure is one of the build
     return LIB
 
 
