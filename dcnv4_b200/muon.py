@@ -28,15 +28,21 @@ _STACK_ELEMENTS = 2 ** 28     # of one orthogonalisation call: 3 GB of workspace
 
 def split_parameters(model: torch.nn.Module) -> Tuple[List[torch.nn.Parameter], List[torch.nn.Parameter]]:
     """(matrices, others): the weights of Linear and of ordinary (not depth-wise) convolution layers, except a classifier
-    `head`, and everything else, each parameter once."""
+    `head` and what Muon has no room for, and everything else, each parameter once."""
     matrices, seen = [], set()
     for name, m in model.named_modules():
         linear = isinstance(m, torch.nn.Linear) and name.split(".")[-1] != "head"
         conv = isinstance(m, torch.nn.Conv2d) and m.groups == 1
-        if (linear or conv) and m.weight.requires_grad and id(m.weight) not in seen:
+        if ((linear or conv) and m.weight.requires_grad and id(m.weight) not in seen
+                and max(_matrix(m.weight)) <= ops.NEWTON_SCHULZ_MAX_SIDE):
             seen.add(id(m.weight))
             matrices.append(m.weight)
     return matrices, [p for p in model.parameters() if p.requires_grad and id(p) not in seen]
+
+
+def _matrix(p: torch.Tensor) -> Tuple[int, int]:
+    """Rows and columns of a weight as a matrix: the outputs, and all inputs of one."""
+    return p.shape[0], p.numel() // max(p.shape[0], 1)
 
 
 class Muon(torch.optim.Optimizer):
@@ -46,19 +52,39 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params: Iterable, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, ns_coefficients=ops.NEWTON_SCHULZ_COEFFICIENTS, eps: float = 1e-7,
                  ns_steps: int = 5, adjust_lr: str = "match_rms_adamw"):
-        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
+        defaults = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                        ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps, adjust_lr=adjust_lr)
+        self._check(dict(defaults, params=[]))
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check(group):
+        """What the constructor and `add_param_group` refuse: a group's options and its parameters."""
+        if group["lr"] < 0 or group["weight_decay"] < 0 or not 0 <= group["momentum"] < 1:
             raise ValueError("lr and weight_decay must not be negative, momentum must lie in [0, 1)")
-        if not 1 <= ns_steps <= 100:
-            raise ValueError("ns_steps must lie between 1 and 100")
-        if adjust_lr not in ("match_rms_adamw", "original"):
+        if not 1 <= group["ns_steps"] <= ops.NEWTON_SCHULZ_MAX_STEPS:
+            raise ValueError(f"ns_steps must lie between 1 and {ops.NEWTON_SCHULZ_MAX_STEPS}")
+        if group["adjust_lr"] not in ("match_rms_adamw", "original"):
             raise ValueError("adjust_lr must be 'match_rms_adamw' or 'original'")
-        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
-                                      ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps,
-                                      adjust_lr=adjust_lr))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError("Muon is for weight matrices: give vectors to another optimiser (split_parameters)")
+        if len(tuple(group["ns_coefficients"])) != 3:
+            raise ValueError("ns_coefficients are three numbers (a, b, c)")
+        for p in group["params"]:
+            if p.dim() < 2:
+                raise ValueError("Muon is for weight matrices: give vectors to another optimiser (split_parameters)")
+            if p.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                raise ValueError(f"Muon takes float32, float16 and bfloat16 parameters, got {p.dtype}")
+            if max(_matrix(p)) > ops.NEWTON_SCHULZ_MAX_SIDE:
+                raise ValueError(f"a weight of {tuple(p.shape)} has a side above {ops.NEWTON_SCHULZ_MAX_SIDE}: give it to another "
+                                 "optimiser")
+
+    @torch._disable_dynamo
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            self._check(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
         """As every optimiser's, but the momentum stays in float32: the base class casts state to the parameter's type."""
@@ -78,13 +104,17 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:                # refusals come before anything has been updated
+            for p in group["params"]:
+                if p.grad is not None and p.grad.is_sparse:
+                    raise RuntimeError("Muon does not take sparse gradients")
+                if p.grad is not None and not p.is_cuda:
+                    raise RuntimeError("Muon: parameter must be a CUDA tensor")
         for group in self.param_groups:
             stacks = {}
             for p in group["params"]:
                 if p.grad is not None:
-                    if p.grad.is_sparse:
-                        raise RuntimeError("Muon does not take sparse gradients")
-                    stacks.setdefault((p.shape[0], p.numel() // max(p.shape[0], 1), p.dtype, p.device), []).append(p)
+                    stacks.setdefault((*_matrix(p), p.dtype, p.device), []).append(p)
             for (rows, cols, _, _), params in stacks.items():
                 if rows * cols == 0:
                     continue
