@@ -20,11 +20,11 @@
 //
 // All of them are bound by memory: a few operations per element, each tensor read and written once.  Rows are contiguous,
 // so a tile of rows is one span per tensor, and a ring of such tiles is kept in flight with bulk copies (cp.async.bulk,
-// mbarriers, bounded waits) while the CTA's 8 or 16 warps compute: the bytes in flight do not depend on how many
+// mbarriers, bounded waits) while the CTA's 12 or 16 warps compute: the bytes in flight do not depend on how many
 // registers a row takes.  A span only has to start on 16 bytes, so rows of any width use the ring; with a width that no
 // vector divides, teams keep to rows that start at the same distance from a vector boundary.
 //
-// A row belongs to a team of `lpr` lanes: 2..32 lanes of a warp, or all computing warps of the CTA.  A lane keeps its
+// A row belongs to a team of `lpr` lanes: 2..32 lanes of a warp, or 2..16 whole warps.  A lane keeps its
 // NV vectors of the row, its slice of the parameters and of A and B in registers; statistics and sums are fp32, two
 // passes over registers (mean, then squared deviations), two elements per instruction (fma.rn.f32x2).  Nothing is
 // accumulated with atomics: the order of every sum is fixed by the sizes alone, so results repeat bit for bit.
@@ -61,7 +61,7 @@ struct LnTrainArgs {
   void* db;
   void* dgamma;
   int rows, C;
-  int lpr;               // lanes of a team (32 * warps when a row takes the whole CTA)
+  int lpr;               // lanes of a team
   int param_f32;         // parameters are fp32 (else: the type TP of the instantiation)
   unsigned rows_per_sample;
   unsigned long long per_mul;  // row / rows_per_sample == (row * per_mul) >> per_shift for row < 2^31
@@ -81,43 +81,16 @@ namespace ln {
 constexpr int kMaxChannels = 8192;
 constexpr int kSms = 148;              // B200: fixes the grid, hence the order of sums and the workspace size
 
-// One lane's vector of N elements as raw words; N * sizeof(T) is 16 or 32 bytes, or N is 1.
-template <typename T, int N> struct Words { uint32_t r[(N * sizeof(T) + 3) / 4]; };
-
-template <typename T, int N>
-__device__ __forceinline__ void load(Words<T, N>& v, const T* p, bool ok) {
-  if constexpr (N == 1) {
-    if constexpr (sizeof(T) == 4) v.r[0] = ok ? __float_as_uint(__ldg((const float*)p)) : 0u;
-    else v.r[0] = ok ? (uint32_t)__ldg((const unsigned short*)p) : 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < (int)(N * sizeof(T)) / 16; ++i) {
-      uint4 t = make_uint4(0u, 0u, 0u, 0u);
-      if (ok) t = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      v.r[4 * i] = t.x; v.r[4 * i + 1] = t.y; v.r[4 * i + 2] = t.z; v.r[4 * i + 3] = t.w;
-    }
-  }
+// One element, or 0 where there is none; the word is widened when it is used, so that a row's loads go out together.
+template <typename T>
+__device__ __forceinline__ uint32_t load(const T* p, bool ok) {
+  if constexpr (sizeof(T) == 4) return ok ? __float_as_uint(__ldg((const float*)p)) : 0u;
+  else return ok ? (uint32_t)__ldg((const unsigned short*)p) : 0u;
 }
-template <typename T, int N>
-__device__ __forceinline__ void to_floats(const Words<T, N>& v, float (&f)[N]) {
-  if constexpr (N == 1) {
-    if constexpr (sizeof(T) == 4) f[0] = __uint_as_float(v.r[0]);
-    else { const unsigned short u = (unsigned short)v.r[0]; f[0] = to_f32(*reinterpret_cast<const T*>(&u)); }
-  } else {
-    widen(v.r, f, (const T*)nullptr);
-  }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store(T* p, const float (&f)[N]) {
-  if constexpr (N == 1) {
-    *p = from_f32<T>(f[0]);
-  } else {
-    uint32_t r[N * sizeof(T) / 4];
-    narrow(f, r, (const T*)nullptr);
-#pragma unroll
-    for (int i = 0; i < (int)(N * sizeof(T)) / 16; ++i)
-      reinterpret_cast<uint4*>(p)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-  }
+template <typename T>
+__device__ __forceinline__ float as_float(uint32_t r) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r);
+  else { const unsigned short u = (unsigned short)r; return to_f32(*reinterpret_cast<const T*>(&u)); }
 }
 
 // Parameters are fp32 or the 16-bit type P; read once per launch.
@@ -827,7 +800,7 @@ ln_ring_bwd_kernel(const LnTrainArgs a) {
 
 // ------------------------------------------------------------------------- element-wise kernels
 
-template <typename TX, typename TY, int VEC, int NV, int MODE, bool GELU>
+template <typename TX, typename TY, int NV, int MODE, bool GELU>
 __global__ void __launch_bounds__(512)
 ln_train_fwd_kernel(const LnTrainArgs a) {
   using P = TX;
@@ -842,77 +815,61 @@ ln_train_fwd_kernel(const LnTrainArgs a) {
   pdl_trigger();
   pdl_wait();
 
-  float w[NV][VEC], b[NV][VEC];
+  float w[NV], b[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int c = (sub + v * lpr) * VEC + e;
-      const bool ok = c < C;
-      w[v][e] = ok ? param<P>(a.w, c, a.param_f32) : 0.f;
-      b[v][e] = ok ? param<P>(a.b, c, a.param_f32) : 0.f;
-      if (MODE == kPost && a.gamma != nullptr) {
-        const float g = ok ? param<P>(a.gamma, c, a.param_f32) : 0.f;
-        w[v][e] *= g;
-        b[v][e] *= g;
-      }
+  for (int v = 0; v < NV; ++v) {
+    const int c = sub + v * lpr;
+    const bool ok = c < C;
+    w[v] = ok ? param<P>(a.w, c, a.param_f32) : 0.f;
+    b[v] = ok ? param<P>(a.b, c, a.param_f32) : 0.f;
+    if (MODE == kPost && a.gamma != nullptr) {
+      const float g = ok ? param<P>(a.gamma, c, a.param_f32) : 0.f;
+      w[v] *= g;
+      b[v] *= g;
     }
+  }
   // the lanes of a warp stay in the loop together: the team sums shuffle across it
-  const int row_step = n_teams;
-  for (int r0 = wide ? team0 : team0 - (int)(threadIdx.x & 31) / lpr; r0 < a.rows; r0 += row_step) {
+  for (int r0 = wide ? team0 : team0 - (int)(threadIdx.x & 31) / lpr; r0 < a.rows; r0 += n_teams) {
     const int row = wide ? r0 : r0 + (int)(threadIdx.x & 31) / lpr;
     const bool live = row < a.rows;
     const long long base = (long long)row * C;
-    Words<TX, VEC> rx[NV];
-    Words<TY, VEC> rr[MODE == kPlain ? 1 : NV];
+    uint32_t rx[NV], rr[MODE == kPlain ? 1 : NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (sub + v * lpr) * VEC;
-      load<TX, VEC>(rx[v], static_cast<const TX*>(a.x) + base + c, live && c < C);
-      if (MODE != kPlain) load<TY, VEC>(rr[v], static_cast<const TY*>(a.res) + base + c, live && c < C);
+      const int c = sub + v * lpr;
+      rx[v] = load(static_cast<const TX*>(a.x) + base + c, live && c < C);
+      if (MODE != kPlain) rr[v] = load(static_cast<const TY*>(a.res) + base + c, live && c < C);
     }
     float s = 1.f;
     if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
-    float xv[NV][VEC];
+    float xv[NV];
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      to_floats<TX, VEC>(rx[v], xv[v]);
+      const int c = sub + v * lpr;
+      xv[v] = as_float<TX>(rx[v]);
       if (MODE == kPre) {
-        float rv[VEC];
-        to_floats<TY, VEC>(rr[v], rv);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) xv[v][e] = fmaf(s, xv[v][e], rv[e]);
-        const int c = (sub + v * lpr) * VEC;
-        if (live && c < C) store<TY, VEC>(static_cast<TY*>(a.h) + base + c, xv[v]);
+        xv[v] = fmaf(s, xv[v], as_float<TY>(rr[v]));
+        if (live && c < C) static_cast<TY*>(a.h)[base + c] = from_f32<TY>(xv[v]);
       }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) sum += xv[v][e];
+      sum += xv[v];
     }
     const float mean = team_sum(sum, 0.f, lpr, red, flip).x * inv_c;
     float sq = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if ((sub + v * lpr) * VEC < C) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { const float d = xv[v][e] - mean; sq = fmaf(d, d, sq); }
-      }
+      if (sub + v * lpr < C) { const float d = xv[v] - mean; sq = fmaf(d, d, sq); }
     const float rstd = rsqrtf(team_sum(sq, 0.f, lpr, red, flip).x * inv_c + a.eps);
     if (!live) continue;
     if (sub == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (sub + v * lpr) * VEC;
+      const int c = sub + v * lpr;
       if (c >= C) continue;
-      float o[VEC], rv[VEC];
-      if (MODE == kPost) to_floats<TY, VEC>(rr[v], rv);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        o[e] = fmaf((xv[v][e] - mean) * rstd, w[v][e], b[v][e]);
-        if (GELU) { float2 cdf, density; normal(both(o[e]), cdf, density); o[e] *= cdf.x; }
-        if (MODE == kPost) o[e] = fmaf(s, o[e], rv[e]);
-      }
-      store<TY, VEC>(static_cast<TY*>(a.y) + base + c, o);
+      float o = fmaf((xv[v] - mean) * rstd, w[v], b[v]);
+      if (GELU) { float2 cdf, density; normal(both(o), cdf, density); o *= cdf.x; }
+      if (MODE == kPost) o = fmaf(s, o, as_float<TY>(rr[v]));
+      static_cast<TY*>(a.y)[base + c] = from_f32<TY>(o);
     }
   }
 }
@@ -921,7 +878,7 @@ ln_train_fwd_kernel(const LnTrainArgs a) {
 
 // TL: type of the normalised tensor and of its gradient; TG: type of the incoming gradients; T2: type of the branch
 // gradient of `pre`; P: parameter type when not fp32.
-template <typename TL, typename TG, typename T2, typename P, int VEC, int NV, int MODE, bool GELU>
+template <typename TL, typename TG, typename T2, typename P, int NV, int MODE, bool GELU>
 __global__ void __launch_bounds__(512)
 ln_train_bwd_kernel(const LnTrainArgs a) {
   __shared__ float2 red[2][16];
@@ -939,148 +896,114 @@ ln_train_bwd_kernel(const LnTrainArgs a) {
   pdl_trigger();
   pdl_wait();
 
-  float w[NV][VEC], b[GELU ? NV : 1][VEC], sa[NV][VEC], sb[NV][VEC];
+  float w[NV], b[GELU ? NV : 1], sa[NV], sb[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int c = (sub + v * lpr) * VEC + e;
-      const bool ok = c < C;
-      w[v][e] = ok ? param<P>(a.w, c, a.param_f32) : 0.f;
-      if (GELU) b[v][e] = ok ? param<P>(a.b, c, a.param_f32) : 0.f;
-      if (MODE == kPost && a.gamma != nullptr && ok) w[v][e] *= param<P>(a.gamma, c, a.param_f32);
-      sa[v][e] = 0.f;
-      sb[v][e] = 0.f;
-    }
+  for (int v = 0; v < NV; ++v) {
+    const int c = sub + v * lpr;
+    const bool ok = c < C;
+    w[v] = ok ? param<P>(a.w, c, a.param_f32) : 0.f;
+    if (GELU) b[v] = ok ? param<P>(a.b, c, a.param_f32) : 0.f;
+    if (MODE == kPost && a.gamma != nullptr && ok) w[v] *= param<P>(a.gamma, c, a.param_f32);
+    sa[v] = 0.f;
+    sb[v] = 0.f;
+  }
   for (int r0 = wide ? team0 : team0 - lane / lpr; r0 < a.rows; r0 += n_teams) {
     const int row = wide ? r0 : r0 + lane / lpr;
     const bool live = row < a.rows;
     const long long base = (long long)row * C;
-    Words<TL, VEC> rx[NV], rr[kNarrow ? NV : 1];
-    Words<TG, VEC> rg[NV], rh[MODE == kPre ? NV : 1];
+    uint32_t rx[NV], rr[kNarrow ? NV : 1], rg[NV], rh[MODE == kPre ? NV : 1];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (sub + v * lpr) * VEC;
+      const int c = sub + v * lpr;
       const bool ok = live && c < C;
-      load<TL, VEC>(rx[v], static_cast<const TL*>(MODE == kPre && !summed ? a.h : a.x) + base + c, ok);
-      if (kNarrow) load<TL, VEC>(rr[v], static_cast<const TL*>(a.res) + base + c, ok && summed);
-      load<TG, VEC>(rg[v], static_cast<const TG*>(a.gy) + base + c, ok);
-      if (MODE == kPre) load<TG, VEC>(rh[v], static_cast<const TG*>(a.gh) + base + c, ok && a.gh != nullptr);
+      rx[v] = load(static_cast<const TL*>(MODE == kPre && !summed ? a.h : a.x) + base + c, ok);
+      if (kNarrow) rr[v] = load(static_cast<const TL*>(a.res) + base + c, ok && summed);
+      rg[v] = load(static_cast<const TG*>(a.gy) + base + c, ok);
+      if (MODE == kPre) rh[v] = load(static_cast<const TG*>(a.gh) + base + c, ok && a.gh != nullptr);
     }
     float mean = live ? __ldg(a.mean + row) : 0.f, rstd = live ? __ldg(a.rstd + row) : 0.f;
     float s = 1.f;
     if (MODE != kPlain && a.s != nullptr) s = live ? __ldg(a.s + sample_of(a, (unsigned)row)) : 0.f;
-    float xh[NV][VEC], gw[NV][VEC];
+    float xh[NV], gw[NV];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      to_floats<TL, VEC>(rx[v], xh[v]);
-      if (kNarrow && summed) {
-        float rv[VEC];
-        to_floats<TL, VEC>(rr[v], rv);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) xh[v][e] = fmaf(s, xh[v][e], rv[e]);
-      }
+      xh[v] = as_float<TL>(rx[v]);
+      if (kNarrow && summed) xh[v] = fmaf(s, xh[v], as_float<TL>(rr[v]));
     }
     if (kNarrow && !summed) {
       float sum = 0.f, sq = 0.f;
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += xh[v][e];
+      for (int v = 0; v < NV; ++v) sum += xh[v];
       mean = team_sum(sum, 0.f, lpr, red, flip).x * inv_c;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if ((sub + v * lpr) * VEC < C) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) { const float d = xh[v][e] - mean; sq = fmaf(d, d, sq); }
-        }
+        if (sub + v * lpr < C) { const float d = xh[v] - mean; sq = fmaf(d, d, sq); }
       rstd = fminf(rstd, rsqrtf(team_sum(sq, 0.f, lpr, red, flip).x * inv_c));
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float g[VEC];
-      to_floats<TG, VEC>(rg[v], g);
-      const bool ok = live && (sub + v * lpr) * VEC < C;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        xh[v][e] = ok ? (xh[v][e] - mean) * rstd : 0.f;
-        if (MODE == kPost) g[e] *= s;
-        if (GELU) {
-          const float z = fmaf(xh[v][e], w[v][e], b[v][e]);
-          float2 cdf, density;
-          normal(both(z), cdf, density);
-          g[e] *= fmaf(z, density.x, cdf.x);
-        }
-        sa[v][e] = fmaf(g[e], xh[v][e], sa[v][e]);
-        sb[v][e] += g[e];
-        gw[v][e] = g[e] * w[v][e];
-        s1 += gw[v][e];
-        s2 = fmaf(gw[v][e], xh[v][e], s2);
+      float g = as_float<TG>(rg[v]);
+      xh[v] = live && sub + v * lpr < C ? (xh[v] - mean) * rstd : 0.f;
+      if (MODE == kPost) g *= s;
+      if (GELU) {
+        const float z = fmaf(xh[v], w[v], b[v]);
+        float2 cdf, density;
+        normal(both(z), cdf, density);
+        g *= fmaf(z, density.x, cdf.x);
       }
+      sa[v] = fmaf(g, xh[v], sa[v]);
+      sb[v] += g;
+      gw[v] = g * w[v];
+      s1 += gw[v];
+      s2 = fmaf(gw[v], xh[v], s2);
     }
     const float2 t = team_sum(s1, s2, lpr, red, flip);
     const float m1 = t.x * inv_c, m2 = t.y * inv_c;
     if (!live) continue;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (sub + v * lpr) * VEC;
+      const int c = sub + v * lpr;
       if (c >= C) continue;
-      float o[VEC], hv[VEC];
-      if (MODE == kPre) to_floats<TG, VEC>(rh[v], hv);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        o[e] = rstd * (gw[v][e] - fmaf(xh[v][e], m2, m1));
-        if (MODE == kPre) o[e] += hv[e];
-      }
-      store<TL, VEC>(static_cast<TL*>(a.dx) + base + c, o);
-      if (MODE == kPre && a.dx2 != nullptr) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] *= s;
-        store<T2, VEC>(static_cast<T2*>(a.dx2) + base + c, o);
-      }
+      float o = rstd * (gw[v] - fmaf(xh[v], m2, m1));
+      if (MODE == kPre) o += as_float<TG>(rh[v]);
+      static_cast<TL*>(a.dx)[base + c] = from_f32<TL>(o);
+      if (MODE == kPre && a.dx2 != nullptr) static_cast<T2*>(a.dx2)[base + c] = from_f32<T2>(o * s);
     }
   }
 
   // this CTA's sums: over the teams of each warp by shuffles, then warp after warp into shared memory
-  if (!wide) {
-    for (int o = lpr; o < 32; o <<= 1) {
+  float* dst = a.partial + (size_t)blockIdx.x * 2 * C;
+  if (wide) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          sa[v][e] += __shfl_xor_sync(0xffffffffu, sa[v][e], o);
-          sb[v][e] += __shfl_xor_sync(0xffffffffu, sb[v][e], o);
-        }
+    for (int v = 0; v < NV; ++v) {
+      const int c = sub + v * lpr;
+      if (c < C) { dst[c] = sa[v]; dst[C + c] = sb[v]; }
     }
-    const int n_warps = blockDim.x >> 5;
-    for (int q = 0; q < n_warps; ++q) {
-      if ((int)(threadIdx.x >> 5) == q && lane < lpr) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int c = (sub + v * lpr) * VEC + e;
-            if (c < C) {
-              acc_smem[c] = (q ? acc_smem[c] : 0.f) + sa[v][e];
-              acc_smem[C + c] = (q ? acc_smem[C + c] : 0.f) + sb[v][e];
-            }
-          }
-      }
-      __syncthreads();
-    }
-    float* dst = a.partial + (size_t)blockIdx.x * 2 * C;
-    for (int i = threadIdx.x; i < 2 * C; i += blockDim.x) dst[i] = acc_smem[i];
-  } else {
-    float* dst = a.partial + (size_t)blockIdx.x * 2 * C;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int c = (sub + v * lpr) * VEC + e;
-        if (c < C) { dst[c] = sa[v][e]; dst[C + c] = sb[v][e]; }
-      }
+    return;
   }
+  for (int o = lpr; o < 32; o <<= 1) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      sa[v] += __shfl_xor_sync(0xffffffffu, sa[v], o);
+      sb[v] += __shfl_xor_sync(0xffffffffu, sb[v], o);
+    }
+  }
+  const int n_warps = blockDim.x >> 5;
+  for (int q = 0; q < n_warps; ++q) {
+    if ((int)(threadIdx.x >> 5) == q && lane < lpr) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = sub + v * lpr;
+        if (c < C) {
+          acc_smem[c] = (q ? acc_smem[c] : 0.f) + sa[v];
+          acc_smem[C + c] = (q ? acc_smem[C + c] : 0.f) + sb[v];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 2 * C; i += blockDim.x) dst[i] = acc_smem[i];
 }
 
 // --------------------------------------------------------------------------------- dispatch
@@ -1244,16 +1167,16 @@ template <typename TX, typename TY, int NV>
 cudaError_t direct_run(bool backward, int mode, int act, const LnTrainArgs& a, const Plan& p, cudaStream_t s) {
   const dim3 g((unsigned)p.grid), t((unsigned)(p.g.lpr > 32 ? p.g.lpr : kDirectThreads));
   if (!backward) {
-    if (mode == kPost) return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPost, false>, g, t, 0, s, a);
-    if (mode == kPre) return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPre, false>, g, t, 0, s, a);
-    if (act) return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPlain, true>, g, t, 0, s, a);
-    return launch_overlapped(ln_train_fwd_kernel<TX, TY, 1, NV, kPlain, false>, g, t, 0, s, a);
+    if (mode == kPost) return launch_overlapped(ln_train_fwd_kernel<TX, TY, NV, kPost, false>, g, t, 0, s, a);
+    if (mode == kPre) return launch_overlapped(ln_train_fwd_kernel<TX, TY, NV, kPre, false>, g, t, 0, s, a);
+    if (act) return launch_overlapped(ln_train_fwd_kernel<TX, TY, NV, kPlain, true>, g, t, 0, s, a);
+    return launch_overlapped(ln_train_fwd_kernel<TX, TY, NV, kPlain, false>, g, t, 0, s, a);
   }
   const size_t smem = a.lpr > 32 ? 0 : (size_t)2 * a.C * sizeof(float);
-  if (mode == kPre) return launch_overlapped(ln_train_bwd_kernel<TY, TY, TX, TX, 1, NV, kPre, false>, g, t, smem, s, a);
-  if (mode == kPost) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, 1, NV, kPost, false>, g, t, smem, s, a);
-  if (act) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, 1, NV, kPlain, true>, g, t, smem, s, a);
-  return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, 1, NV, kPlain, false>, g, t, smem, s, a);
+  if (mode == kPre) return launch_overlapped(ln_train_bwd_kernel<TY, TY, TX, TX, NV, kPre, false>, g, t, smem, s, a);
+  if (mode == kPost) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, NV, kPost, false>, g, t, smem, s, a);
+  if (act) return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, NV, kPlain, true>, g, t, smem, s, a);
+  return launch_overlapped(ln_train_bwd_kernel<TX, TY, TX, TX, NV, kPlain, false>, g, t, smem, s, a);
 }
 
 template <typename TX, typename TY>
