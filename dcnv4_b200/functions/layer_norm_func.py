@@ -38,8 +38,10 @@ def _differentiable(fn, inputs, grads):
     with torch.enable_grad():
         out = fn(*inputs)
         out = out if isinstance(out, tuple) else (out,)
-        pairs = [(o, g) for o, g in zip(out, grads) if g is not None]
+        pairs = [(o, g) for o, g in zip(out, grads) if g is not None and o.requires_grad]
         wanted = [t for t in inputs if t is not None and t.requires_grad]
+        if not pairs or not wanted:          # what was asked for does not go through fn
+            return [None] * len(inputs)
         got = iter(torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs], create_graph=True,
                                        allow_unused=True))
         return [next(got) if t is not None and t.requires_grad else None for t in inputs]

@@ -160,3 +160,27 @@ def test_second_derivative_through_a_strided_input():
         (g,) = torch.autograd.grad((m(leaf.t()) ** 3).sum(), leaf, create_graph=True)
         outs.append(torch.autograd.grad((g ** 2).sum(), leaf)[0])
     torch.testing.assert_close(outs[0], outs[1], rtol=1e-3, atol=1e-3 * float(outs[1].abs().max()))
+
+
+@pytest.mark.parametrize("which", ["post, residual alone", "pre, weight alone and h", "pre f16, weight alone and h", "pre f16, residual alone"])
+def test_differentiable_gradients_of_some_inputs_only(which):
+    """create_graph=True where the wanted gradient does not go through the norm."""
+    from dcnv4_b200 import AddLayerNormFunction, LayerNormResidualFunction
+    g = torch.Generator(device=DEV).manual_seed(8)
+    t = torch.float16 if "f16" in which else torch.float32
+    x, r = (torch.randn(4, 16, device=DEV, generator=g).to(t) for _ in range(2))
+    w, b = (torch.randn(16, device=DEV, generator=g) for _ in range(2))
+    v = torch.randn(4, 16, device=DEV, generator=g).to(t)
+    leaf = (r if "residual" in which else w).requires_grad_()
+    if which.startswith("post"):
+        out = LayerNormResidualFunction.apply(x, r, w, b, 1e-6)
+        (got,) = torch.autograd.grad(out, leaf, v, create_graph=True)
+        assert torch.equal(got, v)
+    elif "weight" in which:
+        h, y = AddLayerNormFunction.apply(x, r, w, b, 1e-6)
+        (got,) = torch.autograd.grad(h, leaf, v, create_graph=True, allow_unused=True)
+        assert got is None or not got.any()
+    else:
+        h, y = AddLayerNormFunction.apply(x, r, w, b, 1e-6)
+        (got,) = torch.autograd.grad(h, leaf, v, create_graph=True)
+        assert torch.equal(got, v)
