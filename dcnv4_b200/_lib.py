@@ -7,7 +7,6 @@ made without a CUDA tensor, an exception is raised.  Build the library with
 from __future__ import annotations
 
 import ctypes as C
-import importlib.metadata
 import importlib.util
 import os
 import sys
@@ -16,15 +15,6 @@ import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_C", "libdcnv4_b200.so")
-
-
-
-def bindings_path() -> str:
-    """The binding links against PyTorch's C++ libraries, so its file is named after the PyTorch and Python it was built for."""
-    tag = f"{importlib.metadata.version('torch')}-{sys.implementation.cache_tag}"
-    return os.path.join(HERE, "_C", f"dcnv4_b200_bindings-{tag}.so")
-
-
 ABI_VERSION = 1
 
 F32, F16, BF16 = 0, 1, 2
@@ -95,6 +85,13 @@ def lib() -> C.CDLL:
                 raise LibraryError(f"ABI mismatch: library {got}, python {ABI_VERSION}; rebuild the library")
             _lib = handle
     return _lib
+
+
+def bindings_path() -> str:
+    """The binding links against PyTorch's C++ libraries, so its file is named after the PyTorch and Python it was built for."""
+    import torch
+    tag = f"{torch.__version__}-{sys.implementation.cache_tag}"
+    return os.path.join(HERE, "_C", f"dcnv4_b200_bindings-{tag}.so")
 
 
 _bindings = None

@@ -92,7 +92,8 @@ class DCNv4(nn.Module):
 
     def _blend_fusable(self, x, x_proj) -> bool:
         w = self.center_feature_scale_proj_weight
-        return (not ops.needs_grad(x, x_proj, w, self.center_feature_scale_proj_bias) and not torch.is_autocast_enabled() and x.dtype == x_proj.dtype
+        return (not ops.needs_grad(x, x_proj, w, self.center_feature_scale_proj_bias)
+                and not torch.is_autocast_enabled() and x.dtype == x_proj.dtype
                 and self.center_feature_scale_proj_bias.dtype == w.dtype
                 and ops.center_scale_blend_supported(x, w, self.group_channels))
 

@@ -672,7 +672,8 @@ class PairedLinear:
 
     def usable(self, x: torch.Tensor) -> bool:
         a, b = self.first, self.second
-        return (FUSED_LINEAR and not needs_grad(x, a.weight, b.weight, a.bias, b.bias) and not torch.is_autocast_enabled() and linear_supported(x, a.weight)
+        return (FUSED_LINEAR and not needs_grad(x, a.weight, b.weight, a.bias, b.bias)
+                and not torch.is_autocast_enabled() and linear_supported(x, a.weight)
                 and b.weight.dtype == x.dtype and b.weight.is_cuda and a.in_features == b.in_features
                 and a.in_features <= FUSED_LINEAR_MAX_K and a.out_features % 64 == 0 and b.out_features % 8 == 0
                 and (a.bias is None) == (b.bias is None) and (a.bias is None or a.bias.dtype == x.dtype))
@@ -738,15 +739,16 @@ def linear_module_forward(x: torch.Tensor, lin: "torch.nn.Linear", residual: Opt
     output features) the pair `(y, norm(y))`.  One fused tensor-core kernel when autograd is not
     needed and the kernel covers the input, else the stock PyTorch operations (same result up
     to fp rounding: the fused kernel rounds at the same points)."""
-    fused = (FUSED_LINEAR and not needs_grad(x, lin.weight, lin.bias, residual) and not torch.is_autocast_enabled() and linear_supported(x, lin.weight)
-             and lin.in_features <= FUSED_LINEAR_MAX_K
+    fused = (FUSED_LINEAR and not needs_grad(x, lin.weight, lin.bias, residual)
+             and not torch.is_autocast_enabled() and linear_supported(x, lin.weight) and lin.in_features <= FUSED_LINEAR_MAX_K
              and (lin.bias is None or (lin.bias.dtype == x.dtype and lin.bias.data_ptr() % 16 == 0))
              and (residual is None or (residual.dtype == x.dtype and residual.is_contiguous()
                                        and residual.data_ptr() % 16 == 0)))
     # The LayerNorm epilogue needs a whole row in one tile, i.e. one tile per 128 rows: with row
     # tiles for fewer than half of the SMs the separate kernels (narrower tiles, more CTAs) are
     # faster (measured on FlashInternImage-T stage 3: 98 tiles fused wins, 49 tiles it loses).
-    if (fused and norm is not None and activation == "none" and not needs_grad(norm.weight, norm.bias) and _norm_fusable(norm, lin.out_features, x.dtype)
+    if (fused and norm is not None and activation == "none" and not needs_grad(norm.weight, norm.bias)
+            and _norm_fusable(norm, lin.out_features, x.dtype)
             and x.numel() // lin.in_features >= LN_FUSION_MIN_ROWS_PER_SM * _sm_count(x.device)):
         return linear_layer_norm_forward(x, lin.weight, lin.bias, residual, norm.weight, norm.bias, norm.eps)
     if fused:
@@ -802,7 +804,8 @@ def conv2d_bias_act(x: torch.Tensor, conv: "torch.nn.Conv2d", activation: str = 
     bf16 the bias and the activation are applied in place by one pass over the convolution's
     output instead of PyTorch's separate broadcast addition and activation kernels."""
     F = torch.nn.functional
-    if (FUSED_LINEAR and not needs_grad(x, conv.weight, conv.bias) and not torch.is_autocast_enabled() and x.is_cuda and conv.bias is not None
+    if (FUSED_LINEAR and not needs_grad(x, conv.weight, conv.bias) and not torch.is_autocast_enabled()
+            and x.is_cuda and conv.bias is not None
             and x.dtype in (torch.float16, torch.bfloat16) and conv.weight.dtype == x.dtype
             and conv.bias.dtype == x.dtype and conv.out_channels % 8 == 0 and conv.padding_mode == "zeros"
             and conv.bias.data_ptr() % 16 == 0):

@@ -17,7 +17,7 @@ def test_the_binding_is_found_by_its_pytorch(monkeypatch):
     import torch
     assert torch.__version__.split("+")[0] in os.path.basename(_lib.bindings_path())
     assert os.path.exists(_lib.bindings_path()) and build.is_current()
-    monkeypatch.setattr(_lib.importlib.metadata, "version", lambda name: "1.0.0+other")
+    monkeypatch.setattr(torch, "__version__", "1.0.0+other")
     assert not os.path.exists(_lib.bindings_path()) and not build.is_current()
 
 
